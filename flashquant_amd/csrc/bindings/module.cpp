@@ -10,6 +10,7 @@ PYBIND11_MODULE(_C, m) {
     m.doc() = "TurboQuant KV-cache kernels for MI355X (gfx950)";
     m.attr("abi_version") = fq_abi_version();
     bind_kernels(m);
+    bind_paged_kv(m);
     bind_codebook(m);
     bind_quantizer(m);
     bind_quantizer_classes(m);

@@ -1,0 +1,158 @@
+// Pages, slots and positions of a step's new tokens, from the requests' lengths: the inputs of every paged entry point, made on
+// the GPU.
+//
+// Request r holds context_r tokens and brings query_r new ones.  Its pages are the first ceil(context / B) entries of its row of the
+// block table; a page that its new tokens begin is taken from the list of free ones, in the order of requests and tokens:
+//   new_r = ceil((context_r + query_r) / B) - ceil(context_r / B),  page i of them = free[start + sum_{s < r} new_s + i].
+// What bounds it: nothing but latency (16 bytes a token; lengths, then free pages or the block table, then the stores: three trips
+// to memory).  So it is one launch of independent workgroups: each adds up all lengths for itself, keeps the requests that reach
+// into its 256 tokens in LDS, and a thread then finds the request of its token as the last one that begins at or before it.
+// A new page has a first token, which is new too: its thread writes the page into the block table.  What a thread reads there are
+// pages from before, so nothing that one workgroup writes is read by another.
+#include "fq_common.hpp"
+
+namespace fq {
+
+constexpr int kScheduleThreads = 256;
+
+struct ScheduleParams {
+    const int32_t* context;
+    const int32_t* query;
+    int32_t* table;
+    const int32_t* free_blocks;
+    const int32_t* free_start;      // may be null: 0
+    int32_t* free_end;
+    int64_t* slots;
+    int64_t* positions;
+    int32_t* seq_lens;
+    int32_t* cu;
+    int64_t table_row;
+    int64_t num_tokens;
+    int S, max_blocks, num_free, page_log2;
+};
+
+// inclusive sums over the workgroup of two values; `sum` gets those of all threads
+__device__ __forceinline__ int2 sums_upto(int2 v, int2 (&waves)[kScheduleThreads / kWave], int2& sum) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int x = __shfl_up(v.x, d, kWave), y = __shfl_up(v.y, d, kWave);
+        v.x += lane >= d ? x : 0;
+        v.y += lane >= d ? y : 0;
+    }
+    __syncthreads();                // the sums of the time before have been read
+    if (lane == kWave - 1) waves[wave] = v;
+    __syncthreads();
+    sum = int2{0, 0};
+#pragma unroll
+    for (int w = 0; w < kScheduleThreads / kWave; ++w) {
+        if (w < wave) { v.x += waves[w].x; v.y += waves[w].y; }
+        sum.x += waves[w].x;
+        sum.y += waves[w].y;
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(kScheduleThreads) void paged_schedule_kernel(const ScheduleParams p) {
+    __shared__ int2 waves[kScheduleThreads / kWave];
+    __shared__ int owner[kScheduleThreads], owner_cu[kScheduleThreads], owner_context[kScheduleThreads], owner_page[kScheduleThreads];
+    __shared__ int wave_last[kScheduleThreads / kWave];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int64_t lo = int64_t(blockIdx.x) * kScheduleThreads, hi = lo + kScheduleThreads;
+    const int page = 1 << p.page_log2;
+    const int64_t room = int64_t(p.max_blocks) << p.page_log2;
+    owner[tid] = -1;
+    const int start = p.free_start != nullptr ? p.free_start[0] : 0;
+    int2 before = {0, 0};           // tokens and pages of the requests so far
+    for (int s = 0; s < p.S; s += kScheduleThreads) {
+        const int r = s + tid;
+        int context = 0, query = 0;
+        if (r < p.S) {
+            context = p.context[r] > 0 ? p.context[r] : 0;
+            query = p.query[r] > 0 ? p.query[r] : 0;
+        }
+        const int64_t had = context < room ? context : room;
+        const int64_t has = int64_t(context) + query < room ? int64_t(context) + query : room;
+        const int2 mine = {query, int((has + page - 1) >> p.page_log2) - int((had + page - 1) >> p.page_log2)};
+        int2 all;
+        const int2 upto = sums_upto(mine, waves, all);       // (its barriers also lie between the clearing of `owner` and what follows)
+        const int64_t cu = int64_t(before.x) + upto.x - query;
+        if (query > 0 && cu < hi && cu + query > lo) {       // of the tokens [lo, hi)
+            const int at = int(cu > lo ? cu - lo : 0);
+            owner[at] = r;
+            owner_cu[at] = int(cu);
+            owner_context[at] = context;
+            owner_page[at] = before.y + upto.y - mine.y;
+        }
+        if (blockIdx.x == 0 && r < p.S) {
+            p.seq_lens[r] = int(has);
+            p.cu[r + 1] = before.x + upto.x;
+        }
+        before.x += all.x;
+        before.y += all.y;
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        p.cu[0] = 0;
+        p.free_end[0] = start + before.y;
+    }
+    __syncthreads();
+    // the last request that begins at or before this thread's token
+    const uint64_t begins = __ballot(owner[tid] >= 0);
+    if (lane == 0) wave_last[wave] = begins != 0 ? wave * kWave + 63 - __clzll(static_cast<long long>(begins)) : -1;
+    __syncthreads();
+    const int64_t token = lo + tid;
+    if (token >= p.num_tokens) return;
+    const uint64_t mine = begins & (~uint64_t(0) >> (63 - lane));
+    int at = mine != 0 ? wave * kWave + 63 - __clzll(static_cast<long long>(mine)) : -1;
+    for (int w = wave - 1; at < 0 && w >= 0; --w) at = wave_last[w];
+    if (token >= before.x || at < 0) {                       // behind the last new token
+        p.slots[token] = -1;
+        p.positions[token] = 0;
+        return;
+    }
+    const int context = owner_context[at];
+    const int64_t position = context + (token - owner_cu[at]);
+    int64_t slot = -1;
+    if (position < room) {
+        const int b = int(position >> p.page_log2), in_page = int(position & (page - 1));
+        const int held = int((int64_t(context) + page - 1) >> p.page_log2);
+        int32_t* entry = p.table + int64_t(owner[at]) * p.table_row + b;
+        int block;
+        if (b < held) {
+            block = *entry;
+        } else {
+            const int64_t i = int64_t(start) + owner_page[at] + (b - held);
+            block = i >= 0 && i < p.num_free ? p.free_blocks[i] : -1;
+            if (in_page == 0) *entry = block;
+        }
+        if (block >= 0) slot = (int64_t(block) << p.page_log2) + in_page;
+    }
+    p.slots[token] = slot;
+    p.positions[token] = position;
+}
+
+}  // namespace fq
+
+extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
+                                 const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
+                                 int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
+                                 int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream) {
+    if (num_reqs < 0 || num_tokens < 0 || num_tokens > 0x7fffffffLL || max_blocks_per_seq <= 0 || num_free < 0 || num_free > 0x7fffffffLL ||
+        block_table_stride < max_blocks_per_seq)
+        return FQ_ERR_BAD_SHAPE;
+    if (block_size != 8 && block_size != 16 && block_size != 32) return FQ_ERR_UNSUPPORTED_BLOCK;
+    if (int64_t(max_blocks_per_seq) * block_size > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    if (!free_end || !cu_seqlens || (num_reqs > 0 && (!context_lens || !query_lens || !block_table || !seq_lens)) ||
+        (num_free > 0 && !free_blocks) || (num_tokens > 0 && (!slot_mapping || !positions)))
+        return FQ_ERR_NULL_POINTER;
+    if (free_end == free_start) return FQ_ERR_BAD_SHAPE;      // one workgroup would write what others read
+    fq::ScheduleParams p;
+    p.context = context_lens; p.query = query_lens; p.table = block_table; p.free_blocks = free_blocks;
+    p.free_start = free_start; p.free_end = free_end; p.slots = slot_mapping; p.positions = positions;
+    p.seq_lens = seq_lens; p.cu = cu_seqlens; p.table_row = block_table_stride; p.num_tokens = num_tokens;
+    p.S = num_reqs; p.max_blocks = max_blocks_per_seq; p.num_free = int(num_free);
+    p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+    const int64_t groups = (num_tokens + fq::kScheduleThreads - 1) / fq::kScheduleThreads;
+    fq::paged_schedule_kernel<<<unsigned(groups > 0 ? groups : 1), fq::kScheduleThreads, 0, static_cast<hipStream_t>(stream)>>>(p);
+    return fq_host::check_launch();
+}

@@ -595,6 +595,87 @@ int fq_split_k_paged_decode_static(const void* q, const uint8_t* kv_cache,
                                    int64_t num_blocks, float sm_scale, int dtype,
                                    int num_splits, void* stream);
 
+/*
+ * Around a paged cache of 16-bit keys and values, which uses the block tables, slots and lengths of the packed one: pages for a
+ * step's tokens, rotary positions, the store of rows and the attention of one new token.  No counterpart in the reference, whose
+ * keys arrive rotated, whose tables come from vLLM and whose 16-bit layers are another library's.
+ *
+ * The caches are addressed by three strides in elements, host arrays {block, token, head}; the D values of a row are contiguous.
+ * (num_blocks, block_size, H_KV, D) tensors, halves of one that holds both, and ones with the heads before the tokens all fit.
+ *
+ * fq_paged_schedule: requests' lengths -> pages, slots, positions of their new tokens, one launch.
+ *   context_lens   (num_reqs,) int32 tokens that request r has in the cache
+ *   query_lens     (num_reqs,) int32 new tokens of request r, their sum below 2^31 (negative lengths count as 0)
+ *   block_table    (num_reqs, max_blocks_per_seq) int32, rows block_table_stride apart: the first ceil(context / block_size)
+ *                  entries of a row are read, the entries of pages that its new tokens begin are written, others stay
+ *   free_blocks    (num_free,) int32 pages that may be taken, from index *free_start on (NULL: 0), in the order of requests and
+ *                  tokens; where they do not suffice an entry becomes -1
+ *   free_end       (1,) int32 out: *free_start + pages wanted (above num_free: there were too few); not free_start itself
+ *   slot_mapping   (num_tokens,) int64 out: block * block_size + position % block_size of the new tokens, request by request; -1
+ *                  for a token without a page or beyond the row's max_blocks_per_seq pages, and behind the last new token
+ *   positions      (num_tokens,) int64 out: context + index of the token in its request; 0 behind the last
+ *   seq_lens       (num_reqs,) int32 out: context + query, at most max_blocks_per_seq * block_size
+ *   cu_seqlens     (num_reqs + 1,) int32 out: first new token of every request
+ * Of new tokens beyond num_tokens neither slot nor page is written (seq_lens, cu_seqlens and free_end count them).  No output may
+ * overlap an input but block_table itself.  block_size in {8, 16, 32}.
+ */
+int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
+                      const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
+                      int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
+                      int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream);
+
+/*
+ * fq_rotary_embedding: pairs (x0, x1) of a head's first 2 * half coordinates become
+ *     scale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a),  a = position * inv_freq[i]  (inverse != 0: -a),
+ *   pair i = coordinates (i, i + half), or (2 i, 2 i + 1) where interleaved != 0; coordinates from 2 * half on are copied.  With
+ *   inverse it is the gradient with respect to its input, and at scale 1 the way back.
+ *   q, k           (batch, tokens, H, D) fp16 / bf16 / float32 rows of contiguous values, elsewhere any strides (host arrays {batch,
+ *                  token, head}, in elements); H_Q or H_K may be 0
+ *   q_out, k_out   the same shape and dtype; the input itself (same strides), or memory that no input shares
+ *   positions      (batch, tokens) of position_bytes (4 or 8) bytes, rows of a batch positions_batch_stride apart (0: shared)
+ *   inv_freq       (half,) float64.  Angles are computed in 64 bits and reduced there: off by 2^-52 of their size
+ * 1 <= half, 2 * half <= D <= 1024, at most 4096 heads each.  Fastest where rows lie at multiples of 16 bytes and half and D are
+ * multiples of 16 bytes' worth of values.
+ *
+ * fq_rotary_paged_store: the same on q (tokens, H_Q, D) and k (tokens, H_KV, D) with k's rows and those of v (tokens, H_KV, D)
+ *   written to their slots of the caches, one launch.  Strides {token, head}.  fp16 / bf16, the caches of the same type.
+ *   slot_mapping   (num_mapped,) int64, num_mapped <= tokens: flat slot (block * block_size + token in block) of token i.  Tokens
+ *                  beyond it, and negative or out-of-range slots, are not stored (their queries are rotated).  Tokens that map
+ *                  to the same slot race.
+ */
+int fq_rotary_embedding(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int H_Q, const void* k,
+                        const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int H_K, const void* positions,
+                        int position_bytes, int64_t positions_batch_stride, const double* inv_freq, int half, int interleaved,
+                        float scale, int inverse, int64_t batch, int64_t tokens, int D, int dtype, void* stream);
+
+int fq_rotary_paged_store(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int H_Q, const void* k,
+                          const int64_t* k_strides, const void* v, const int64_t* v_strides, int H_KV, const void* positions,
+                          int position_bytes, const double* inv_freq, int half, int interleaved, float scale,
+                          const int64_t* slot_mapping, int64_t num_mapped, void* key_cache, const int64_t* key_strides,
+                          void* value_cache, const int64_t* value_strides, int block_size, int64_t num_blocks, int64_t tokens, int D,
+                          int dtype, void* stream);
+
+/*
+ * fq_paged_kv_decode: attention of one query per sequence over such a cache.
+ *   q              (num_seqs, H_Q, D) fp16 / bf16, strides {sequence, head}, 16-byte aligned rows
+ *   block_table    (num_seqs, max_blocks_per_seq) int32, rows block_table_stride apart; seq_lens (num_seqs,) int32 (the new token
+ *                  counted; below 0: 0, beyond max_blocks_per_seq * block_size: that)
+ *   window         0, or how many of the last tokens are seen
+ *   out            (num_seqs, H_Q, D) contiguous, dtype of q and of the caches
+ *   lse            (num_seqs, H_Q) float32 out, or NULL: log sum exp(sm_scale q.k), which joins the result to that over other keys
+ * Tokens on pages outside [0, num_blocks) are not seen.  A row that sees no token, or whose scores are all -inf, is 0 with an lse of
+ * -inf.  Weights keep 16 bits and more, sums and maxima 32.  Long sequences are cut into parts that a second launch joins; the
+ * parts follow from all lengths, so the last bits of a row may differ with the batch that it is in.
+ *   workspace      fq_paged_kv_decode_workspace_bytes bytes (0: none needed), 256-byte aligned, any contents
+ * D in {64, 128, 256}, block_size in {8, 16, 32}, H_Q / H_KV <= 16, caches 16-byte aligned with strides that are multiples of 8.
+ */
+size_t fq_paged_kv_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq);
+int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
+                       const void* value_cache, const int64_t* value_strides, const int32_t* block_table, int64_t block_table_stride,
+                       const int32_t* seq_lens, void* out, float* lse, int num_seqs, int H_Q, int H_KV, int D, int block_size,
+                       int max_blocks_per_seq, int64_t num_blocks, float sm_scale, int window, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
