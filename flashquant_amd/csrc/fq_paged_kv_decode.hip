@@ -7,19 +7,34 @@
 // What bounds it: every key and value is read once, 4 D bytes a token and KV head for 4 G D flops, so HBM does.  The tile loop
 // therefore only has to keep enough loads in flight, and is laid out so that nothing but registers stands between a load and
 // the matrix cores:
-//   * A wavefront takes 32 keys at a time.  S^T = K Q^T runs on v_mfma_f32_16x16x32: the A operand is a key's row as it lies in
-//     memory (16 bytes a lane).  Row m of tile t is key 8 (m / 4) + 4 t + m % 4, so that after two tiles lane (g, h) holds the
-//     scores of keys 8 g .. 8 g + 7 for head h: exactly the B operand of O^T = V^T P, without a move between lanes.
-//   * A lane loads coordinates 8 n .. 8 n + 7 of the values of keys 8 g .. 8 g + 7 (whole rows of 256 bytes a group of 16
-//     lanes) and turns them into the A operand, 8 keys of one coordinate, with half a v_perm_b32 an element.
-//   * O^T has the head along the lanes: the running maximum, sum and rescaling are a lane's own.
+//   * A wavefront takes 32 keys at a time.  S^T = K Q^T and O^T = V^T P run on v_mfma_f32_16x16x32, heads along the columns.  Row m
+//     of tile t of the scores is key 8 (m / 4) + 4 t + m % 4, so that after two tiles lane (g, h) holds the scores of keys 8 g ..
+//     8 g + 7 for head h: exactly the B operand of the second product, without a move between lanes.  Maximum, sum and
+//     rescaling of a head are a lane's own.
+//   * A load takes whole lines of 128 bytes.  Of a key that is 64 coordinates, twice what the A operand holds: rows 0 to 7 of
+//     the operand are eight keys' first halves, rows 8 to 15 their second halves; it is multiplied with both halves of the
+//     query, and the right quarters of the two results are added across the halves of the wavefront.  That doubles a product that
+//     costs nothing, where 64 bytes a key and load read every line twice (32 x 4096 tokens, 8 heads of 128, non-temporal: 105 us
+//     for 95).
+//   * A lane loads coordinates 8 n .. 8 n + 7 of the values of keys 8 g .. 8 g + 7 (whole rows) and turns them into the A operand, 8
+//     keys of one coordinate, with half a v_perm_b32 an element; a key that is not seen becomes zero there, whatever it holds.
+//   * Loads are non-temporal: a layer's keys and values are read once a step, and other layers' pass through the 256 MB of
+//     shared cache in between (32 x 4096: 105 us -> 95; a stream of 2 GB of its own: 6.2 TB/s -> 7.0).
+//   * The wavefronts of a workgroup take up to four neighbouring heads of the same tokens, whose rows lie side by side (against one
+//     head a workgroup: 61 sequences of 500 to 16000 tokens, 64 heads over 8, 364 us -> 348; a plain read of the rows 6.6 ->
+//     6.95 TB/s), and the tiles in turn; wavefronts of the same head are joined in LDS.
 //   * A weight goes to the second product as two 16-bit terms (16 significant bits and more), so that the only rounding
 //     that shows is that of the output; the matrix cores are idle otherwise.  Maximum and sum are float32, of the unrounded
 //     weights.
-// The wavefronts of a workgroup take a part's tiles in turn and are joined in LDS.  Long sequences are cut into parts, joined by
-// a second launch (find_part below).
+// Measured: 32 sequences of 4096 tokens, 32 heads over 8 of 128, bf16, 84.6 us (6.35 TB/s); 61 of 500 to 16000, 64 over 8, fp16, 342.6 us
+// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 22.8 us; one of 777, 32 over 8, 10.7 us.
+#include <type_traits>
+
 #include "fq_device.hpp"
 
+#ifndef MINPER
+#define MINPER 1
+#endif
 namespace fq {
 
 constexpr int kKvTile = 32;               // keys of a wavefront's step
@@ -33,15 +48,15 @@ struct KvDecodeParams {
     const int32_t* lens;
     uint16_t* out;
     float* lse;                           // may be null
-    float* part_o;                        // (S + extra, H_KV, G, D)
-    float* part_m;                        // (S + extra, H_KV, G)
+    float* part_o;                        // (S + shares, H_KV, G, D)
+    float* part_m;                        // (S + shares, H_KV, G)
     float* part_l;
     int64_t q_seq, q_head;                // strides in elements
     int64_t k_block, k_token, k_head, v_block, v_token, v_head;
     int64_t table_row;
     int S, H_KV, G, page_log2, max_blocks, num_blocks, window;
-    int extra;                            // parts beyond one a sequence, of a KV head; 0: no sequence is cut
-    int min_tiles;                        // of a part of a sequence that is cut
+    int shares;                           // workgroups among which the tiles of a KV head are divided; 0: one a sequence
+    int min_tiles;                        // of such a share
     float scale_log2;
 };
 
@@ -59,34 +74,31 @@ __device__ __forceinline__ KvSpan kv_span(const KvDecodeParams& p, int len) {
     return r;
 }
 
-// Which part of which sequence is number x.  Nothing on the host knows the lengths, so every workgroup works it out from them:
-// a part has `size` tiles, so chosen that all sequences together have at most S + extra parts; each sequence is then cut into
-// equal ones.  Arithmetic on the lengths alone: the same in every workgroup and in the launch that joins the parts.
-struct KvPart {
-    int seq, part, parts, base;           // base: number of the sequence's first part
+// How the work is divided where contexts may be long: the tiles of all sequences, one after another, are cut into equal shares, one
+// a workgroup (of a KV head), so that all of them end together whatever the lengths are.  Nothing on the host knows the lengths:
+// every workgroup adds them up for itself.  The piece of sequence s in share x is number x + s of the partial results: from
+// one piece to the next either the share or the sequence goes up by one.
+struct KvPlace {
+    int size;                             // tiles of a share
+    int seq, before;                      // a sequence, and the tiles of those before it
     KvSpan span;
 };
-__device__ __forceinline__ int kv_part_size(const KvDecodeParams& p, int lane) {
-    uint32_t total = 0;
-    for (int s = 0; s < p.S; s += kWave) total += uint32_t(s + lane < p.S ? kv_span(p, p.lens[s + lane]).tiles : 0);
-    total = wave_sum(total);
-    const int share = int((total + uint32_t(p.extra) - 1) / uint32_t(p.extra));
-    return share > p.min_tiles ? share : p.min_tiles;
-}
-__device__ __forceinline__ int kv_parts(int tiles, int size) { return tiles <= size ? 1 : (tiles + size - 1) / size; }
+__device__ __forceinline__ int kv_tiles_of(const KvDecodeParams& p, int s) { return s < p.S ? kv_span(p, p.lens[s]).tiles : 0; }
 
-// by_seq: x is a sequence and the answer its first part; else x is a part's number.  False: there is none of that number.
-template <bool by_seq>
-__device__ __forceinline__ bool find_part(const KvDecodeParams& p, int x, int lane, KvPart& r) {
-    if (p.extra == 0) {
-        r = {x, 0, 1, x, kv_span(p, p.lens[x])};
-        return true;
-    }
-    const int size = kv_part_size(p, lane);
+// `of_seq`: the place of sequence x; else of the sequence that holds the first tile of share x.  False: there is no such tile.
+template <bool of_seq>
+__device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lane, KvPlace& r) {
+    const int first = kv_tiles_of(p, lane);                  // (up to 64 sequences are read once)
+    uint32_t total = uint32_t(first);
+    for (int s = kWave; s < p.S; s += kWave) total += uint32_t(kv_tiles_of(p, s + lane));
+    total = wave_sum(total);
+    const int share = int((total + uint32_t(p.shares) - 1) / uint32_t(p.shares));
+    r.size = share > p.min_tiles ? share : p.min_tiles;
+    const int64_t wanted = int64_t(x) * r.size;
+    if (!of_seq && wanted >= int64_t(total)) return false;
     int before = 0;
     for (int s = 0; s < p.S; s += kWave) {
-        const int len = s + lane < p.S ? p.lens[s + lane] : 0;
-        const int n = s + lane < p.S ? kv_parts(kv_span(p, len).tiles, size) : 0;
+        const int n = s == 0 ? first : kv_tiles_of(p, s + lane);
         int upto = n;                                        // inclusive sum over the lanes
 #pragma unroll
         for (int d = 1; d < kWave; d *= 2) {
@@ -94,15 +106,10 @@ __device__ __forceinline__ bool find_part(const KvDecodeParams& p, int x, int la
             upto += lane >= d ? below : 0;
         }
         const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
-        const bool here = by_seq ? x < s + kWave : x < before + all;
-        if (here) {
-            const int at = by_seq ? x - s : __ffsll(static_cast<unsigned long long>(__ballot(before + upto > x))) - 1;
-            const int l = __builtin_amdgcn_readlane(len, at);
+        if (of_seq ? x < s + kWave : wanted < int64_t(before) + all) {
+            const int at = of_seq ? x - s : __ffsll(static_cast<unsigned long long>(__ballot(before + upto > int(wanted)))) - 1;
             r.seq = s + at;
-            r.parts = __builtin_amdgcn_readlane(n, at);
-            r.base = before + __builtin_amdgcn_readlane(upto, at) - r.parts;
-            r.part = by_seq ? 0 : x - r.base;
-            r.span = kv_span(p, l);
+            r.before = before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
             return true;
         }
         before += all;
@@ -128,284 +135,375 @@ template <int DT> __device__ __forceinline__ float high_value(uint32_t w) {
 // Words of a lane's piece of one value row: 8 coordinates of 128, 4 of 64.
 template <int D> struct ValueWords { static constexpr int n = D == 64 ? 2 : 4; };
 
-template <int D, int DT, int W>
-__global__ __launch_bounds__(W * kWave) void paged_kv_decode_kernel(const KvDecodeParams p) {
-    constexpr int KJ = D / 32;                       // steps of 32 coordinates in a score
+template <int D, int DT, int HW, int TW, bool SHARED>
+__global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const KvDecodeParams p) {
+    constexpr int KP = D / 64;                       // lines of 128 bytes of a key
     constexpr int VH = D == 256 ? 2 : 1;             // halves of 128 coordinates
     constexpr int VW = ValueWords<D>::n;
     constexpr int VE = 2 * VW;                       // coordinates of a lane's piece
+    constexpr int W = HW * TW;
     extern __shared__ __align__(16) float lds[];     // (W, G, D), then (W, 2, 16), then (2, 16)
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int n = lane & 15, g = lane >> 4;
+    const int n = lane & 15, g = lane >> 4, kgroup = (n >> 2) & 1;
     const int G = p.G;
-    const int x = blockIdx.x / p.H_KV, head = blockIdx.x - x * p.H_KV;
+        const int groups = p.H_KV / HW;                  // of HW neighbouring heads
+    const int x = blockIdx.x / groups, head = (blockIdx.x - x * groups) * HW + wave % HW, turn = wave / HW;
 
-    KvPart at;
-    if (!find_part<false>(p, x, lane, at)) return;
-    int begin = 0, end = at.span.tiles;
-    if (at.parts > 1) {
-        const int each = at.span.tiles / at.parts, more = at.span.tiles - each * at.parts;
-        begin = at.part * each + (at.part < more ? at.part : more);
-        end = begin + each + (at.part < more ? 1 : 0);
-    }
-    begin += at.span.first;
-    end += at.span.first;
-
-    const int32_t* table = p.table + int64_t(at.seq) * p.table_row;
-    const uint16_t* kbase = p.kc + head * p.k_head + 8 * g + int64_t(n & 3) * p.k_token;
+    const uint16_t* kbase = p.kc + head * p.k_head + 8 * (g + 4 * (n >> 3)) + int64_t(n & 3) * p.k_token;
     const uint16_t* vbase = p.vc + head * p.v_head + VE * n;
     const int page_mask = (1 << p.page_log2) - 1;
+    const int last_tile = ((p.max_blocks << p.page_log2) - 1) / kKvTile;
 
-    // the block of the 8 keys that this lane reads a key of, and of those that it reads the values of
-    auto block_of = [&](int tile, int group) {
-        const int b = (tile * kKvTile + 8 * group) >> p.page_log2;
+    // Where a wavefront's next 16 tiles lie: lane 4 i + b knows it of keys 8 b .. 8 b + 7 of the i-th (one load and one
+    // multiplication a group of 8 keys; the tiles fetch it across lanes).  Bit 4 i + b of `present`: the page is one of the cache.
+    int64_t key_at = 0, value_at = 0;
+    uint64_t present = 0;
+    auto token_of = [&](int tile) {                  // of lane 4 i + b, the i-th tile from `tile` on
+        const int t = tile + TW * (lane >> 2);
+        return (t < last_tile ? t : last_tile) * kKvTile + 8 * (lane & 3);
+    };
+    auto block_of = [&](const int32_t* table, int tile) {
+        const int b = token_of(tile) >> p.page_log2;
         return table[b < p.max_blocks ? b : p.max_blocks - 1];
     };
-    auto in_cache = [&](int block) { return uint32_t(block) < uint32_t(p.num_blocks); };
+    auto locate = [&](int tile, int block) {
+        const bool in_cache = uint32_t(block) < uint32_t(p.num_blocks);
+        present = __ballot(in_cache);
+        const int b = in_cache ? block : 0, t = token_of(tile) & page_mask;
+        key_at = int64_t(b) * p.k_block + int64_t(t) * p.k_token;
+        value_at = int64_t(b) * p.v_block + int64_t(t) * p.v_token;
+    };
+    auto fetch = [&](int64_t v, int at) {            // from lane at / 4
+        const int lo = __builtin_amdgcn_ds_bpermute(at, int(v)), hi = __builtin_amdgcn_ds_bpermute(at, int(v >> 32));
+        return (int64_t(hi) << 32) | uint32_t(lo);
+    };
 
-    uint4v kr[2][KJ];
+    uint4v kr[2][2][KP];
     uint32_t vr[8][VH][VW];
-    auto load_keys = [&](int tile, int block) {
-        const int group = n >> 2;
-        const uint16_t* src = kbase + int64_t(in_cache(block) ? block : 0) * p.k_block +
-                              int64_t((tile * kKvTile + 8 * group) & page_mask) * p.k_token;
+    auto load_keys = [&](int i) {                    // of the i-th tile of the 16
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int h = 0; h < 2; ++h) {
+            const uint16_t* src = kbase + fetch(key_at, 16 * i + 4 * kgroup + 8 * h);
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) kr[t][j] = *reinterpret_cast<const uint4v*>(src + 32 * j);
-            src += 4 * p.k_token;
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int a = 0; a < KP; ++a) kr[t][h][a] = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(src + 64 * a));
+                src += 4 * p.k_token;
+            }
         }
     };
-    auto load_values = [&](int tile, int block) {
-        const uint16_t* src = vbase + int64_t(in_cache(block) ? block : 0) * p.v_block +
-                              int64_t((tile * kKvTile + 8 * g) & page_mask) * p.v_token;
+    auto load_values = [&](int i) {
+        const uint16_t* src = vbase + fetch(value_at, 16 * i + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int k = 0; k < 8; ++k) {
 #pragma unroll
             for (int h = 0; h < VH; ++h) {
                 if constexpr (VW == 4) {
-                    const uint4v w = *reinterpret_cast<const uint4v*>(src + 128 * h);
-                    vr[i][h][0] = w.x; vr[i][h][1] = w.y; vr[i][h][2] = w.z; vr[i][h][3] = w.w;
+                    const uint4v w = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(src + 128 * h));
+                    vr[k][h][0] = w.x; vr[k][h][1] = w.y; vr[k][h][2] = w.z; vr[k][h][3] = w.w;
                 } else {
-                    const uint2v w = *reinterpret_cast<const uint2v*>(src);
-                    vr[i][h][0] = w.x; vr[i][h][1] = w.y;
+                    const uint2v w = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(src));
+                    vr[k][h][0] = w.x; vr[k][h][1] = w.y;
                 }
             }
             src += p.v_token;
         }
     };
 
-    float4v acc[VH][VE];
-#pragma unroll
-    for (int h = 0; h < VH; ++h)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[h][e] = float4v{0.f, 0.f, 0.f, 0.f};
-    float m = -__builtin_inff(), l = 0.0f;
-
-    int tile = begin + wave;
-    if (tile < end) {
-        int kblock = block_of(tile, n >> 2), vblock = block_of(tile, g);
-        load_keys(tile, kblock);
-        load_values(tile, vblock);
-        uint4v qr[KJ];
+    int seq = x, offset = 0, left = 0;               // the sequence, its first tile here, the tiles left of the share
+    if constexpr (SHARED) {
+        KvPlace at;
+        if (!kv_place<false>(p, x, lane, at)) return;
+        seq = at.seq;
+        offset = x * at.size - at.before;
+        left = at.size;
+    }
+    bool again = false;
+    do {
+        const int32_t* table = p.table + int64_t(seq) * p.table_row;
+        int block = 0;
+        if (!SHARED && p.window == 0) block = block_of(table, turn);     // known before the length is
+        uint4v qr[2 * KP];
         {
-            const uint16_t* src = p.q + int64_t(at.seq) * p.q_seq + int64_t(head * G + (n < G ? n : 0)) * p.q_head + 8 * g;
+            const uint16_t* src = p.q + int64_t(seq) * p.q_seq + int64_t(head * G + (n < G ? n : 0)) * p.q_head + 8 * g;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) qr[j] = n < G ? *reinterpret_cast<const uint4v*>(src + 32 * j) : uint4v{0u, 0u, 0u, 0u};
+            for (int j = 0; j < 2 * KP; ++j) qr[j] = *reinterpret_cast<const uint4v*>(src + 32 * j);
         }
-        int next_k = 0, next_v = 0;
-        if (tile + W < end) { next_k = block_of(tile + W, n >> 2); next_v = block_of(tile + W, g); }
-        for (; tile < end; tile += W) {
-            const bool more = tile + W < end;
-            float4v s[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                s[t] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < KJ; ++j) s[t] = kv_mfma<DT>(kr[t][j], qr[j], s[t]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            int after_k = 0, after_v = 0;
-            if (more) {
-                load_keys(tile + W, next_k);
-                if (tile + 2 * W < end) { after_k = block_of(tile + 2 * W, n >> 2); after_v = block_of(tile + 2 * W, g); }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            float sv[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sv[i] = s[i >> 2][i & 3] * p.scale_log2;
-            // whole tiles whose pages are all in the cache need no mask
-            const int key = tile * kKvTile + 8 * g;
-            const bool page_ok = in_cache(vblock);
-            const bool whole = tile * kKvTile >= at.span.lo && tile * kKvTile + kKvTile <= at.span.len && __all(page_ok);
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool seen = page_ok && key + i >= at.span.lo && key + i < at.span.len;
-                    sv[i] = seen ? sv[i] : -__builtin_inff();
-                }
-            }
-            float top = sv[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, sv[i]);
-            top = max_xor32(max_xor16(top));
-            if (__any(top > m)) {
-                const float higher = __builtin_fmaxf(m, top);
-                const float shrink = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
-                l *= shrink;
-#pragma unroll
-                for (int h = 0; h < VH; ++h)
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) acc[h][e] *= shrink;
-                m = higher;
-            }
-            const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift;
-            uint4v hi, lo;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float a = __builtin_amdgcn_exp2f(sv[i] - ref), b = __builtin_amdgcn_exp2f(sv[i + 1] - ref);
-                l += a + b;
-                hi[i / 2] = round_pair<DT>(a, b);
-                lo[i / 2] = round_pair<DT>(a - low_value<DT>(hi[i / 2]), b - high_value<DT>(hi[i / 2]));
-            }
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool seen = page_ok && key + i >= at.span.lo && key + i < at.span.len;
-#pragma unroll
-                    for (int h = 0; h < VH; ++h)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) vr[i][h][w] = seen ? vr[i][h][w] : 0u;
-                }
-            }
-            uint4v vt[VH][VE];
-#pragma unroll
-            for (int h = 0; h < VH; ++h)
-#pragma unroll
-                for (int e = 0; e < VE; ++e)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        vt[h][e][i] = __builtin_amdgcn_perm(vr[2 * i + 1][h][e / 2], vr[2 * i][h][e / 2],
-                                                            e & 1 ? 0x07060302u : 0x05040100u);
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) load_values(tile + W, next_v);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int h = 0; h < VH; ++h)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    acc[h][e] = kv_mfma<DT>(vt[h][e], lo, acc[h][e]);
-                    acc[h][e] = kv_mfma<DT>(vt[h][e], hi, acc[h][e]);
-                }
-            kblock = next_k; vblock = next_v;
-            next_k = after_k; next_v = after_v;
-        }
-        l = sum_xor32(sum_xor16(l));
-    }
+        const KvSpan span = kv_span(p, p.lens[seq]);
+        const int count = !SHARED || span.tiles - offset < left ? span.tiles - offset : left;
+        const int end = span.first + offset + count;
 
-    // the wavefronts' results, joined: lane (g, h) holds coordinates VE (4 g + r) + e of head h
-    float* sm = lds + W * G * D;
-    float* total = sm + W * 32;
-    if (g == 0) {
-        sm[wave * 32 + n] = m;
-        sm[wave * 32 + 16 + n] = l;
-    }
-    __syncthreads();
-    float top = sm[n];
-#pragma unroll
-    for (int w = 1; w < W; ++w) top = __builtin_fmaxf(top, sm[w * 32 + n]);
-    if (wave == 0 && g == 0) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float mw = sm[w * 32 + n], lw = sm[w * 32 + 16 + n];
-            sum += lw * piece_weight(mw, lw, top);
-        }
-        total[n] = top;
-        total[16 + n] = sum;
-    }
-    const float weight = piece_weight(m, l, top);
-    if (n < G) {
+        float4v acc[VH][VE];
 #pragma unroll
         for (int h = 0; h < VH; ++h)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float* dst = lds + (wave * G + n) * D + 128 * h + VE * (4 * g + r);
+            for (int e = 0; e < VE; ++e) acc[h][e] = float4v{0.f, 0.f, 0.f, 0.f};
+        float m = -__builtin_inff(), l = 0.0f;
+
+        int tile = span.first + offset + turn;
+        if (tile < end) {
+            if (SHARED || p.window != 0) block = block_of(table, tile);
+            locate(tile, block);
+            load_keys(0);
+            load_values(0);
+            int i = 0;                               // the tile's number among the 16
+            int pages = int(present & 15);
+            block = block_of(table, tile + 16 * TW);
 #pragma unroll
-                for (int e = 0; e < VE; e += 4)
-                    *reinterpret_cast<float4v*>(dst + e) = float4v{acc[h][e][r] * weight, acc[h][e + 1][r] * weight,
-                                                                   acc[h][e + 2][r] * weight, acc[h][e + 3][r] * weight};
+            for (int j = 0; j < 2 * KP; ++j) qr[j] = n < G ? qr[j] : uint4v{0u, 0u, 0u, 0u};
+            // (whether another tile follows is known at compile time: a branch round the loads would make the waits for
+            // the values wait for the next keys as well)
+            auto step = [&](auto followed) {
+                constexpr bool more = decltype(followed)::value;
+                float4v s[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float4v half[2][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            half[h][c] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int a = 0; a < KP; ++a) half[h][c] = kv_mfma<DT>(kr[t][h][a], qr[2 * a + c], half[h][c]);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t lo = float_to_bits(lane < 32 ? half[0][0][r] : half[0][1][r]);
+                        const uint32_t hi = float_to_bits(lane < 32 ? half[1][0][r] : half[1][1][r]);
+                        const auto both = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+                        s[t][r] = bits_to_float(both[0]) + bits_to_float(both[1]);
+                    }
+                }
+                const int pages_now = pages;
+                if constexpr (more) {
+                    if (++i == 16) {
+                        i = 0;
+                        locate(tile + TW, block);
+                        block = block_of(table, tile + 17 * TW);
+                    }
+                    pages = int(present >> (4 * i)) & 15;
+                    load_keys(i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                float sv[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sv[k] = s[k >> 2][k & 3] * p.scale_log2;
+                // v_perm selectors that turn two keys' words into two coordinates' pairs of keys; a byte of 12 is a zero
+                uint32_t even[4], odd[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { even[k] = 0x05040100u; odd[k] = 0x07060302u; }
+                // whole tiles whose pages are all in the cache need no mask
+                if (pages_now != 15 || tile * kKvTile < span.lo || tile * kKvTile + kKvTile > span.len) {
+                    const int key = tile * kKvTile + 8 * g;
+                    int from = span.lo - key, to = span.len - key;
+                    from = from < 0 ? 0 : from > 8 ? 8 : from;
+                    to = to < 0 ? 0 : to > 8 ? 8 : to;
+                    uint32_t seen = ((1u << to) - 1u) & ~((1u << from) - 1u);
+                    seen = (pages_now >> g) & 1 ? seen : 0u;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sv[k] = (seen >> k) & 1u ? sv[k] : -__builtin_inff();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t keep = ((seen >> (2 * k)) & 1u ? 0x0000ffffu : 0u) | ((seen >> (2 * k + 1)) & 1u ? 0xffff0000u : 0u);
+                        even[k] = (even[k] & keep) | (0x0c0c0c0cu & ~keep);
+                        odd[k] = (odd[k] & keep) | (0x0c0c0c0cu & ~keep);
+                    }
+                }
+                float top = sv[0];
+#pragma unroll
+                for (int k = 1; k < 8; ++k) top = __builtin_fmaxf(top, sv[k]);
+                top = max_xor32(max_xor16(top));
+                if (__any(top > m)) {
+                    const float higher = __builtin_fmaxf(m, top);
+                    const float shrink = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
+                    l *= shrink;
+#pragma unroll
+                    for (int h = 0; h < VH; ++h)
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) acc[h][e] *= shrink;
+                    m = higher;
+                }
+                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift;
+                uint4v hi, lo;
+                float w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = __builtin_amdgcn_exp2f(sv[k] - ref);
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {
+                    hi[k / 2] = round_pair<DT>(w[k], w[k + 1]);
+                    lo[k / 2] = round_pair<DT>(w[k] - low_value<DT>(hi[k / 2]), w[k + 1] - high_value<DT>(hi[k / 2]));
+                }
+                l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                // (all of this before the wait for the values)
+                asm volatile("" : "+v"(hi), "+v"(lo), "+v"(l));
+                uint4v vt[VH][VE];
+#pragma unroll
+                for (int h = 0; h < VH; ++h)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            vt[h][e][k] = __builtin_amdgcn_perm(vr[2 * k + 1][h][e / 2], vr[2 * k][h][e / 2], e & 1 ? odd[k] : even[k]);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (more) load_values(i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int h = 0; h < VH; ++h)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) acc[h][e] = kv_mfma<DT>(vt[h][e], lo, acc[h][e]);
+#pragma unroll
+                for (int h = 0; h < VH; ++h)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) acc[h][e] = kv_mfma<DT>(vt[h][e], hi, acc[h][e]);
+            };
+            for (; tile + TW < end; tile += TW) step(std::true_type{});
+            step(std::false_type{});
+            l = sum_xor32(sum_xor16(l));
+        }
+
+        const bool complete = !SHARED || count == span.tiles;
+        const int64_t row = (int64_t(x + seq) * p.H_KV + head) * G;      // of the partial results
+        const int64_t orow = (int64_t(seq) * p.H_KV + head) * G;         // of the outputs
+        auto write_sum = [&](int h, float mt, float lt) {
+            if (!complete) {
+                p.part_m[row + h] = mt;
+                p.part_l[row + h] = lt;
+            } else if (p.lse != nullptr) {
+                p.lse[orow + h] = lt == 0.0f ? -__builtin_inff() : (mt - kKvLift + __builtin_amdgcn_logf(lt)) * (1.0f / kLog2e);
             }
-    }
-    __syncthreads();
-    const int64_t row = int64_t(x) * p.H_KV + head;                  // of the parts
-    const int64_t orow = (int64_t(at.seq) * p.H_KV + head) * G;      // of the outputs
-    for (int i = 4 * int(threadIdx.x); i < G * D; i += 4 * W * kWave) {
-        float4v o = *reinterpret_cast<const float4v*>(lds + i);
+        };
+        // lane (g, h) holds coordinates VE (4 g + r) + e of head h
+        if constexpr (TW == 1) {
+            if (n < G) {
+                const float inv = inverse_sum(l);
 #pragma unroll
-        for (int w = 1; w < W; ++w) o += *reinterpret_cast<const float4v*>(lds + w * G * D + i);
-        if (at.parts == 1) {
-            const float inv = inverse_sum(total[16 + i / D]);
-            *reinterpret_cast<uint2v*>(p.out + orow * D + i) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
+                for (int h = 0; h < VH; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int c = 128 * h + VE * (4 * g + r);
+#pragma unroll
+                        for (int e = 0; e < VE; e += 4) {
+                            if (complete)
+                                *reinterpret_cast<uint2v*>(p.out + (orow + n) * D + c + e) =
+                                    uint2v{round_pair<DT>(acc[h][e][r] * inv, acc[h][e + 1][r] * inv),
+                                           round_pair<DT>(acc[h][e + 2][r] * inv, acc[h][e + 3][r] * inv)};
+                            else
+                                *reinterpret_cast<float4v*>(p.part_o + (row + n) * D + c + e) =
+                                    float4v{acc[h][e][r], acc[h][e + 1][r], acc[h][e + 2][r], acc[h][e + 3][r]};
+                        }
+                    }
+                if (g == 0) write_sum(n, m, l);
+            }
         } else {
-            *reinterpret_cast<float4v*>(p.part_o + row * G * D + i) = o;
+            // the wavefronts of a head are joined in LDS
+            float* sm = lds + W * G * D;             // (W, 2, 16)
+            if (SHARED && again) __syncthreads();    // the piece before has been read
+            if (g == 0) {
+                sm[wave * 32 + n] = m;
+                sm[wave * 32 + 16 + n] = l;
+            }
+            __syncthreads();
+            const int mine = wave % HW;
+            float top = sm[mine * 32 + n];
+#pragma unroll
+            for (int w = 1; w < TW; ++w) top = __builtin_fmaxf(top, sm[(mine + w * HW) * 32 + n]);
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < TW; ++w) {
+                const float mw = sm[(mine + w * HW) * 32 + n], lw = sm[(mine + w * HW) * 32 + 16 + n];
+                sum += lw * piece_weight(mw, lw, top);
+            }
+            float* scale = sm + W * 32;              // (HW, 16)
+            if (turn == 0 && g == 0) {
+                if (n < G) write_sum(n, top, sum);
+                scale[mine * 16 + n] = complete ? inverse_sum(sum) : 1.0f;
+            }
+            const float weight = piece_weight(m, l, top);
+            if (n < G) {
+#pragma unroll
+                for (int h = 0; h < VH; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float* dst = lds + (wave * G + n) * D + 128 * h + VE * (4 * g + r);
+#pragma unroll
+                        for (int e = 0; e < VE; e += 4)
+                            *reinterpret_cast<float4v*>(dst + e) = float4v{acc[h][e][r] * weight, acc[h][e + 1][r] * weight,
+                                                                           acc[h][e + 2][r] * weight, acc[h][e + 3][r] * weight};
+                    }
+            }
+            __syncthreads();
+            // the HW heads' rows lie side by side, in LDS and in memory
+            for (int i = 4 * int(threadIdx.x); i < HW * G * D; i += 4 * W * kWave) {
+                float4v o = *reinterpret_cast<const float4v*>(lds + i);
+#pragma unroll
+                for (int w = 1; w < TW; ++w) o += *reinterpret_cast<const float4v*>(lds + w * HW * G * D + i);
+                const int h = i / D;
+                const float inv = scale[h / G * 16 + h % G];
+                const int64_t first = -int64_t(mine) * G * D + i;        // from this wavefront's head to the group's first
+                if (complete)
+                    *reinterpret_cast<uint2v*>(p.out + orow * D + first) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
+                else
+                    *reinterpret_cast<float4v*>(p.part_o + row * D + first) = o;
+            }
         }
-    }
-    if (int(threadIdx.x) < G) {
-        const float mt = total[threadIdx.x], lt = total[16 + threadIdx.x];
-        if (at.parts > 1) {
-            p.part_m[row * G + threadIdx.x] = mt;
-            p.part_l[row * G + threadIdx.x] = lt;
-        } else if (p.lse != nullptr) {
-            p.lse[orow + threadIdx.x] = lt == 0.0f ? -__builtin_inff() : (mt - kKvLift + __builtin_amdgcn_logf(lt)) * (1.0f / kLog2e);
+        if constexpr (SHARED) {
+            left -= count;
+            offset = 0;
+            again = true;
+            do ++seq;
+            while (left > 0 && seq < p.S && kv_tiles_of(p, seq) == 0);   // (sequences of no tokens: the second launch)
         }
-    }
+    } while (SHARED && left > 0 && seq < p.S);
 }
 
-// Joins the parts of the sequences that have several; one workgroup a sequence and query head.
-template <int D, int DT>
+// Joins the pieces of the sequences that several shares hold, and writes the rows of those that have no tokens.  A workgroup
+// takes 4 Q neighbouring values of the G rows of one sequence and KV head, R pieces at a time, each thread with a maximum and a
+// sum of its own (so one trip to memory brings all it needs).
+template <int D, int DT, int Q>
 __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams p) {
-    constexpr int Q = D / 4;                         // lanes of a row
-    constexpr int R = 256 / Q;                       // rows at a time
-    __shared__ __align__(16) float rows[R][D];
-    __shared__ float wave_m[4], sums[R];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int H_Q = p.H_KV * p.G;
-    const int seq = blockIdx.x / H_Q, hq = blockIdx.x - seq * H_Q;
-    KvPart at;
-    find_part<true>(p, seq, lane, at);
-    if (at.parts == 1) return;
-    // parts of one KV head lie H_KV * G rows apart
-    const int64_t first = int64_t(at.base) * H_Q + hq;
-    float top = -__builtin_inff();
-    for (int i = threadIdx.x; i < at.parts; i += 256) top = __builtin_fmaxf(top, p.part_m[first + int64_t(i) * H_Q]);
-    top = wave_max(top);
-    if (lane == 0) wave_m[wave] = top;
-    __syncthreads();
-    top = __builtin_fmaxf(__builtin_fmaxf(wave_m[0], wave_m[1]), __builtin_fmaxf(wave_m[2], wave_m[3]));
-    const int c = 4 * (threadIdx.x % Q), r0 = threadIdx.x / Q;
+    constexpr int R = 256 / Q;
+    __shared__ __align__(16) float4v rows[R][Q];
+    __shared__ float2v sums[R][Q];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int columns = p.G * D / (4 * Q);
+    const int64_t group = blockIdx.x / columns;                          // sequence and KV head
+    const int seq = int(group / p.H_KV);
+    const int c = 4 * (int(blockIdx.x % columns) * Q + threadIdx.x % Q), r0 = threadIdx.x / Q, h = c / D;
+    KvPlace at;
+    kv_place<true>(p, seq, lane, at);
+    const int tiles = kv_tiles_of(p, seq);
+    const int share0 = at.before / at.size, share1 = tiles > 0 ? (at.before + tiles - 1) / at.size : share0;
+    const int pieces = tiles > 0 ? share1 - share0 + 1 : 0;
+    if (pieces == 1) return;
+    const int64_t step = int64_t(p.H_KV) * p.G;                          // rows from one piece to the next
+    const int64_t first = int64_t(share0 + seq) * step + (group - int64_t(seq) * p.H_KV) * p.G;
     float4v o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.0f;
-    for (int i = r0; i < at.parts; i += R) {
-        const int64_t row = first + int64_t(i) * H_Q;
-        const float l = p.part_l[row], w = piece_weight(p.part_m[row], l, top);
-        o += *reinterpret_cast<const float4v*>(p.part_o + row * D + c) * w;
-        sum += l * w;
+    float top = -__builtin_inff(), sum = 0.0f;
+    auto take = [&](float4v v, float m, float l) {
+        const float higher = __builtin_fmaxf(top, m);
+        const float a = piece_weight(top, sum, higher), b = piece_weight(m, l, higher);
+        o = o * a + v * b;
+        sum = sum * a + l * b;
+        top = higher;
+    };
+    for (int i = r0; i < pieces; i += R) {
+        const int64_t row = first + i * step;
+        take(*reinterpret_cast<const float4v*>(p.part_o + row * D + c), p.part_m[row + h], p.part_l[row + h]);
     }
-    *reinterpret_cast<float4v*>(&rows[r0][c]) = o;
-    if (threadIdx.x % Q == 0) sums[r0] = sum;
-    __syncthreads();
+    if (R > 1) {
+        rows[r0][threadIdx.x % Q] = o;
+        sums[r0][threadIdx.x % Q] = float2v{top, sum};
+        __syncthreads();
+    }
     if (threadIdx.x < Q) {
-        float den = sums[0];
-        for (int r = 1; r < R; ++r) {
-            o += *reinterpret_cast<const float4v*>(&rows[r][c]);
-            den += sums[r];
-        }
-        const float inv = inverse_sum(den);
-        const int64_t out = int64_t(seq) * H_Q + hq;
+        const int used = pieces < R ? pieces : R;
+        for (int r = 1; r < used; ++r) take(rows[r][threadIdx.x], sums[r][threadIdx.x].x, sums[r][threadIdx.x].y);
+        const float inv = inverse_sum(sum);
+        const int64_t out = group * p.G;
         *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
-        if (threadIdx.x == 0 && p.lse != nullptr)
-            p.lse[out] = den == 0.0f ? -__builtin_inff() : (top - kKvLift + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
+        if (c % D == 0 && p.lse != nullptr)
+            p.lse[out + h] = sum == 0.0f ? -__builtin_inff() : (top - kKvLift + __builtin_amdgcn_logf(sum)) * (1.0f / kLog2e);
     }
 }
 
@@ -413,14 +511,24 @@ __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams
 
 namespace {
 
-constexpr int kWaves = 8;
+// KV heads that a workgroup takes together, and the wavefronts of a workgroup.
+int kv_heads_together(int H_KV) { return H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1; }
+constexpr int kv_waves(int D) { return D == 256 ? 4 : 8; }
 
-// Parts beyond one a sequence, of a KV head (0: no sequence is cut, and no second launch).
-int kv_extra(int S, int H_KV, int64_t max_tokens) {
-    const int64_t tiles = (max_tokens + fq::kKvTile - 1) / fq::kKvTile;
-    if (tiles <= 2 * kWaves || int64_t(S) * tiles >= (1LL << 31)) return 0;
-    const int target = 2 * fq_host::device_cu_count();
-    return (target + H_KV - 1) / H_KV;
+// Among how many workgroups the tiles of a KV head are divided; 0: one workgroup a sequence, and no second launch.  A CU draws at
+// most about 43 GB/s for itself, so few long sequences have to be spread, but the second launch costs 4 us, and a share that goes
+// on with another sequence starts from nothing again (3 us).  In us, undivided / divided, 32 heads over 8 of 128, bf16: 1 x 500
+// tokens 9.3 / 11.9, 1 x 777 11.2 / 12.2, 1 x 1000 15.5 / 12.9, 1 x 2000 27.3 / 13.4, 16 x 1000 18.4 / 18.7, 32 x 1000 23.9 /
+// 27.6, 32 x 2000 43.7 / 46.9, 64 x 1000 47.2 / 48.5, 200 of 100 to 2000 175 / 158; 8 heads over 1: 128 of 100 to 700 12.9 / 19.2,
+// 64 of 200 to 1500 20.1 / 16.6, 300 of them 30.7 / 37.8; 32 over 32, 16 of 300 to 1000 38.7 / 35.8.
+int kv_shares(int S, int H_KV, int64_t max_tokens, int window) {
+    int64_t tiles = (max_tokens + fq::kKvTile - 1) / fq::kKvTile;
+    if (window > 0 && window / fq::kKvTile + 2 < tiles) tiles = window / fq::kKvTile + 2;
+    const int64_t whole = int64_t(S) * H_KV, cus = fq_host::device_cu_count();
+    if (tiles <= 25 || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus)) return 0;
+    if (int64_t(S) * tiles >= (1LL << 31)) return 0;         // more tiles than are counted
+    const int groups = H_KV / kv_heads_together(H_KV);
+    return int((cus + groups - 1) / groups);                 // a workgroup a CU: more are no faster (two: 32 x 4096 86.7 -> 96)
 }
 
 int check_kv_shape(int S, int H_Q, int H_KV, int D, int block_size, int max_blocks, int64_t num_blocks) {
@@ -437,24 +545,46 @@ size_t round_up(size_t n) { return (n + 255) & ~size_t(255); }
 struct KvRoom {
     size_t o, m, all;
 };
-KvRoom kv_room(int S, int H_Q, int D, int extra) {
-    const size_t rows = (size_t(S) + size_t(extra)) * size_t(H_Q);
+KvRoom kv_room(int S, int H_Q, int D, int shares) {
+    const size_t rows = (size_t(S) + size_t(shares)) * size_t(H_Q);
     KvRoom r;
     r.o = round_up(rows * size_t(D) * 4);
     r.m = round_up(rows * 4);
-    r.all = extra == 0 ? 0 : r.o + 2 * r.m;
+    r.all = shares == 0 ? 0 : r.o + 2 * r.m;
     return r;
+}
+
+template <int D, int DT, int HW, int TW, bool SHARED>
+int launch_attend(const fq::KvDecodeParams& p, hipStream_t s) {
+    const size_t lds = TW == 1 ? 0 : (size_t(HW * TW) * p.G * D + HW * TW * 32 + HW * 16) * 4;
+    auto kernel = fq::paged_kv_decode_kernel<D, DT, HW, TW, SHARED>;
+    if (lds > 32768 && !fq_host::lds_limit_raised(reinterpret_cast<const void*>(kernel), lds)) return FQ_ERR_LAUNCH;
+    kernel<<<unsigned(SHARED ? p.shares : p.S) * unsigned(p.H_KV / HW), HW * TW * 64, lds, s>>>(p);
+    return FQ_OK;
 }
 
 template <int D, int DT>
 int launch_kv(const fq::KvDecodeParams& p, hipStream_t s) {
-    constexpr int W = D == 256 ? 4 : kWaves;
-    const size_t lds = (size_t(W) * p.G * D + W * 32 + 32) * 4;
-    auto kernel = fq::paged_kv_decode_kernel<D, DT, W>;
-    if (lds > 32768 && !fq_host::lds_limit_raised(reinterpret_cast<const void*>(kernel), lds)) return FQ_ERR_LAUNCH;
-    kernel<<<unsigned(p.S + p.extra) * unsigned(p.H_KV), W * 64, lds, s>>>(p);
-    if (p.extra > 0) fq::paged_kv_join_kernel<D, DT><<<unsigned(p.S) * unsigned(p.H_KV * p.G), 256, 0, s>>>(p);
-    return fq_host::check_launch();
+    constexpr int W = kv_waves(D);
+    const int hw = kv_heads_together(p.H_KV);
+    int st;
+    if (p.shares > 0) {
+        st = hw == 4 ? launch_attend<D, DT, 4, W / 4, true>(p, s)
+                     : hw == 2 ? launch_attend<D, DT, 2, W / 2, true>(p, s) : launch_attend<D, DT, 1, W, true>(p, s);
+        if (st != FQ_OK) return st;
+        // as many values a workgroup as leave enough workgroups
+        const int64_t values = int64_t(p.S) * p.H_KV * p.G * D;
+        if (p.G * D % 256 == 0 && values / 256 >= 2 * fq_host::device_cu_count())
+            fq::paged_kv_join_kernel<D, DT, 64><<<unsigned(values / 256), 256, 0, s>>>(p);
+        else
+            fq::paged_kv_join_kernel<D, DT, 16><<<unsigned(values / 64), 256, 0, s>>>(p);
+    } else if (hw == 4 && int64_t(p.S) * p.H_KV >= 8 * fq_host::device_cu_count()) {
+        // many sequences: fewer workgroups (256 of 50 to 300 tokens, 32 heads over 8 of 128: 40 us, 52 with a head a workgroup)
+        st = launch_attend<D, DT, 4, W / 4, false>(p, s);
+    } else {
+        st = launch_attend<D, DT, 1, W, false>(p, s);
+    }
+    return st != FQ_OK ? st : fq_host::check_launch();
 }
 
 template <int D>
@@ -466,8 +596,8 @@ int launch_kv_type(const fq::KvDecodeParams& p, int dtype, hipStream_t s) {
 
 extern "C" size_t fq_paged_kv_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq) {
     if (check_kv_shape(num_seqs, H_Q, H_KV, D, block_size, max_blocks_per_seq, 1) != FQ_OK || num_seqs == 0) return 0;
-    const int extra = kv_extra(num_seqs, H_KV, int64_t(max_blocks_per_seq) * block_size);
-    return kv_room(num_seqs, H_Q, D, extra).all;
+    const int shares = kv_shares(num_seqs, H_KV, int64_t(max_blocks_per_seq) * block_size, 0);     // (a window only takes from it)
+    return kv_room(num_seqs, H_Q, D, shares).all;
 }
 
 extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
@@ -488,9 +618,9 @@ extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const
     }
     if (!fq_host::aligned(q, 16) || !fq_host::aligned(key_cache, 16) || !fq_host::aligned(value_cache, 16) || !fq_host::aligned(out, 16))
         return FQ_ERR_MISALIGNED;
-    const int extra = kv_extra(num_seqs, H_KV, int64_t(max_blocks_per_seq) * block_size);
-    if ((int64_t(num_seqs) + extra) * H_Q > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
-    const KvRoom room = kv_room(num_seqs, H_Q, D, extra);
+    const int shares = kv_shares(num_seqs, H_KV, int64_t(max_blocks_per_seq) * block_size, window);
+    if ((int64_t(num_seqs) + shares) * H_Q * (D / 32) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    const KvRoom room = kv_room(num_seqs, H_Q, D, shares);
     if (room.all > 0) {
         if (!workspace || workspace_bytes < room.all) return FQ_ERR_WORKSPACE;
         if (!fq_host::aligned(workspace, 256)) return FQ_ERR_MISALIGNED;
@@ -514,7 +644,7 @@ extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const
     p.S = num_seqs; p.H_KV = H_KV; p.G = H_Q / H_KV;
     p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
     p.max_blocks = max_blocks_per_seq; p.num_blocks = int(num_blocks); p.window = window;
-    p.extra = extra; p.min_tiles = kWaves;
+    p.shares = shares; p.min_tiles = kv_waves(D) / kv_heads_together(H_KV);      // a tile a wavefront
     p.scale_log2 = sm_scale * fq::kLog2e;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (D) {

@@ -441,6 +441,13 @@ def test_decode_of_many_sequences(lens):
     assert torch.equal(out, again) and torch.equal(lse, lse2)              # the same call, the same bits
 
 
+# so many sequences that a workgroup takes four heads of one; so many tokens that a wavefront looks its pages up more than once
+@pytest.mark.parametrize("lens,hq,hkv,d,page", [([0, 1, 30, 33, 65, 300, 200] * 40, 16, 8, 64, 16), ([5, 0, 129, 40] * 130, 8, 4, 256, 8), ([70000], 16, 16, 64, 8),
+                                                ([40000, 3, 50000], 32, 16, 64, 32), ([38000, 0, 1], 16, 16, 256, 16)])
+def test_decode_of_full_workgroups(lens, hq, hkv, d, page):
+    check_decode(*decode_case(lens, hq, hkv, d, page, BF, seed=len(lens)))
+
+
 @pytest.mark.parametrize("layout", ["together", "heads first", "one row"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_decode_of_strided_operands(layout, d):
