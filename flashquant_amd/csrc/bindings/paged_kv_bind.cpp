@@ -3,6 +3,7 @@
 // they are.  There is no CPU path: a tensor that is not on the GPU is an error.
 
 #include <ATen/MemoryOverlap.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <optional>
@@ -24,6 +25,11 @@ void check(bool ok, const char* msg) {
 void check_place(const at::Tensor& t, const at::Tensor& like, const char* name) {
     fqbind::require_gpu(t, name);
     if (t.device() != like.device()) throw std::invalid_argument(std::string(name) + " must be on the device of the first operand");
+}
+
+// (past torch's dispatcher: half of what at::empty costs a call)
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
 }
 
 // rows (..., H, D) of contiguous values, as the kernels take them; others are copied
@@ -59,7 +65,7 @@ bool same_view(const at::Tensor& a, const at::Tensor& b) { return a.data_ptr() =
 
 // What a result is written to: `out`, checked against all inputs, or new memory.
 at::Tensor rows_out(const MaybeTensor& out, const at::Tensor& x, const at::Tensor& original, const MaybeTensor& other, const char* name) {
-    if (!out.has_value()) return at::empty(x.sizes(), x.options());
+    if (!out.has_value()) return new_tensor(x.sizes(), x.scalar_type(), x);
     check_place(*out, x, name);
     check(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type(), "out must have the shape and dtype of its input");
     check(out->stride(-1) == 1 || out->size(-1) <= 1, "out must have contiguous rows");
@@ -219,12 +225,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
             for (int j = 0; j < i; ++j) check(!meet(*written[i], *written[j]), "outputs must share no memory with each other");
         }
     } else {
-        const auto longs = context_lens.options().dtype(at::kLong);
-        slots = at::empty({num_tokens}, longs);
-        positions = at::empty({num_tokens}, longs);
-        lens = at::empty({S}, context_lens.options());
-        cu = at::empty({S + 1}, context_lens.options());
-        end = at::empty({1}, context_lens.options());
+        slots = new_tensor({num_tokens}, at::kLong, context_lens);
+        positions = new_tensor({num_tokens}, at::kLong, context_lens);
+        lens = new_tensor({S}, at::kInt, context_lens);
+        cu = new_tensor({S + 1}, at::kInt, context_lens);
+        end = new_tensor({1}, at::kInt, context_lens);
     }
     check(S <= 0x7fffffff - 1 && block_table.size(1) <= 0x7fffffff, "too many requests or pages");
     const int64_t row = S <= 1 ? block_table.size(1) : block_table.stride(0);
@@ -266,9 +271,9 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
               "out must be a contiguous GPU tensor with the shape and dtype of q");
         check(!may_meet(result, qc), "out must share no memory with q");
     } else {
-        result = at::empty(q.sizes(), q.options());
+        result = new_tensor(q.sizes(), q.scalar_type(), q);
     }
-    if (return_lse) lse = at::empty({S, HQ}, q.options().dtype(at::kFloat));
+    if (return_lse) lse = new_tensor({S, HQ}, at::kFloat, q);
     const int bs = int(key_cache.size(1)), mb = int(block_table.size(1));
     const size_t bytes = fq_paged_kv_decode_workspace_bytes(int(S), int(HQ), int(HKV), int(D), bs, mb);
     at::Tensor ws;
@@ -278,7 +283,7 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
         check(ws.is_contiguous() && ws.scalar_type() == at::kByte && size_t(ws.numel()) >= bytes,
               "workspace must be a contiguous uint8 GPU tensor of at least paged_kv_decode_workspace_bytes(...) bytes");
     } else if (bytes > 0) {
-        ws = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
+        ws = new_tensor({int64_t(bytes)}, at::kByte, q);
     }
     const int64_t qs[2] = {qc.stride(0), qc.stride(1)};
     const int st = fq_paged_kv_decode(qc.data_ptr(), qs, key_cache.data_ptr(), ks.s, value_cache.data_ptr(), vs.s, block_table.data_ptr<int32_t>(),

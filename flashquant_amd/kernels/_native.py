@@ -6,8 +6,15 @@ import torch
 from flashquant_amd import load_native
 
 
+_module = None
+
+
 def native():
-    return load_native()
+    # (an import statement costs a call most of a microsecond)
+    global _module
+    if _module is None:
+        _module = load_native()
+    return _module
 
 
 def require_gpu(t: torch.Tensor, name: str) -> None:

@@ -98,7 +98,7 @@ def test_rotary_rows_that_are_no_numbers_stay_in_their_pairs():
     assert bad[0, 0, 3] and bad[0, 0, 19] and out[1, 0, 40] == math.inf and int(bad.sum()) == 3
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
 @pytest.mark.parametrize("off", [0, 1, 8])
 def test_rotary_of_strided_rows_in_batches(dtype, off):
     """Slices of one matrix product, a batch with shared and with its own positions, heads before tokens, rows at odd addresses."""
@@ -123,6 +123,24 @@ def test_rotary_of_strided_rows_in_batches(dtype, off):
         want = qkv.clone()
         want[:, :, :hq, off:], want[:, :, hq:hq + hk, off:] = qo, ko
         assert torch.equal(whole, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_has_the_same_bits_at_every_size_and_alignment(interleaved, dtype):
+    """More than goes through the shared cache, a part of it, and rows at odd addresses."""
+    n, h, d, rot = 9000, 40, 256 if dtype != F32 else 128, 96
+    g = torch.Generator(device=DEV).manual_seed(8)
+    q = torch.randn(n, h, d, generator=g, device=DEV).to(dtype)
+    freq, scale = K.rotary_frequencies(rot, 500000.0, "bands", factor=8.0, original_max_position=8192, device=DEV)
+    positions = torch.randint(0, 131072, (n,), generator=g, device=DEV)
+    out, _ = K.rotary_embedding(q, None, positions, freq, interleaved=interleaved, scale=0.75)
+    check_turn(out[-500:], q[-500:], positions[-500:], freq, interleaved, 0.75)
+    part, _ = K.rotary_embedding(q[:777, :3], None, positions[:777], freq, interleaved=interleaved, scale=0.75)
+    assert torch.equal(part, out[:777, :3])
+    odd = torch.empty(n, h, d + 1, dtype=dtype, device=DEV)[..., 1:]
+    odd.copy_(q)
+    assert torch.equal(K.rotary_embedding(odd, None, positions, freq, interleaved=interleaved, scale=0.75)[0], out)
 
 
 def test_rotary_of_columns_apart_and_expanded_inputs():
@@ -329,6 +347,9 @@ def test_schedule_at_its_edges():
     run_schedule([3, 9], [0, 0], 4, [1], 0, 8, 0)
     run_schedule([3, 9], [1, 1], 4, [1], 0, 8, 0)                                                       # no room at all
     run_schedule([0] * 300 + [40], [0] * 300 + [600], 30, list(range(100)), 0, 32, 600)
+    # requests that the threads share out unevenly, and more than they take at a time
+    for n in (255, 256, 257, 511, 513, 1500, 2047, 2048, 2049, 5000):
+        run_schedule([i % 37 for i in range(n)], [i % 3 for i in range(n)], 6, list(range(n)), 2, 8, n + 1)
     # many requests of one token, and one request over many workgroups
     run_schedule(list(range(3000)), [1] * 3000, 400, list(range(3000)), 0, 8, 3000)
     run_schedule([1], [5000], 700, list(range(3000)), 0, 8, 5100)
