@@ -1,0 +1,189 @@
+"""Scheduling, rotary positions, stores and attention as a serving loop runs them: one page table, layers at 16 bits and packed,
+prompts, generated tokens, sequences that end and begin, and a captured step."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from flashquant_amd import kernels as K
+from flashquant_amd.cache import PagedKVLayer, PagedTQ4Layer, PageTable
+from flashquant_amd.vllm.impl import TQ4AttentionKernels
+from tests.test_gpu_paged_kv import attended
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HQ, HKV = 8, 8
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def qkv_of(tokens, d, dtype, g):
+    return (torch.randn(tokens, HQ + 2 * HKV, d, generator=g).to(dtype).to(DEV)).split([HQ, HKV, HKV], 1)
+
+
+class Told:
+    """What the layers hold, kept by sequence on the side: rotated keys and values, and the packed path on pages of its own."""
+
+    def __init__(self, seqs, d, page, dtype, freq, scale):
+        self.k = [torch.empty(0, HKV, d, dtype=dtype, device=DEV) for _ in range(seqs)]
+        self.v = [torch.empty_like(x) for x in self.k]
+        self.page, self.freq, self.scale, self.d = page, freq, scale, d
+        self.most = 40
+        self.cache = torch.zeros(seqs * self.most, page, HKV * (d + 8), dtype=torch.uint8, device=DEV)
+        self.table = torch.arange(seqs * self.most, dtype=torch.int32, device=DEV).view(seqs, self.most)
+        self.kernels = TQ4AttentionKernels(HKV, d, 1 / math.sqrt(d), torch.device(DEV))
+
+    def positions(self, counts):
+        return torch.cat([torch.arange(len(self.k[s]), len(self.k[s]) + n, device=DEV) for s, n in enumerate(counts)])
+
+    def add(self, counts, q, k, v):
+        """The rotated queries, and the slots of the tokens on this cache."""
+        q, k = K.rotary_embedding(q, k, self.positions(counts), self.freq, scale=self.scale)
+        at, slots = 0, []
+        for s, n in enumerate(counts):
+            p = torch.arange(len(self.k[s]), len(self.k[s]) + n, device=DEV)
+            slots.append(self.table[s].long()[p // self.page] * self.page + p % self.page)
+            self.k[s], self.v[s] = torch.cat([self.k[s], k[at:at + n]]), torch.cat([self.v[s], v[at:at + n]])
+            at += n
+        return q, k, torch.cat(slots)
+
+    def lens(self):
+        return i32([len(x) for x in self.k])
+
+    def forget(self, s):
+        self.k[s], self.v[s] = self.k[s][:0], self.v[s][:0]
+
+    def check(self, q, out):
+        """One query a sequence against the definition over what was kept."""
+        n = max(len(x) for x in self.k)
+        kc = torch.zeros(len(self.k), n, HKV, self.d, dtype=q.dtype, device=DEV)
+        vc = torch.zeros_like(kc)
+        for s, (k, v) in enumerate(zip(self.k, self.v)):
+            kc[s, :len(k)], vc[s, :len(v)] = k, v
+        want, _, tol, _ = attended(q, kc, vc, torch.arange(len(self.k), dtype=torch.int32, device=DEV)[:, None], self.lens(), 1 / math.sqrt(self.d))
+        off = (out.double() - want).abs() - tol
+        assert (off <= 0).all(), float(off.max())
+
+
+@pytest.mark.parametrize("d,page,dtype", [(128, 16, torch.bfloat16), (64, 32, torch.float16), (256, 8, torch.bfloat16)])
+def test_a_serving_loop(d, page, dtype):
+    seqs, g = 5, torch.Generator().manual_seed(d)
+    freq, scale = K.rotary_frequencies(d, 10000.0, "yarn", factor=4.0, original_max_position=64)
+    table = PageTable(5 * 300 // page + 7, page, seqs, 300 // page + 1)
+    plain, packed = PagedKVLayer(table, HKV, d, freq, scale, dtype=dtype), PagedTQ4Layer(table, HKV, d, freq, scale)
+    told = Told(seqs, d, page, dtype, freq.to(DEV), scale)
+    held = [0] * seqs
+    for turn, counts in enumerate([[37, 1, 100, 16, 64], [1] * 5, [1] * 5, [3, 70, 1, 16, 1], [1] * 5, "end 2", "end 0", [50, 1, 33, 1, 1], [1] * 5, [1] * 5]):
+        if isinstance(counts, str):
+            s = int(counts.split()[1])
+            table.release(s)
+            told.forget(s)
+            held[s] = 0
+            continue
+        tokens = sum(counts)
+        q, k, v = qkv_of(tokens, d, dtype, g)
+        step = table.schedule(i32(counts), tokens)
+        assert torch.equal(step.positions, told.positions(counts))
+        qr, kr, slots = told.add(counts, q, k, v)
+        lens = told.lens()
+        assert torch.equal(step.seq_lens, lens) and torch.equal(table.context_lens, lens)
+        # every page belongs to one sequence
+        held = [h + n for h, n in zip(held, counts)]
+        pages = torch.cat([table.block_table[s, :-(-h // page)] for s, h in enumerate(held)])
+        assert len(pages.unique()) == len(pages) and int(pages.min()) >= 0 and int(table.free_start) == len(pages)
+        if max(counts) == 1:
+            told.check(qr, plain.step(q, k, v, step))
+            got = packed.step(q, k, v, step)
+            want = told.kernels.decode_step(qr, kr, v, told.cache, slots, told.table[:, :table.block_table.shape[1]].contiguous(), lens)
+        else:
+            assert torch.equal(plain.store(q, k, v, step), qr)
+            got = packed.prefill(q, k, v, step, max(counts))
+            told.kernels.compress_and_store(kr, v, told.cache, slots)
+            want = told.kernels.prefill(qr, step.cu_seqlens, max(counts), told.cache, told.table[:, :table.block_table.shape[1]].contiguous(), lens)
+        assert torch.equal(got, want), turn
+
+
+def test_a_page_table_that_runs_out_and_recovers():
+    table = PageTable(6, 16, 2, 10)
+    step = table.schedule(i32([40, 70]), 110)              # 3 + 5 pages
+    assert int(step.pages_taken) == 8 and int(table.free_start) == 6
+    assert step.block_table[0].tolist()[:4] == [0, 1, 2, -1] and step.block_table[1].tolist()[:6] == [3, 4, 5, -1, -1, -1]
+    assert (step.slot_mapping[40 + 48:] == -1).all() and (step.slot_mapping[:88] >= 0).all()
+    table.release(1)
+    assert int(table.free_start) == 3 and sorted(table.free_blocks[3:].tolist()) == [3, 4, 5]
+    table.release(0)
+    assert int(table.free_start) == 0 and sorted(table.free_blocks.tolist()) == list(range(6))
+    table.release(0)                                        # nothing held
+    assert int(table.free_start) == 0
+    step = table.schedule(i32([96, 0]), 96)
+    assert sorted(step.slot_mapping.tolist()) == list(range(96))
+
+
+@pytest.mark.parametrize("d,first", [(128, 700), (64, 3)])
+def test_a_captured_step(d, first):
+    """Replays, with eager work of the same kind between them, give what the eager step gives."""
+    seqs, page, dtype = 4, 16, torch.bfloat16
+    freq, _ = K.rotary_frequencies(d)
+
+    def model():
+        table = PageTable(seqs * 60, page, seqs, 60)
+        return table, PagedKVLayer(table, HKV, d, freq, dtype=dtype), PagedTQ4Layer(table, HKV, d, freq)
+
+    def fill(table, plain, packed):
+        g = torch.Generator().manual_seed(1)
+        counts = [first, 1, first // 2 + 1, 15]
+        q, k, v = qkv_of(sum(counts), d, dtype, g)
+        step = table.schedule(i32(counts), sum(counts))
+        plain.store(q, k, v, step)
+        packed.store(q, k, v, step)
+
+    ones = i32([1] * seqs)
+
+    def run(m, q, k, v):
+        step = m[0].schedule(ones, seqs)
+        return m[1].step(q, k, v, step), m[2].step(q, k, v, step), step.slot_mapping
+
+    eager, captured, warm = model(), model(), model()
+    for m in (eager, captured, warm):
+        fill(*m)
+    inputs = [torch.empty(seqs, h, d, dtype=dtype, device=DEV) for h in (HQ, HKV, HKV)]
+    g = torch.Generator().manual_seed(2)
+    for x, y in zip(inputs, qkv_of(seqs, d, dtype, g)):
+        x.copy_(y)
+    run(warm, *inputs)                                      # loads what a first call loads
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(captured, *inputs)
+    for turn in range(20):                                  # over the ends of pages
+        for x, y in zip(inputs, qkv_of(seqs, d, dtype, g)):
+            x.copy_(y)
+        graph.replay()
+        want = run(eager, *inputs)
+        torch.cuda.synchronize()
+        for got, w in zip(out, want):
+            assert torch.equal(got, w), turn
+    assert torch.equal(captured[0].context_lens, eager[0].context_lens)
+
+
+def test_calls_on_another_stream():
+    d, dtype = 128, torch.bfloat16
+    freq, _ = K.rotary_frequencies(d, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    kc, vc = (torch.randn(90, 16, HKV, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    table = torch.randperm(90, generator=g).int().view(1, 90).to(DEV)
+    q, k, v = qkv_of(1, d, dtype, g)
+    lens, slot = i32([1440]), table[0, -1:].long() * 16 + 15
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mine = kc.clone(), vc.clone()
+        out = K.paged_kv_decode(K.rotary_paged_store(q, k, v, slot, slot, freq, *mine), *mine, table, lens)
+        s = K.paged_schedule(i32([1439]), i32([1]), table.clone(), i32([5]), 16, 1)
+    side.synchronize()
+    want = K.paged_kv_decode(K.rotary_paged_store(q, k, v, slot, slot, freq, kc, vc), kc, vc, table, lens)
+    assert torch.equal(out, want) and torch.equal(mine[0], kc) and torch.equal(s.slot_mapping, slot)
