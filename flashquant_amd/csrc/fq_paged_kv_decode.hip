@@ -132,17 +132,16 @@ template <int DT> __device__ __forceinline__ float high_value(uint32_t w) {
     else return f16_to_float(uint16_t(w >> 16));
 }
 
-// Words of a lane's piece of one value row: 8 coordinates of 128, 4 of 64.
-template <int D> struct ValueWords { static constexpr int n = D == 64 ? 2 : 4; };
+// HW heads of a workgroup, TW wavefronts of each; SHARED: a share of all tiles, else one sequence.
 
 template <int D, int DT, int HW, int TW, bool SHARED>
 __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const KvDecodeParams p) {
     constexpr int KP = D / 64;                       // lines of 128 bytes of a key
     constexpr int VH = D == 256 ? 2 : 1;             // halves of 128 coordinates
-    constexpr int VW = ValueWords<D>::n;
-    constexpr int VE = 2 * VW;                       // coordinates of a lane's piece
+    constexpr int VW = D == 64 ? 2 : 4;              // words of a lane's piece of a value row
+    constexpr int VE = 2 * VW;                       // its coordinates
     constexpr int W = HW * TW;
-    extern __shared__ __align__(16) float lds[];     // (W, G, D), then (W, 2, 16), then (2, 16)
+    extern __shared__ __align__(16) float lds[];     // (W, G, D), then (W, 2, 16), then (HW, 16)
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n = lane & 15, g = lane >> 4, kgroup = (n >> 2) & 1;
     const int G = p.G;
@@ -440,11 +439,11 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
                 for (int w = 1; w < TW; ++w) o += *reinterpret_cast<const float4v*>(lds + w * HW * G * D + i);
                 const int h = i / D;
                 const float inv = scale[h / G * 16 + h % G];
-                const int64_t first = -int64_t(mine) * G * D + i;        // from this wavefront's head to the group's first
+                const int64_t at = i - int64_t(mine) * G * D;        // from this wavefront's head on
                 if (complete)
-                    *reinterpret_cast<uint2v*>(p.out + orow * D + first) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
+                    *reinterpret_cast<uint2v*>(p.out + orow * D + at) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
                 else
-                    *reinterpret_cast<float4v*>(p.part_o + row * D + first) = o;
+                    *reinterpret_cast<float4v*>(p.part_o + row * D + at) = o;
             }
         }
         if constexpr (SHARED) {
@@ -511,25 +510,45 @@ __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams
 
 namespace {
 
-// KV heads that a workgroup takes together, and the wavefronts of a workgroup.
-int kv_heads_together(int H_KV) { return H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1; }
-constexpr int kv_waves(int D) { return D == 256 ? 4 : 8; }
+// How a call is divided.
+struct KvPlan {
+    int shares;          // workgroups among which the tiles of a KV head are divided; 0: one a sequence, and no second launch
+    int heads, waves;    // KV heads of a workgroup, wavefronts of each
+};
 
-// Among how many workgroups the tiles of a KV head are divided; 0: one workgroup a sequence, and no second launch.  A CU draws at
-// most about 43 GB/s for itself, so few long sequences have to be spread, but the second launch costs 4 us, and a share that goes
-// on with another sequence starts from nothing again (3 us).  In us, undivided / divided, 32 heads over 8 of 128, bf16: 1 x 500
-// tokens 9.3 / 11.9, 1 x 777 11.2 / 12.2, 1 x 1000 15.5 / 12.9, 1 x 2000 27.3 / 13.4, 16 x 1000 18.4 / 18.7, 32 x 1000 23.9 /
-// 27.6, 32 x 2000 43.7 / 46.9, 64 x 1000 47.2 / 48.5, 200 of 100 to 2000 175 / 158; 8 heads over 1: 128 of 100 to 700 12.9 / 19.2,
-// 64 of 200 to 1500 20.1 / 16.6, 300 of them 30.7 / 37.8; 32 over 32, 16 of 300 to 1000 38.7 / 35.8.
-int kv_shares(int S, int H_KV, int64_t max_tokens, int window) {
+// Undivided sequences or shares: a CU takes its tiles at 40 to 60 GB/s, so few long sequences have to be spread, but the
+// second launch costs 4 us, and a share that goes on with another sequence starts from nothing again (3 us).  In us, undivided /
+// shares, 32 heads over 8 of 128, bf16: 1 x 500 tokens 9.3 / 10.0, 1 x 1000 15.5 / 10.9, 4 x 500 10.4 / 10.4, 16 x 500 11.4 / 14.5,
+// 16 x 1000 18.4 / 18.5, 32 x 1000 23.9 / 27.5, 32 x 2000 43.7 / 46.9, 64 x 1000 47.2 / 48.5, 200 of 100 to 2000 175 / 158; 8 heads
+// over 1: 32 of 100 to 700 11.7 / 12.7, 128 of them 12.9 / 16.7, 64 of 200 to 1500 20.1 / 16.5, 300 of them 30.7 / 37.4; 32 over 32,
+// 16 of 300 to 1000 38.7 / 35.8.
+// The workgroup: four heads and two wavefronts of each draw best where there is much (see above); where a call has at most two
+// tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.9 -> 10.9 us,
+// 1 x 4000 14.3 -> 12.7, 8 heads over 1, 4 x 1500 15.0 -> 12.8; but 61 of 500 to 16000 343 -> 355.
+KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {
     int64_t tiles = (max_tokens + fq::kKvTile - 1) / fq::kKvTile;
     if (window > 0 && window / fq::kKvTile + 2 < tiles) tiles = window / fq::kKvTile + 2;
     const int64_t whole = int64_t(S) * H_KV, cus = fq_host::device_cu_count();
-    if (tiles <= 25 || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus)) return 0;
-    if (int64_t(S) * tiles >= (1LL << 31)) return 0;         // more tiles than are counted
-    const int groups = H_KV / kv_heads_together(H_KV);
-    return int((cus + groups - 1) / groups);                 // a workgroup a CU: more are no faster (two: 32 x 4096 86.7 -> 96)
+    const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
+    KvPlan r = {0, 1, most};
+    if (tiles <= 16 || (tiles <= 25 && whole >= 16) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
+        int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
+        if (together == 4 && whole >= 8 * cus) {
+            // fewer workgroups: 256 of 50 to 300 tokens, 32 heads over 8 of 128, 40 us; 52 with a head a workgroup
+            r.heads = 4;
+            r.waves = most / 4;
+        }
+        return r;
+    }
+    const bool few = D != 256 && whole * tiles <= 16 * cus;
+    r.heads = few && together == 4 ? 2 : together;
+    r.waves = (few ? 4 : most) / r.heads;
+    // as many workgroups as run at a time: more are no faster (two rounds, 32 x 4096: 86.7 -> 96 us)
+    r.shares = int(((few ? 2 : 1) * cus * r.heads + H_KV - 1) / H_KV);
+    return r;
 }
+// the most shares of any of these plans, and of those for a window
+int kv_most_shares(int H_KV) { return int((4 * int64_t(fq_host::device_cu_count()) + H_KV - 1) / H_KV); }
 
 int check_kv_shape(int S, int H_Q, int H_KV, int D, int block_size, int max_blocks, int64_t num_blocks) {
     if (S < 0 || H_Q <= 0 || H_KV <= 0 || max_blocks <= 0 || num_blocks <= 0) return FQ_ERR_BAD_SHAPE;
@@ -564,13 +583,13 @@ int launch_attend(const fq::KvDecodeParams& p, hipStream_t s) {
 }
 
 template <int D, int DT>
-int launch_kv(const fq::KvDecodeParams& p, hipStream_t s) {
-    constexpr int W = kv_waves(D);
-    const int hw = kv_heads_together(p.H_KV);
+int launch_kv(const fq::KvDecodeParams& p, const KvPlan& plan, hipStream_t s) {
+    constexpr int W = D == 256 ? 4 : 8;
     int st;
-    if (p.shares > 0) {
-        st = hw == 4 ? launch_attend<D, DT, 4, W / 4, true>(p, s)
-                     : hw == 2 ? launch_attend<D, DT, 2, W / 2, true>(p, s) : launch_attend<D, DT, 1, W, true>(p, s);
+    if (plan.shares > 0) {
+        if (plan.heads == 4) st = launch_attend<D, DT, 4, W / 4, true>(p, s);
+        else if (plan.heads == 2) st = plan.waves == W / 2 ? launch_attend<D, DT, 2, W / 2, true>(p, s) : launch_attend<D, DT, 2, 2, true>(p, s);
+        else st = plan.waves == W ? launch_attend<D, DT, 1, W, true>(p, s) : launch_attend<D, DT, 1, 4, true>(p, s);
         if (st != FQ_OK) return st;
         // as many values a workgroup as leave enough workgroups
         const int64_t values = int64_t(p.S) * p.H_KV * p.G * D;
@@ -578,8 +597,7 @@ int launch_kv(const fq::KvDecodeParams& p, hipStream_t s) {
             fq::paged_kv_join_kernel<D, DT, 64><<<unsigned(values / 256), 256, 0, s>>>(p);
         else
             fq::paged_kv_join_kernel<D, DT, 16><<<unsigned(values / 64), 256, 0, s>>>(p);
-    } else if (hw == 4 && int64_t(p.S) * p.H_KV >= 8 * fq_host::device_cu_count()) {
-        // many sequences: fewer workgroups (256 of 50 to 300 tokens, 32 heads over 8 of 128: 40 us, 52 with a head a workgroup)
+    } else if (plan.heads == 4) {
         st = launch_attend<D, DT, 4, W / 4, false>(p, s);
     } else {
         st = launch_attend<D, DT, 1, W, false>(p, s);
@@ -588,16 +606,18 @@ int launch_kv(const fq::KvDecodeParams& p, hipStream_t s) {
 }
 
 template <int D>
-int launch_kv_type(const fq::KvDecodeParams& p, int dtype, hipStream_t s) {
-    return dtype == FQ_BF16 ? launch_kv<D, FQ_BF16>(p, s) : launch_kv<D, FQ_F16>(p, s);
+int launch_kv_type(const fq::KvDecodeParams& p, const KvPlan& plan, int dtype, hipStream_t s) {
+    return dtype == FQ_BF16 ? launch_kv<D, FQ_BF16>(p, plan, s) : launch_kv<D, FQ_F16>(p, plan, s);
 }
 
 }  // namespace
 
 extern "C" size_t fq_paged_kv_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq) {
     if (check_kv_shape(num_seqs, H_Q, H_KV, D, block_size, max_blocks_per_seq, 1) != FQ_OK || num_seqs == 0) return 0;
-    const int shares = kv_shares(num_seqs, H_KV, int64_t(max_blocks_per_seq) * block_size, 0);     // (a window only takes from it)
-    return kv_room(num_seqs, H_Q, D, shares).all;
+    // (a window only takes tiles away: what needs none without it needs none with it, but for tiles beyond what is counted)
+    const int64_t tokens = int64_t(max_blocks_per_seq) * block_size;
+    if (kv_plan(num_seqs, H_KV, D, tokens, 0).shares == 0 && int64_t(num_seqs) * (tokens / fq::kKvTile + 1) < (1LL << 31)) return 0;
+    return kv_room(num_seqs, H_Q, D, kv_most_shares(H_KV)).all;
 }
 
 extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
@@ -618,9 +638,10 @@ extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const
     }
     if (!fq_host::aligned(q, 16) || !fq_host::aligned(key_cache, 16) || !fq_host::aligned(value_cache, 16) || !fq_host::aligned(out, 16))
         return FQ_ERR_MISALIGNED;
-    const int shares = kv_shares(num_seqs, H_KV, int64_t(max_blocks_per_seq) * block_size, window);
-    if ((int64_t(num_seqs) + shares) * H_Q * (D / 32) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
-    const KvRoom room = kv_room(num_seqs, H_Q, D, shares);
+    const KvPlan plan = kv_plan(num_seqs, H_KV, D, int64_t(max_blocks_per_seq) * block_size, window);
+    const int most = plan.shares == 0 ? 0 : kv_most_shares(H_KV);
+    if ((int64_t(num_seqs) + most) * H_Q * (D / 32) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    const KvRoom room = kv_room(num_seqs, H_Q, D, most);
     if (room.all > 0) {
         if (!workspace || workspace_bytes < room.all) return FQ_ERR_WORKSPACE;
         if (!fq_host::aligned(workspace, 256)) return FQ_ERR_MISALIGNED;
@@ -644,12 +665,12 @@ extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const
     p.S = num_seqs; p.H_KV = H_KV; p.G = H_Q / H_KV;
     p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
     p.max_blocks = max_blocks_per_seq; p.num_blocks = int(num_blocks); p.window = window;
-    p.shares = shares; p.min_tiles = kv_waves(D) / kv_heads_together(H_KV);      // a tile a wavefront
+    p.shares = plan.shares; p.min_tiles = plan.waves;        // a tile a wavefront
     p.scale_log2 = sm_scale * fq::kLog2e;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (D) {
-        case 64: return launch_kv_type<64>(p, dtype, s);
-        case 128: return launch_kv_type<128>(p, dtype, s);
-        default: return launch_kv_type<256>(p, dtype, s);
+        case 64: return launch_kv_type<64>(p, plan, dtype, s);
+        case 128: return launch_kv_type<128>(p, plan, dtype, s);
+        default: return launch_kv_type<256>(p, plan, dtype, s);
     }
 }

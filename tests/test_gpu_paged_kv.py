@@ -584,6 +584,19 @@ def test_decode_of_nothing_and_refusals():
         K.paged_kv_decode(q, kc, vc, long, sl, workspace=torch.empty(256, dtype=torch.uint8, device=DEV))
 
 
+@pytest.mark.parametrize("seqs", [1, 5, 40, 300])
+@pytest.mark.parametrize("columns", [10, 33, 60, 130, 700])
+def test_decode_has_room_for_every_window(seqs, columns):
+    """What a call without a window needs suffices with one, however the work is divided then."""
+    g = gen(columns)
+    kc, vc, _ = caches("apart", 50, 16, 4, 64, BF, g)
+    table = torch.randint(0, 50, (seqs, columns), dtype=torch.int32, generator=g).to(DEV)
+    lens = torch.randint(0, 16 * columns + 1, (seqs,), dtype=torch.int32, generator=g).to(DEV)
+    q = torch.randn(seqs, 4, 64, generator=g).to(BF).to(DEV)
+    outs = [K.paged_kv_decode(q, kc, vc, table, lens, window=w).float() for w in (0, 1, 300, 900, 3000, 1 << 20)]
+    assert torch.equal(outs[5], outs[0]) and all(torch.isfinite(o).all() for o in outs)
+
+
 def test_decode_joins_two_caches_by_their_normalisers():
     q, kc, vc, table, sl = decode_case([1500], 8, 2, 128, 16, HF, seed=4)
     first = torch.tensor([800], dtype=torch.int32, device=DEV)

@@ -171,3 +171,4 @@ def test_decode_argument_errors_and_sizes(lib):
     assert call(columns=4000, ws=320, room=bytes_) == FQ_ALIGN
     assert need(2, 8, 2, 96, 16, 4000) == 0 and need(0, 8, 2, 128, 16, 4000) == 0
     assert need(1, 8, 2, 128, 16, 4) == 0                                  # a context of one part
+    assert need(70000, 8, 8, 64, 32, 1 << 16) > 0                          # more tiles than are counted, fewer with a window
