@@ -101,9 +101,8 @@ Angles angles_of(const at::Tensor& positions, const at::Tensor& inv_freq, const 
     return a;
 }
 
-std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions,
-                                                     const at::Tensor& inv_freq, bool interleaved, double scale, bool inverse,
-                                                     const MaybeTensor& q_out, const MaybeTensor& k_out) {
+std::tuple<at::Tensor, MaybeTensor> rotate(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions, const at::Tensor& inv_freq,
+                                           bool interleaved, double scale, bool inverse, const MaybeTensor& q_out, const MaybeTensor& k_out) {
     fqbind::require_gpu(q, "q");
     check(q.dim() == 3 || q.dim() == 4, "q must have shape (tokens, H, D) or (batch, tokens, H, D)");
     check(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kFloat, "q must be float16, bfloat16 or float32");
@@ -137,6 +136,52 @@ std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const 
         fqbind::raise_on_error(st, "rotary_embedding");
     }
     return {qo, k.has_value() ? MaybeTensor(ko) : std::nullopt};
+}
+
+std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions,
+                                                     const at::Tensor& inv_freq, bool interleaved, double scale, bool inverse,
+                                                     const MaybeTensor& q_out, const MaybeTensor& k_out);
+
+// The rotation is linear and its transpose the rotation by the negative angles: the gradient is the same operator, as often as it
+// is asked for.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const MaybeTensor& k,
+                                                  const at::Tensor& positions, const at::Tensor& inv_freq, bool interleaved, double scale,
+                                                  bool inverse) {
+        ctx->save_for_backward({positions, inv_freq});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["inverse"] = inverse;
+        ctx->set_materialize_grads(false);
+        auto [qo, ko] = rotate(q, k, positions, inv_freq, interleaved, scale, inverse, std::nullopt, std::nullopt);
+        torch::autograd::variable_list r = {qo};
+        if (ko.has_value()) r.push_back(*ko);
+        return r;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+        const auto saved = ctx->get_saved_variables();
+        const bool dq = grads[0].defined() && ctx->needs_input_grad(0);
+        const bool dk = grads.size() > 1 && grads[1].defined() && ctx->needs_input_grad(1);
+        torch::autograd::variable_list r(7);
+        if (!dq && !dk) return r;
+        auto [a, b] = rotary_embedding(dq ? grads[0] : grads[1], dq && dk ? MaybeTensor(grads[1]) : std::nullopt, saved[0], saved[1],
+                                       ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble(),
+                                       !ctx->saved_data["inverse"].toBool(), std::nullopt, std::nullopt);
+        if (dq) r[0] = a;
+        if (dk) r[1] = dq ? *b : a;
+        return r;
+    }
+};
+
+std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions,
+                                                     const at::Tensor& inv_freq, bool interleaved, double scale, bool inverse,
+                                                     const MaybeTensor& q_out, const MaybeTensor& k_out) {
+    if (at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad()))) {
+        check(!q_out.has_value() && !k_out.has_value(), "out cannot be combined with gradients");
+        const auto r = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, scale, inverse);
+        return {r[0], r.size() > 1 ? MaybeTensor(r[1]) : std::nullopt};
+    }
+    return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out);
 }
 
 struct Cache {

@@ -84,28 +84,6 @@ def rotary_frequencies(
     return inv_freq.to(device) if device is not None else inv_freq, scale
 
 
-class _Rotary(torch.autograd.Function):
-    """The rotation is linear and its transpose the rotation by the negative angles, so the gradient is the same operator."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.how = interleaved, scale, inverse
-        ctx.set_materialize_grads(False)
-        return native().rotary_embedding(q, k, positions, inv_freq, interleaved, scale, inverse)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        positions, inv_freq = ctx.saved_tensors
-        interleaved, scale, inverse = ctx.how
-        dq, dk = (g if needed else None for g, needed in zip((dq, dk), ctx.needs_input_grad))
-        if dq is None and dk is None:
-            return (None,) * 7
-        first, second = (dk, None) if dq is None else (dq, dk)
-        first, second = _Rotary.apply(first, second, positions, inv_freq, interleaved, scale, not inverse)
-        return ((None, first) if dq is None else (first, second)) + (None,) * 5
-
-
 def rotary_embedding(
     q: torch.Tensor,
     k: Optional[torch.Tensor],
@@ -126,10 +104,6 @@ def rotary_embedding(
     ``out`` = (q_out, k_out): written instead of new tensors; either may be its input itself.  Differentiable with respect to q and
     k (any number of times) where ``out`` is not given."""
     require_gpu(q, "q")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        if out is not None:
-            raise ValueError("out cannot be combined with gradients")
-        return _Rotary.apply(q, k, positions, inv_freq, interleaved, scale, inverse)
     q_out, k_out = (None, None) if out is None else out
     return native().rotary_embedding(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out)
 
