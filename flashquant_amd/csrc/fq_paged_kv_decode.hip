@@ -83,14 +83,25 @@ struct KvPlace {
     int seq, before;                      // a sequence, and the tiles of those before it
     KvSpan span;
 };
-__device__ __forceinline__ int kv_tiles_of(const KvDecodeParams& p, int s) { return s < p.S ? kv_span(p, p.lens[s]).tiles : 0; }
+__device__ __forceinline__ int kv_len_of(const KvDecodeParams& p, int s) { return s < p.S ? p.lens[s] : 0; }
+
+// The sum over this lane and those before it (a wavefront's length in six vector instructions).
+__device__ __forceinline__ int sum_upto(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // row_bcast:31 into rows 2 and 3
+    return v;
+}
 
 // `of_seq`: the place of sequence x; else of the sequence that holds the first tile of share x.  False: there is no such tile.
 template <bool of_seq>
 __device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lane, KvPlace& r) {
-    const int first = kv_tiles_of(p, lane);                  // (up to 64 sequences are read once)
-    uint32_t total = uint32_t(first);
-    for (int s = kWave; s < p.S; s += kWave) total += uint32_t(kv_tiles_of(p, s + lane));
+    const int len0 = kv_len_of(p, lane);                     // (up to 64 sequences are read once)
+    uint32_t total = uint32_t(kv_span(p, len0).tiles);
+    for (int s = kWave; s < p.S; s += kWave) total += uint32_t(kv_span(p, kv_len_of(p, s + lane)).tiles);
     total = wave_sum(total);
     const int share = int((total + uint32_t(p.shares) - 1) / uint32_t(p.shares));
     r.size = share > p.min_tiles ? share : p.min_tiles;
@@ -98,18 +109,14 @@ __device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lan
     if (!of_seq && wanted >= int64_t(total)) return false;
     int before = 0;
     for (int s = 0; s < p.S; s += kWave) {
-        const int n = s == 0 ? first : kv_tiles_of(p, s + lane);
-        int upto = n;                                        // inclusive sum over the lanes
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const int below = __shfl_up(upto, d, kWave);
-            upto += lane >= d ? below : 0;
-        }
+        const int len = s == 0 ? len0 : kv_len_of(p, s + lane);
+        const int n = kv_span(p, len).tiles, upto = sum_upto(n);
         const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
         if (of_seq ? x < s + kWave : wanted < int64_t(before) + all) {
             const int at = of_seq ? x - s : __ffsll(static_cast<unsigned long long>(__ballot(before + upto > int(wanted)))) - 1;
             r.seq = s + at;
             r.before = before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
+            r.span = kv_span(p, __builtin_amdgcn_readlane(len, at));
             return true;
         }
         before += all;
@@ -210,8 +217,8 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
     };
 
     int seq = x, offset = 0, left = 0;               // the sequence, its first tile here, the tiles left of the share
+    KvPlace at;
     if constexpr (SHARED) {
-        KvPlace at;
         if (!kv_place<false>(p, x, lane, at)) return;
         seq = at.seq;
         offset = x * at.size - at.before;
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
 #pragma unroll
             for (int j = 0; j < 2 * KP; ++j) qr[j] = *reinterpret_cast<const uint4v*>(src + 32 * j);
         }
-        const KvSpan span = kv_span(p, p.lens[seq]);
+        const KvSpan span = SHARED && !again ? at.span : kv_span(p, p.lens[seq]);
         const int count = !SHARED || span.tiles - offset < left ? span.tiles - offset : left;
         const int end = span.first + offset + count;
 
@@ -451,7 +458,7 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
             offset = 0;
             again = true;
             do ++seq;
-            while (left > 0 && seq < p.S && kv_tiles_of(p, seq) == 0);   // (sequences of no tokens: the second launch)
+            while (left > 0 && seq < p.S && kv_span(p, p.lens[seq]).tiles == 0);   // (sequences of no tokens: the second launch)
         }
     } while (SHARED && left > 0 && seq < p.S);
 }
@@ -471,7 +478,7 @@ __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams
     const int c = 4 * (int(blockIdx.x % columns) * Q + threadIdx.x % Q), r0 = threadIdx.x / Q, h = c / D;
     KvPlace at;
     kv_place<true>(p, seq, lane, at);
-    const int tiles = kv_tiles_of(p, seq);
+    const int tiles = at.span.tiles;
     const int share0 = at.before / at.size, share1 = tiles > 0 ? (at.before + tiles - 1) / at.size : share0;
     const int pieces = tiles > 0 ? share1 - share0 + 1 : 0;
     if (pieces == 1) return;
