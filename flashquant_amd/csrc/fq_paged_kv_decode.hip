@@ -27,7 +27,7 @@
 //     that shows is that of the output; the matrix cores are idle otherwise.  Maximum and sum are float32, of the unrounded
 //     weights.
 // Measured: 32 sequences of 4096 tokens, 32 heads over 8 of 128, bf16, 84.6 us (6.35 TB/s); 61 of 500 to 16000, 64 over 8, fp16, 342.6 us
-// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 22.8 us; one of 777, 32 over 8, 10.7 us.
+// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 22.7 us; one of 777, 32 over 8, 9.0 us.
 #include <type_traits>
 
 #include "fq_device.hpp"
@@ -523,22 +523,22 @@ struct KvPlan {
     int heads, waves;    // KV heads of a workgroup, wavefronts of each
 };
 
-// Undivided sequences or shares: a CU takes its tiles at 40 to 60 GB/s, so few long sequences have to be spread, but the
-// second launch costs 4 us, and a share that goes on with another sequence starts from nothing again (3 us).  In us, undivided /
-// shares, 32 heads over 8 of 128, bf16: 1 x 500 tokens 9.3 / 10.0, 1 x 1000 15.5 / 10.9, 4 x 500 10.4 / 10.4, 16 x 500 11.4 / 14.5,
-// 16 x 1000 18.4 / 18.5, 32 x 1000 23.9 / 27.5, 32 x 2000 43.7 / 46.9, 64 x 1000 47.2 / 48.5, 200 of 100 to 2000 175 / 158; 8 heads
-// over 1: 32 of 100 to 700 11.7 / 12.7, 128 of them 12.9 / 16.7, 64 of 200 to 1500 20.1 / 16.5, 300 of them 30.7 / 37.4; 32 over 32,
-// 16 of 300 to 1000 38.7 / 35.8.
+// Undivided sequences or shares: a CU takes its tiles at 40 to 60 GB/s, so few long sequences have to be spread, but the second
+// launch costs 3 us, and a share that goes on with another sequence starts from nothing again (3 us).  In us, undivided / shares,
+// 32 heads over 8 of 128, bf16: 1 x 200 tokens 6.2 / 8.6, 1 x 500 9.8 / 9.3, 1 x 777 11.3 / 9.6, 1 x 2000 28.4 / 10.6, 4 x 500 10.6 /
+// 9.7, 16 x 500 12.0 / 14.3, 16 x 1000 18.5 / 18.5, 32 x 1000 25.0 / 27.9, 32 x 2000 45.6 / 48.5, 64 x 1000 47.4 / 48.2, 200 of
+// 100 to 2000 181 / 162; 8 heads over 1: 32 of 100 to 700 11.5 / 12.7, 128 of them 12.9 / 16.6, 64 of 200 to 1500 20.2 / 16.1, 300
+// of them 30.6 / 36.8; 32 over 32, 16 of 300 to 1000 38.7 / 36.2.
 // The workgroup: four heads and two wavefronts of each draw best where there is much (see above); where a call has at most two
-// tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.9 -> 10.9 us,
-// 1 x 4000 14.3 -> 12.7, 8 heads over 1, 4 x 1500 15.0 -> 12.8; but 61 of 500 to 16000 343 -> 355.
+// tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.2 -> 10.1 us,
+// 1 x 4000 13.6 -> 12.0, 8 heads over 1, 4 x 1500 14.6 -> 12.6; but 61 of 500 to 16000 343 -> 355.
 KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {
     int64_t tiles = (max_tokens + fq::kKvTile - 1) / fq::kKvTile;
     if (window > 0 && window / fq::kKvTile + 2 < tiles) tiles = window / fq::kKvTile + 2;
     const int64_t whole = int64_t(S) * H_KV, cus = fq_host::device_cu_count();
     const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
     KvPlan r = {0, 1, most};
-    if (tiles <= 16 || (tiles <= 25 && whole >= 16) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
+    if (tiles <= most || (tiles <= 25 && whole >= 32) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
         int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
         if (together == 4 && whole >= 8 * cus) {
             // fewer workgroups: 256 of 50 to 300 tokens, 32 heads over 8 of 128, 40 us; 52 with a head a workgroup
