@@ -493,23 +493,49 @@ __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams
         sum = sum * a + l * b;
         top = higher;
     };
-    for (int i = r0; i < pieces; i += R) {
-        const int64_t row = first + i * step;
-        take(*reinterpret_cast<const float4v*>(p.part_o + row * D + c), p.part_m[row + h], p.part_l[row + h]);
+    if (pieces <= R) {                                                   // (most sequences: one trip, nothing read twice)
+        if (r0 < pieces) {
+            const int64_t row = first + r0 * step;
+            o = *reinterpret_cast<const float4v*>(p.part_o + row * D + c);
+            top = p.part_m[row + h];
+            sum = p.part_l[row + h];
+        }
+    } else {
+        for (int i = r0; i < pieces; i += 4 * R) {                       // four pieces a trip
+            float4v v[4];
+            float m[4], l[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t row = first + (i + k * R < pieces ? i + k * R : i) * step;
+                v[k] = *reinterpret_cast<const float4v*>(p.part_o + row * D + c);
+                m[k] = p.part_m[row + h];
+                l[k] = p.part_l[row + h];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k * R < pieces) take(v[k], m[k], l[k]);
+        }
     }
-    if (R > 1) {
-        rows[r0][threadIdx.x % Q] = o;
-        sums[r0][threadIdx.x % Q] = float2v{top, sum};
-        __syncthreads();
-    }
+    // the R rows' results, weighed against the highest maximum and added (a row without pieces has a sum of zero, so weight 0)
+    const int q = threadIdx.x % Q;
+    sums[r0][q] = float2v{top, sum};
+    __syncthreads();
+    float highest = -__builtin_inff(), den = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) highest = __builtin_fmaxf(highest, sums[r][q].x);
+#pragma unroll
+    for (int r = 0; r < R; ++r) den += sums[r][q].y * piece_weight(sums[r][q].x, sums[r][q].y, highest);
+    rows[r0][q] = o * piece_weight(top, sum, highest);
+    __syncthreads();
     if (threadIdx.x < Q) {
-        const int used = pieces < R ? pieces : R;
-        for (int r = 1; r < used; ++r) take(rows[r][threadIdx.x], sums[r][threadIdx.x].x, sums[r][threadIdx.x].y);
-        const float inv = inverse_sum(sum);
+        float4v all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < R; ++r) all += rows[r][q];
+        const float inv = inverse_sum(den);
         const int64_t out = group * p.G;
-        *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
+        *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(all.x * inv, all.y * inv), round_pair<DT>(all.z * inv, all.w * inv)};
         if (c % D == 0 && p.lse != nullptr)
-            p.lse[out + h] = sum == 0.0f ? -__builtin_inff() : (top - kKvLift + __builtin_amdgcn_logf(sum)) * (1.0f / kLog2e);
+            p.lse[out + h] = den == 0.0f ? -__builtin_inff() : (highest - kKvLift + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
     }
 }
 
