@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from flashquant_amd import kernels as K
+from flashquant_amd.kernels._native import native
 from flashquant_amd.vllm.impl import TQ4AttentionKernels
 
 pytestmark = pytest.mark.gpu
@@ -460,6 +461,17 @@ def test_decode_of_many_sequences(lens):
     out, lse = check_decode(q, kc, vc, table, sl)
     again, lse2 = K.paged_kv_decode(q, kc, vc, table, sl, return_lse=True)
     assert torch.equal(out, again) and torch.equal(lse, lse2)              # the same call, the same bits
+
+
+# rows of no tokens before, between and after those that have some, by the tens and the hundreds; and so many sequences that their
+# lengths are read in several parts
+@pytest.mark.parametrize("lens", [[0] * 600 + [2100] + [0] * 130 + [5, 3000] + [0] * 700, [1700, 40] + [0] * 254, [0] * 63 + [4000] + [0] * 64 + [3000, 0],
+                                  [900] * 20 + [0] * 500 + [1200] * 30, [n % 97 for n in range(1130)], [0] * 1100, [0] * 1023 + [5000]])
+def test_decode_of_padded_batches(lens):
+    q, kc, vc, table, sl = decode_case(lens, 8, 2, 64, 32, BF, seed=len(lens), extra_columns=80)
+    ws = torch.full((native().paged_kv_decode_workspace_bytes(len(lens), 8, 2, 64, 32, table.shape[1]),), 0xff, dtype=torch.uint8, device=DEV)
+    check_decode(q, kc, vc, table, sl, workspace=ws)
+    check_decode(q, kc, vc, table, sl, window=100, workspace=ws)
 
 
 # so many sequences that a workgroup takes four heads of one; so many tokens that a wavefront looks its pages up more than once
