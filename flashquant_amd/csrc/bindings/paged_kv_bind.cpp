@@ -52,9 +52,8 @@ RowStrides strides_of(const at::Tensor& x) {
     return {{n == 4 ? x.stride(0) : 0, x.stride(n - 3), x.stride(n - 2)}};
 }
 
-// Whether two row tensors may share elements: false where their addresses do not meet, or where they are slices of one buffer
-// side by side in every token (the queries and keys of one matrix product).
-bool may_meet(const at::Tensor& a, const at::Tensor& b) {
+// Whether the memory between the first and the last element of two tensors overlaps.
+bool extents_meet(const at::Tensor& a, const at::Tensor& b) {
     if (a.numel() == 0 || b.numel() == 0) return false;
     auto end = [](const at::Tensor& t) {
         int64_t last = 0;
@@ -62,7 +61,27 @@ bool may_meet(const at::Tensor& a, const at::Tensor& b) {
         return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
     };
     const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
-    if (end(a) <= pb || end(b) <= pa) return false;
+    return pa < end(b) && pb < end(a);
+}
+bool extents_meet_any(const at::Tensor& a, std::initializer_list<const at::Tensor*> others) {
+    for (const at::Tensor* t : others)
+        if (extents_meet(a, *t)) return true;
+    return false;
+}
+
+// A tensor that a call writes in place: autograd is told, so that a backward pass which saved what was there before is refused.
+void check_written(const at::Tensor& t) {
+    check(!(at::GradMode::is_enabled() && t.requires_grad()), "a tensor that requires a gradient cannot be written in place");
+}
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// Whether two row tensors may share elements: false where their addresses do not meet, or where they are slices of one buffer
+// side by side in every token (the queries and keys of one matrix product).
+bool may_meet(const at::Tensor& a, const at::Tensor& b) {
+    if (!extents_meet(a, b)) return false;
+    const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
     const RowStrides sa = strides_of(a), sb = strides_of(b);
     const int64_t step = sa.s[1], size = a.element_size();
     if (step <= 0 || sb.s[1] != step || sa.s[0] % step != 0 || sb.s[0] % step != 0 || (pb - pa) % size != 0) return true;
@@ -81,6 +100,7 @@ at::Tensor rows_out(const MaybeTensor& out, const at::Tensor& x, const at::Tenso
     check(at::has_internal_overlap(*out) != at::MemOverlap::Yes, "out must not be expanded");
     check(same_view(*out, original) || !may_meet(*out, original), "out must be its input itself or share no memory with it");
     check(!other.has_value() || !may_meet(*out, *other), "out must share no memory with the other operands");
+    check_written(*out);
     return *out;
 }
 
@@ -139,6 +159,8 @@ std::tuple<at::Tensor, MaybeTensor> rotate(const at::Tensor& q, const MaybeTenso
             ko = rows_out(k_out, kc, *k, q, "k_out");
             check(!q_out.has_value() || !k_out.has_value() || !may_meet(qo, ko), "the outputs must share no memory");
         }
+        for (const MaybeTensor* o : {&q_out, &k_out})
+            check(!o->has_value() || !extents_meet_any(**o, {&positions, &inv_freq}), "out must share no memory with the other operands");
     }
     const bool batched = q.dim() == 4;
     const RowStrides qs = strides_of(qc), qos = strides_of(qo);
@@ -152,6 +174,8 @@ std::tuple<at::Tensor, MaybeTensor> rotate(const at::Tensor& q, const MaybeTenso
                                            a.inv_freq.data_ptr<double>(), a.half, interleaved, float(scale), inverse, batch, tokens,
                                            int(q.size(-1)), fqbind::dtype_code(q.scalar_type(), "rotary_embedding"), fqbind::current_stream(q));
         fqbind::raise_on_error(st, "rotary_embedding");
+        if (q_out.has_value()) written(qo);
+        if (k_out.has_value()) written(ko);
     }
     return {qo, k.has_value() ? MaybeTensor(ko) : std::nullopt};
 }
@@ -241,7 +265,13 @@ at::Tensor rotary_paged_store(const at::Tensor& q, const at::Tensor& k, const at
     const Angles a = angles_of(positions, inv_freq, q);
     const at::Tensor qc = rows_in(q), kc = rows_in(k), vc = rows_in(v), sm = slot_mapping.contiguous();
     const at::Tensor qo = rows_out(out, qc, q, k, "out");
-    check(!out.has_value() || !may_meet(qo, v), "out must share no memory with the other operands");
+    check(!out.has_value() || (!may_meet(qo, v) && !extents_meet_any(qo, {&positions, &inv_freq, &slot_mapping})),
+          "out must share no memory with the other operands");
+    for (const at::Tensor* c : {&key_cache, &value_cache}) {
+        check_written(*c);
+        check(!extents_meet_any(*c, {&q, &k, &v, &qo, &positions, &inv_freq, &slot_mapping}), "the caches must share no memory with the other operands");
+    }
+    check(key_cache.numel() == 0 || key_cache.data_ptr() != value_cache.data_ptr(), "keys and values must have a cache each");
     const int64_t qs[2] = {qc.stride(0), qc.stride(1)}, qos[2] = {qo.stride(0), qo.stride(1)};
     const int64_t kst[2] = {kc.stride(0), kc.stride(1)}, vst[2] = {vc.stride(0), vc.stride(1)};
     const int st = fq_rotary_paged_store(qc.data_ptr(), qs, qo.data_ptr(), qos, int(q.size(1)), kc.data_ptr(), kst, vc.data_ptr(), vst,
@@ -250,6 +280,9 @@ at::Tensor rotary_paged_store(const at::Tensor& q, const at::Tensor& k, const at
                                          vs.s, int(key_cache.size(1)), key_cache.size(0), q.size(0), int(q.size(2)),
                                          fqbind::dtype_code(q.scalar_type(), "rotary_paged_store"), fqbind::current_stream(q));
     fqbind::raise_on_error(st, "rotary_paged_store");
+    written(key_cache);
+    written(value_cache);
+    if (out.has_value()) written(qo);
     return qo;
 }
 
@@ -274,6 +307,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
         check_place(*free_start, context_lens, "free_start");
         check(free_start->scalar_type() == at::kInt && free_start->numel() == 1, "free_start must be one int32");
     }
+    check_written(block_table);
+    check(!extents_meet_any(block_table, {&context_lens, &query_lens, &free_blocks, free_start.has_value() ? &*free_start : &free_blocks}),
+          "block_table must share no memory with the other inputs");
     c10::DeviceGuard guard(context_lens.device());
     at::Tensor slots, positions, lens, cu, end;
     if (out.has_value()) {
@@ -283,17 +319,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
         check(longs(slots) && longs(positions) && ints(lens, S) && ints(cu, S + 1) && ints(end, 1),
               "out must be what a call with these sizes returns: int64 slots and positions (num_tokens,), int32 seq_lens (num_reqs,), "
               "cu_seqlens (num_reqs + 1,) and free_end (1,)");
-        const at::Tensor* const written[] = {&slots, &positions, &lens, &cu, &end};
+        const at::Tensor* const outputs[] = {&slots, &positions, &lens, &cu, &end};
         const at::Tensor* const read[] = {&context_lens, &query_lens, &free_blocks, free_start.has_value() ? &*free_start : &free_blocks, &block_table};
-        auto meet = [](const at::Tensor& a, const at::Tensor& b) {
-            if (a.numel() == 0 || b.numel() == 0) return false;
-            auto begin = [](const at::Tensor& t) { return static_cast<const char*>(t.data_ptr()); };
-            auto bytes = [](const at::Tensor& t) { return (t.dim() == 2 ? (t.size(0) - 1) * t.stride(0) + t.size(1) : t.numel()) * t.element_size(); };
-            return begin(a) < begin(b) + bytes(b) && begin(b) < begin(a) + bytes(a);
-        };
         for (int i = 0; i < 5; ++i) {
-            for (const at::Tensor* r : read) check(!meet(*written[i], *r), "outputs must share no memory with inputs");
-            for (int j = 0; j < i; ++j) check(!meet(*written[i], *written[j]), "outputs must share no memory with each other");
+            check_written(*outputs[i]);
+            for (const at::Tensor* r : read) check(!extents_meet(*outputs[i], *r), "outputs must share no memory with inputs");
+            for (int j = 0; j < i; ++j) check(!extents_meet(*outputs[i], *outputs[j]), "outputs must share no memory with each other");
         }
     } else {
         // one piece of memory for all five (five took 2.4 us of a call's 7)
@@ -312,6 +343,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
                                      slots.data_ptr<int64_t>(), positions.data_ptr<int64_t>(), lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(),
                                      int(S), num_tokens, int(block_table.size(1)), int(block_size), fqbind::current_stream(context_lens));
     fqbind::raise_on_error(st, "paged_schedule");
+    written(block_table);
+    if (out.has_value())
+        for (const at::Tensor* t : {&slots, &positions, &lens, &cu, &end}) written(*t);
     return {slots, positions, lens, cu, end};
 }
 
@@ -342,7 +376,9 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
         check_place(result, q, "out");
         check(result.is_contiguous() && result.scalar_type() == q.scalar_type() && result.sizes() == q.sizes(),
               "out must be a contiguous GPU tensor with the shape and dtype of q");
-        check(!may_meet(result, qc), "out must share no memory with q");
+        check(!may_meet(result, qc) && !extents_meet_any(result, {&key_cache, &value_cache, &block_table, &seq_lens}),
+              "out must share no memory with the inputs");
+        check_written(result);
     } else {
         result = new_tensor(q.sizes(), q.scalar_type(), q);
     }
@@ -355,6 +391,7 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
         check_place(ws, q, "workspace");
         check(ws.is_contiguous() && ws.scalar_type() == at::kByte && size_t(ws.numel()) >= bytes,
               "workspace must be a contiguous uint8 GPU tensor of at least paged_kv_decode_workspace_bytes(...) bytes");
+        check(!extents_meet_any(ws, {&qc, &key_cache, &value_cache, &block_table, &seq_lens, &result}), "workspace must share no memory with the operands");
     } else if (bytes > 0) {
         ws = new_tensor({int64_t(bytes)}, at::kByte, q);
     }
@@ -365,6 +402,7 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
                                       fqbind::dtype_code(q.scalar_type(), "paged_kv_decode"), ws.defined() ? ws.data_ptr() : nullptr,
                                       ws.defined() ? size_t(ws.numel()) : 0, fqbind::current_stream(q));
     fqbind::raise_on_error(st, "paged_kv_decode");
+    if (out.has_value()) written(result);
     return {result, return_lse ? MaybeTensor(lse) : std::nullopt};
 }
 

@@ -74,8 +74,8 @@ template <int DT, typename T> __device__ __forceinline__ T from_float(float v) {
     if constexpr (DT == FQ_F32) {
         return v;
     } else {
-    if constexpr (DT == FQ_F16) asm("" : "+v"(v));           // two roundings everywhere: no v_fma_mixlo_f16 here and there
-    return store_elem<DT>(v);
+        if constexpr (DT == FQ_F16) asm("" : "+v"(v));       // two roundings everywhere: no v_fma_mixlo_f16 here and there
+        return store_elem<DT>(v);
     }
 }
 template <typename T, int VEC, bool STREAM> __device__ __forceinline__ Piece<T, VEC> load_piece(const T* src) {

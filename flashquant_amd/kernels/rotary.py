@@ -102,7 +102,8 @@ def rotary_embedding(
     ``rotary_frequencies``.  Rows may be strided (slices of one matrix product).
 
     ``out`` = (q_out, k_out): written instead of new tensors; either may be its input itself.  Differentiable with respect to q and
-    k (any number of times) where ``out`` is not given."""
+    k (any number of times) where ``out`` is not given.  As with torch's own operators, a backward pass is captured in a graph only
+    while no record of the same leaves from outside the capture is alive."""
     require_gpu(q, "q")
     q_out, k_out = (None, None) if out is None else out
     return native().rotary_embedding(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out)
@@ -126,6 +127,6 @@ def rotary_paged_store(
     ``key_cache`` / ``value_cache`` (num_blocks, block_size, H_KV, D) at flat slot ``slot_mapping[i]``, in one launch; returns the
     rotated queries (``out``: new memory, or ``q`` itself).  Tokens beyond ``len(slot_mapping)`` and slots outside the cache are not
     stored.  float16 or bfloat16.  The caches may be strided (halves of one tensor, heads before tokens); they may not share memory
-    with the other operands."""
+    with the other operands.  No gradient is recorded."""
     require_gpu(q, "q")
     return native().rotary_paged_store(q, k, v, positions, slot_mapping, inv_freq, key_cache, value_cache, interleaved, scale, out)

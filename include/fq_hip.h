@@ -617,7 +617,8 @@ int fq_split_k_paged_decode_static(const void* q, const uint8_t* kv_cache,
  *   seq_lens       (num_reqs,) int32 out: context + query, at most max_blocks_per_seq * block_size
  *   cu_seqlens     (num_reqs + 1,) int32 out: first new token of every request
  * Of new tokens beyond num_tokens neither slot nor page is written (seq_lens, cu_seqlens and free_end count them).  No output may
- * overlap an input but block_table itself.  block_size in {8, 16, 32}.
+ * overlap an input but block_table itself.  block_size in {8, 16, 32}, num_reqs <= 2^30, num_tokens and
+ * max_blocks_per_seq * block_size < 2^31.
  */
 int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
                       const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
@@ -634,7 +635,7 @@ int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, in
  *   q_out, k_out   the same shape and dtype; the input itself (same strides), or memory that no input shares
  *   positions      (batch, tokens) of position_bytes (4 or 8) bytes, rows of a batch positions_batch_stride apart (0: shared)
  *   inv_freq       (half,) float64.  Angles are computed in 64 bits and reduced there: off by 2^-52 of their size
- * 1 <= half, 2 * half <= D <= 1024, at most 4096 heads each.  Fastest where rows lie at multiples of 16 bytes and half and D are
+ * 1 <= half, 2 * half <= D <= 1024, at most 4096 heads each, strides of tokens and heads below 2^31 in magnitude.  Fastest where rows lie at multiples of 16 bytes and half and D are
  * multiples of 16 bytes' worth of values.
  *
  * fq_rotary_paged_store: the same on q (tokens, H_Q, D) and k (tokens, H_KV, D) with k's rows and those of v (tokens, H_KV, D)
@@ -642,6 +643,7 @@ int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, in
  *   slot_mapping   (num_mapped,) int64, num_mapped <= tokens: flat slot (block * block_size + token in block) of token i.  Tokens
  *                  beyond it, and negative or out-of-range slots, are not stored (their queries are rotated).  Tokens that map
  *                  to the same slot race.
+ * All three strides of the caches are below 2^31 in magnitude; the caches themselves may be of any size.
  */
 int fq_rotary_embedding(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int H_Q, const void* k,
                         const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int H_K, const void* positions,

@@ -201,6 +201,10 @@ def test_rotary_of_nothing_and_refusals():
         args = dict(q=q, k=k, positions=p, inv_freq=freq, out=None) | bad
         with pytest.raises(ValueError):
             K.rotary_embedding(args["q"], args["k"], args["positions"], args["inv_freq"], out=args["out"])
+    longs = torch.zeros(5 * 4 * 64, dtype=torch.long, device=DEV)
+    for out in ((longs.view(BF)[:5 * 4 * 64].view(5, 4, 64), None), (None, longs.view(BF)[:5 * 2 * 64].view(5, 2, 64))):
+        with pytest.raises(ValueError):
+            K.rotary_embedding(q, k, longs[:5], freq, out=out)
     buf = torch.zeros(6 * 4 * 64, dtype=BF, device=DEV)
     a, b = buf[:5 * 4 * 64].view(5, 4, 64), buf[64:64 + 5 * 4 * 64].view(5, 4, 64)
     for out in ((b, None), (torch.empty_like(a), a)):                     # memory that an input shares
@@ -210,6 +214,63 @@ def test_rotary_of_nothing_and_refusals():
         K.rotary_embedding(q, q.clone(), p, freq, out=(a, a))
     with pytest.raises(ValueError):
         K.rotary_embedding(q.clone().requires_grad_(), k, p, freq, out=(torch.empty_like(q), torch.empty_like(k)))
+
+
+def test_rotary_captured_with_its_gradient():
+    g, (freq, scale) = gen(8), K.rotary_frequencies(128, 5e5, "linear", factor=4.0, device=DEV)
+    q, k = (torch.randn(300, h, 128, generator=g).to(BF).to(DEV).requires_grad_() for h in (8, 2))
+    dq, dk = (torch.randn(300, h, 128, generator=g).to(BF).to(DEV) for h in (8, 2))
+    positions = torch.arange(300, device=DEV)
+
+    def both_ways():
+        y, z = K.rotary_embedding(q, k, positions, freq, scale=scale)
+        return [*torch.autograd.grad((y, z), (q, k), (dq, dk)), y.detach(), z.detach()]      # (no record of q and k outlives it)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both_ways()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both_ways()
+    for i in range(6):
+        with torch.no_grad():
+            for t in (q, k, dq, dk):
+                t.copy_(torch.randn(t.shape, generator=g))
+            positions.add_(1000 * i)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        assert all(torch.equal(a, b) for a, b in zip(got, both_ways()))
+
+
+def test_what_a_call_writes_is_known_to_autograd():
+    """A gradient that needs what a later call has overwritten is refused, not computed from the new values."""
+    i32, (freq, _) = dict(dtype=torch.int32, device=DEV), K.rotary_frequencies(64, device=DEV)
+    lens, one, table, free = torch.zeros(3, **i32), torch.ones(3, **i32), torch.full((3, 4), -1, **i32), torch.arange(12, **i32)
+    s = K.paged_schedule(lens, one, table, free, 16, 3)
+    q = torch.randn(3, 2, 64, device=DEV, requires_grad=True)
+    y, _ = K.rotary_embedding(q, None, s.positions, freq)
+    K.paged_schedule(one, one, table, free, 16, 3, out=s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    for written in ("out", "key_cache", "value_cache"):
+        x = torch.randn(3, 2, 64, dtype=BF, device=DEV)
+        t = dict(q=x, k=x.clone(), v=x.clone(), positions=s.positions, slot_mapping=s.slot_mapping, inv_freq=freq, out=torch.zeros_like(x),
+                 key_cache=torch.zeros(2, 16, 2, 64, dtype=BF, device=DEV), value_cache=torch.zeros(2, 16, 2, 64, dtype=BF, device=DEV))
+        w = torch.ones((), dtype=BF, device=DEV, requires_grad=True)
+        z = t[written] * w                                                # keeps what the call overwrites
+        K.rotary_paged_store(**t)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        with pytest.raises(ValueError, match="gradient"):
+            K.rotary_paged_store(**(t | {written: t[written].clone().requires_grad_()}))
+        with torch.no_grad():
+            K.rotary_paged_store(**(t | {written: t[written].clone().requires_grad_()}))
+    with torch.inference_mode():                                          # whose tensors have no versions
+        K.rotary_embedding(x, None, s.positions, freq, out=(torch.zeros_like(x), None))
+        K.paged_schedule(one, one, table.clone(), free, 16, 3, out=K.paged_schedule(one, one, table.clone(), free, 16, 3))
 
 
 # ---- rotary store -------------------------------------------------------------------------------------------------------------
@@ -274,6 +335,15 @@ def test_rotary_store_refusals():
             K.rotary_paged_store(**(t | {name: bad}))
     with pytest.raises(ValueError):                                       # pages of 12 tokens
         K.rotary_paged_store(**(t | dict(key_cache=t["key_cache"][:, :12], value_cache=t["value_cache"][:, :12])))
+    # memory that two operands share
+    both = torch.zeros(5 * 4 * 64 + 2 * 16 * 2 * 64, dtype=BF, device=DEV)
+    cache = both[4 * 64:4 * 64 + 2 * 16 * 2 * 64].view(2, 16, 2, 64)
+    longs = torch.zeros(5 * 4 * 64, dtype=torch.long, device=DEV)
+    for bad in (dict(value_cache=t["key_cache"]), dict(q=both[:5 * 4 * 64].view(5, 4, 64), key_cache=cache), dict(out=both[:5 * 4 * 64].view(5, 4, 64), value_cache=cache),
+                dict(v=cache[0, :5], key_cache=cache), dict(k=cache[1, :5], value_cache=cache), dict(out=longs.view(BF)[:5 * 4 * 64].view(5, 4, 64), positions=longs[:5]),
+                dict(out=longs.view(BF)[:5 * 4 * 64].view(5, 4, 64), slot_mapping=longs[:5])):
+        with pytest.raises(ValueError):
+            K.rotary_paged_store(**(t | bad))
     # no pages at all: nothing is stored, the queries are rotated
     got = K.rotary_paged_store(**(t | dict(q=torch.ones_like(t["q"]), key_cache=t["key_cache"][:0], value_cache=t["value_cache"][:0])))
     assert (got[:, :, :32] == 1).all()
@@ -373,7 +443,8 @@ def test_schedule_writes_given_outputs_and_refuses():
                 dict(block_table=table[0].expand(2, 5)), dict(block_table=table.t().contiguous().t()), dict(free_blocks=free.long()), dict(free_blocks=free[::2]), dict(block_size=12),
                 dict(num_tokens=-1), dict(num_tokens=14, out=a), dict(free_start=torch.zeros(2, **i32)), dict(free_start=a.free_end, out=a),
                 dict(query_lens=query.cpu()), dict(out=a._replace(seq_lens=context)), dict(out=a._replace(seq_lens=table[0, :2])),
-                dict(out=a._replace(positions=a.slot_mapping))):
+                dict(out=a._replace(positions=a.slot_mapping)), dict(context_lens=table[0, :2]), dict(query_lens=table[1, 2:4]), dict(free_blocks=table[1]),
+                dict(free_start=table[0, :1])):
         args = dict(context_lens=context, query_lens=query, block_table=table, free_blocks=free, block_size=16, num_tokens=15) | bad
         with pytest.raises(ValueError):
             K.paged_schedule(**args)
@@ -588,6 +659,15 @@ def test_decode_of_nothing_and_refusals():
         args = dict(q=q, key_cache=kc, value_cache=vc, block_table=table, seq_lens=sl) | bad
         with pytest.raises(ValueError):
             K.paged_kv_decode(**args)
+    room = torch.zeros(2 * 4000 * 16 * 128, dtype=BF, device=DEV)               # results and workspaces in the operands' memory
+    cache, big = room[:kc.numel()].view_as(kc), torch.zeros(2, 4000, dtype=torch.int32, device=DEV)
+    for bad in (dict(key_cache=cache, out=room[:q.numel()].view_as(q)), dict(value_cache=cache, out=room[:q.numel()].view_as(q)),
+                dict(block_table=big, out=big.view(BF).view(-1)[:q.numel()].view_as(q)), dict(seq_lens=big[0, :2], out=big.view(BF).view(-1)[:q.numel()].view_as(q)),
+                dict(key_cache=cache, block_table=big, workspace=room.view(torch.uint8)),
+                dict(out=room[:q.numel()].view_as(q), block_table=big, workspace=room.view(torch.uint8)),
+                dict(q=room[:q.numel()].view_as(q), block_table=big, workspace=room.view(torch.uint8))):
+        with pytest.raises(ValueError, match="share no memory"):
+            K.paged_kv_decode(**(dict(q=q, key_cache=kc, value_cache=vc, block_table=table, seq_lens=sl) | bad))
     wide = torch.zeros(kc.numel() + 1, dtype=BF, device=DEV)[1:].view_as(kc)  # a cache at an odd address
     with pytest.raises(ValueError):
         K.paged_kv_decode(q, wide, vc, table, sl)
