@@ -26,8 +26,8 @@
 //   * A weight goes to the second product as two 16-bit terms (16 significant bits and more), so that the only rounding
 //     that shows is that of the output; the matrix cores are idle otherwise.  Maximum and sum are float32, of the unrounded
 //     weights.
-// Measured: 32 sequences of 4096 tokens, 32 heads over 8 of 128, bf16, 84.6 us (6.35 TB/s); 61 of 500 to 16000, 64 over 8, fp16, 342.6 us
-// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 22.7 us; one of 777, 32 over 8, 9.0 us.
+// Measured: 32 sequences of 4096 tokens, 32 heads over 8 of 128, bf16, 84 us (6.4 TB/s); 61 of 500 to 16000, 64 over 8, fp16, 343 us
+// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 22 us; one of 777, 32 over 8, 9.1 us.
 #include <type_traits>
 
 #include "fq_device.hpp"
@@ -589,11 +589,14 @@ struct KvPlan {
 };
 
 // Undivided sequences or shares: a CU takes its tiles at 40 to 60 GB/s, so few long sequences have to be spread, but the second
-// launch costs 3 us, and a share that goes on with another sequence starts from nothing again (3 us).  In us, undivided / shares,
-// 32 heads over 8 of 128, bf16: 1 x 200 tokens 6.2 / 8.6, 1 x 500 9.8 / 9.3, 1 x 777 11.3 / 9.6, 1 x 2000 28.4 / 10.6, 4 x 500 10.6 /
-// 9.7, 16 x 500 12.0 / 14.3, 16 x 1000 18.5 / 18.5, 32 x 1000 25.0 / 27.9, 32 x 2000 45.6 / 48.5, 64 x 1000 47.4 / 48.2, 200 of
-// 100 to 2000 181 / 162; 8 heads over 1: 32 of 100 to 700 11.5 / 12.7, 128 of them 12.9 / 16.6, 64 of 200 to 1500 20.2 / 16.1, 300
-// of them 30.6 / 36.8; 32 over 32, 16 of 300 to 1000 38.7 / 36.2.
+// launch costs 3 us, and a share that goes on with another sequence starts from nothing again (3 us; asking for that one's
+// pages ahead was no faster).  In us, undivided / shares, 32 heads over 8 of 128, bf16: 1 x 200 tokens 6.2 / 9.2, 1 x 500 9.8 / 9.4,
+// 1 x 777 11.1 / 9.1, 1 x 2000 27.6 / 10.4, 4 x 500 10.5 / 9.8, 16 x 500 12.0 / 14.2, 16 x 1000 20.0 / 18.1, 32 x 1000 25.0 / 27.8, 32 x
+// 2000 45.8 / 48.7, 64 x 1000 47.3 / 48.0, 200 of 100 to 2000 181 / 159; 8 heads over 1: 32 of 100 to 700 11.6 / 12.9, 128 of them 12.8
+// / 16.1, 64 of 200 to 1500 20.1 / 15.9, 300 of them 31.6 / 33.6; 32 over 32, 16 of 300 to 1000 38.8 / 36.6.
+// Eight wavefronts of one head have few tiles of a sequence each, so there a share that goes on costs most: 8 heads over 1, 600 of 100 to
+// 1200 43.3 / 48.6 (of 64: 24.4 / 33.3; of 256: 80.1 / 82.0), 1500 of 100 to 2000 138 / 150, 600 of 100 to 3500 103 / 98.6 (of 256: 204 /
+// 188); 16 over 2, 1000 of 100 to 1200 127 / 125.
 // The workgroup: four heads and two wavefronts of each draw best where there is much (see above); where a call has at most two
 // tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.2 -> 10.1 us,
 // 1 x 4000 13.6 -> 12.0, 8 heads over 1, 4 x 1500 14.6 -> 12.6; but 61 of 500 to 16000 343 -> 355.
@@ -604,7 +607,7 @@ KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {
     const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
     KvPlan r = {0, 1, most};
     if (tiles <= most || (tiles <= 25 && whole >= 32) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
-        int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
+        (together == 1 && D != 256 && tiles <= 80 && whole >= 2 * cus) || int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
         if (together == 4 && whole >= 8 * cus) {
             // fewer workgroups: 256 of 50 to 300 tokens, 32 heads over 8 of 128, 40 us; 52 with a head a workgroup
             r.heads = 4;
