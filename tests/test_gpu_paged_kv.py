@@ -349,6 +349,26 @@ def test_rotary_store_refusals():
     assert (got[:, :, :32] == 1).all()
 
 
+def test_rotary_and_store_beyond_32_bit_offsets():
+    """The last tokens of 2.4 10^9 elements, and the last pages of as many, against the same rows by themselves."""
+    freq, _ = K.rotary_frequencies(128, device=DEV)
+    tokens, blocks = 590_000, 147_000
+    q = torch.empty(tokens, 32, 128, dtype=BF, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q[-40:] = torch.randn(40, 32, 128, generator=g, device=DEV).to(BF)
+    q[:40] = q[-40:]
+    positions = torch.arange(tokens, device=DEV) % 1000
+    alone, _ = K.rotary_embedding(q[-40:].clone(), None, positions[-40:].clone(), freq)
+    keys, values = (torch.zeros(blocks, 16, 8, 128, dtype=BF, device=DEV) for _ in range(2))
+    got, _ = K.rotary_embedding(q, None, positions, freq)
+    assert got.numel() > 2 ** 31 and keys.numel() > 2 ** 31 and torch.equal(got[-40:], alone)
+    del got
+    k, v, slots = alone[:, :8].contiguous(), alone[:, 8:16].contiguous(), torch.arange(blocks * 16 - 40, blocks * 16, device=DEV)
+    K.rotary_paged_store(q[:40], k, v, torch.zeros(40, dtype=torch.long, device=DEV), slots, freq, keys, values)   # (position 0: as they are)
+    assert torch.equal(keys.view(-1, 8, 128)[-40:], k) and torch.equal(values.view(-1, 8, 128)[-40:], v)
+    assert not keys.view(-1, 8, 128)[:-40].any() and not values.view(-1, 8, 128)[:-40].any()
+
+
 # ---- pages, slots and positions -------------------------------------------------------------------------------------------------
 
 def scheduled(context, query, table, free, start, page, room):
