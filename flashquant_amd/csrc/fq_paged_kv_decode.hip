@@ -27,7 +27,7 @@
 //     that shows is that of the output; the matrix cores are idle otherwise.  Maximum and sum are float32, of the unrounded
 //     weights.
 // Measured: 32 sequences of 4096 tokens, 32 heads over 8 of 128, bf16, 84 us (6.4 TB/s); 61 of 500 to 16000, 64 over 8, fp16, 343 us
-// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 22 us; one of 777, 32 over 8, 9.1 us.
+// (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 21 us; one of 777, 32 over 8, 9.2 us.
 #include <type_traits>
 
 #include "fq_device.hpp"
@@ -72,13 +72,15 @@ __device__ __forceinline__ KvSpan kv_span(const KvDecodeParams& p, int len) {
     return r;
 }
 
-// How the work is divided where contexts may be long: the tiles of all sequences, one after another, are cut into equal shares, one
-// a workgroup (of a KV head), so that all of them end together whatever the lengths are.  Nothing on the host knows the lengths:
-// every workgroup adds them up for itself.  The piece of sequence s in share x is number x + s of the partial results: from
-// one piece to the next either the share or the sequence goes up by one.
+// How the work is divided where contexts may be long: the tiles of all sequences are cut into equal shares, one a workgroup (of a KV
+// head), so that all of them end together whatever the lengths are.  Nothing on the host knows the lengths: every workgroup
+// adds them up for itself.  Where there are shares enough, each belongs to one sequence, whose last one may be smaller (8 x 2000
+// tokens, 32 heads over 8 of 128: 20.4 -> 17.9 us; 3 of 40000 to 65536, 8 over 1: 23.0 -> 21.4); otherwise the sequences are laid
+// one after another before they are cut, and a share goes on from one to the next.  The piece of sequence s in share x is
+// number x + s of the partial results: from one piece to the next either the share or the sequence goes up by one.
 struct KvPlace {
-    int size, all;                        // tiles of a share, and of all sequences
-    int seq, before;                      // the sequence that holds the first tile of a share, and the tiles of those before it
+    int size;                             // tiles of a share
+    int seq, offset, left;                // the sequence where a share begins, its first tile there, the tiles of the share
     KvSpan span;
 };
 __device__ __forceinline__ int kv_len_of(const KvDecodeParams& p, int s) { return s < p.S ? p.lens[s] : 0; }
@@ -94,11 +96,12 @@ __device__ __forceinline__ int sum_upto(int v) {
     return v;
 }
 
-// Where share x begins.  False: there is no such tile.  The lengths are read kGroups x 64 at a time, all of them asked for before
+// Where share x begins.  False: there is no such share.  The lengths are read kGroups x 64 at a time, all of them asked for before
 // the first is used, and up to that many only once (4096 sequences of 100 to 1200 tokens, 8 heads over 1: 268 us, and 468 with 64
 // at a time here and in the second kernel; 1 x 777 tokens 9.2, and 9.4 with 512).
 template <int kGroups>
 __device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lane, KvPlace& r) {
+    constexpr int kAll = kGroups * kWave;
     int len[kGroups];
     auto read = [&](int s0) {
 #pragma unroll
@@ -107,30 +110,50 @@ __device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lan
             if (s0 + k * kWave < p.S) len[k] = kv_len_of(p, s0 + k * kWave + lane);
         }
     };
-    auto tiles_of = [&](int s0) {
+    // the sum of f(tiles) over the sequences, or over those that have been read
+    auto sum_read = [&](int s0, auto f) {
         uint32_t sum = 0;
 #pragma unroll
         for (int k = 0; k < kGroups; ++k)
-            if (s0 + k * kWave < p.S) sum += uint32_t(kv_span(p, len[k]).tiles);
+            if (s0 + k * kWave < p.S) sum += uint32_t(f(kv_span(p, len[k]).tiles));
         return sum;
     };
-    constexpr int kAll = kGroups * kWave;
-    uint32_t total = 0;
-    for (int s0 = 0; s0 < p.S; s0 += kAll) {
-        read(s0);
-        total += tiles_of(s0);
+    auto sum_all = [&](auto f) {
+        uint32_t sum = 0;
+        for (int s0 = 0; s0 < p.S; s0 += kAll) {
+            if (p.S > kAll) read(s0);
+            sum += sum_read(s0, f);
+        }
+        return wave_sum(sum);
+    };
+    if (p.S <= kAll) read(0);
+    const uint32_t total = sum_all([](int n) { return n; });
+    auto size_of = [&](uint32_t shares) {
+        const int size = int((total + shares - 1) / shares);
+        return size > p.min_tiles ? size : p.min_tiles;
+    };
+    r.size = size_of(uint32_t(p.shares));
+    bool apart = p.S == 1;                                   // no share holds tiles of two sequences
+    if (!apart && p.S <= kAll) {
+        auto shares_of = [&](int n) { return (n + r.size - 1) / r.size; };
+        apart = sum_all(shares_of) <= uint32_t(p.shares);
+        if (!apart) {
+            const uint32_t some = sum_all([](int n) { return n > 0 ? 1 : 0; });
+            if (8 * some <= uint32_t(p.shares)) {            // (at most a seventh more tiles a share)
+                r.size = size_of(uint32_t(p.shares) - some);
+                apart = true;
+            }
+        }
     }
-    total = wave_sum(total);
-    const int share = int((total + uint32_t(p.shares) - 1) / uint32_t(p.shares));
-    r.size = share > p.min_tiles ? share : p.min_tiles;
-    r.all = int(total);
-    const int64_t wanted = int64_t(x) * r.size;
-    if (wanted >= int64_t(total)) return false;
+    // in shares, or in tiles
+    auto units_of = [&](int n) { return apart ? (n + r.size - 1) / r.size : n; };
+    const int64_t wanted = apart ? int64_t(x) : int64_t(x) * r.size;
+    if (!apart && wanted >= int64_t(total)) return false;
     int before = 0;
     for (int s0 = 0; s0 < p.S; s0 += kAll) {
         if (p.S > kAll) {
             read(s0);
-            const int all = s0 + kAll < p.S ? int(wave_sum(tiles_of(s0))) : 0;
+            const int all = s0 + kAll < p.S ? int(wave_sum(sum_read(s0, units_of))) : 0;
             if (s0 + kAll < p.S && wanted >= int64_t(before) + all) {
                 before += all;
                 continue;
@@ -139,13 +162,16 @@ __device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lan
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
             if (s0 + k * kWave >= p.S) break;
-            const int n = kv_span(p, len[k]).tiles, upto = sum_upto(n);
+            const int n = units_of(kv_span(p, len[k]).tiles), upto = sum_upto(n);
             const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
             if (wanted < int64_t(before) + all) {
                 const int at = __ffsll(static_cast<unsigned long long>(__ballot(before + upto > int(wanted)))) - 1;
+                const int skipped = int(wanted) - (before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
                 r.seq = s0 + k * kWave + at;
-                r.before = before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
                 r.span = kv_span(p, __builtin_amdgcn_readlane(len[k], at));
+                r.offset = apart ? skipped * r.size : skipped;
+                const int rest = apart ? r.span.tiles - r.offset : int(total) - int(wanted);       // (the last share ends with the last tile)
+                r.left = rest < r.size ? rest : r.size;
                 return true;
             }
             before += all;
@@ -250,9 +276,8 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
     if constexpr (SHARED) {
         if (!(p.S <= kWave ? kv_place<1>(p, x, lane, at) : kv_place<8>(p, x, lane, at))) return;
         seq = at.seq;
-        offset = x * at.size - at.before;
-        // (the last one ends with the last sequence that has tokens)
-        left = at.all - x * at.size < at.size ? at.all - x * at.size : at.size;
+        offset = at.offset;
+        left = at.left;
     }
     bool again = false;
     do {
@@ -590,12 +615,15 @@ struct KvPlan {
 
 // Undivided sequences or shares: a CU takes its tiles at 40 to 60 GB/s, so few long sequences have to be spread, but the second
 // launch costs 3 us, and a share that goes on with another sequence starts from nothing again (3 us; asking for that one's
-// pages ahead was no faster).  In us, undivided / shares, 32 heads over 8 of 128, bf16: 1 x 200 tokens 6.2 / 9.2, 1 x 500 9.8 / 9.4,
-// 1 x 777 11.1 / 9.1, 1 x 2000 27.6 / 10.4, 4 x 500 10.5 / 9.8, 16 x 500 12.0 / 14.2, 16 x 1000 20.0 / 18.1, 32 x 1000 25.0 / 27.8, 32 x
-// 2000 45.8 / 48.7, 64 x 1000 47.3 / 48.0, 200 of 100 to 2000 181 / 159; 8 heads over 1: 32 of 100 to 700 11.6 / 12.9, 128 of them 12.8
-// / 16.1, 64 of 200 to 1500 20.1 / 15.9, 300 of them 31.6 / 33.6; 32 over 32, 16 of 300 to 1000 38.8 / 36.6.
+// pages ahead was no faster).  In us, undivided / shares, 32 heads over 8, bf16:
+//   of 128: 1 x 200 tokens 6.1 / 9.1, 1 x 430 9.1 / 9.3, 1 x 777 11.1 / 9.2, 1 x 2000 28.3 / 10.4, 10 x 430 10.0 / 12.6, 10 x 700 13.5 / 13.3,
+//     16 x 500 12.2 / 14.1, 16 x 1000 18.5 / 18.4, 32 x 1000 25.0 / 27.2, 32 x 2000 45.7 / 47.9, 64 x 1000 47.4 / 48.5, 200 of 100 to 2000
+//     181 / 159; 8 heads over 1: 10 x 700 12.1 / 10.1, 32 of 100 to 700 11.7 / 10.4, 128 of them 13.0 / 14.1, 64 of 200 to 1500 20.1 / 13.5,
+//     300 of them 30.7 / 34.3; 32 over 32, 16 of 300 to 1000 38.9 / 36.6
+//   of 64: 1 x 640 7.1 / 8.4, 10 x 700 9.9 / 11.3, 64 x 500 15.7 / 17.7, 64 of 300 to 1000 20.7 / 20.1
+//   of 256: 1 x 200 9.4 / 11.5, 1 x 300 11.6 / 11.6, 1 x 430 14.5 / 11.6, 10 x 300 12.2 / 14.2, 10 x 700 21.2 / 18.5, 30 x 700 30.7 / 36.1.
 // Eight wavefronts of one head have few tiles of a sequence each, so there a share that goes on costs most: 8 heads over 1, 600 of 100 to
-// 1200 43.3 / 48.6 (of 64: 24.4 / 33.3; of 256: 80.1 / 82.0), 1500 of 100 to 2000 138 / 150, 600 of 100 to 3500 103 / 98.6 (of 256: 204 /
+// 1200 43 / 49 (of 64: 24 / 33; of 256: 80 / 82), 1500 of 100 to 2000 138 / 150, 600 of 100 to 3500 103 / 99 (of 256: 204 /
 // 188); 16 over 2, 1000 of 100 to 1200 127 / 125.
 // The workgroup: four heads and two wavefronts of each draw best where there is much (see above); where a call has at most two
 // tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.2 -> 10.1 us,
@@ -606,7 +634,8 @@ KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {
     const int64_t whole = int64_t(S) * H_KV, cus = fq_host::device_cu_count();
     const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
     KvPlan r = {0, 1, most};
-    if (tiles <= most || (tiles <= 25 && whole >= 32) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
+    const int small = D == 256 ? 10 : D == 128 ? 14 : 24, middle = D == 256 ? 12 : 25;
+    if (tiles <= small || (tiles <= middle && whole * tiles >= most * cus) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
         (together == 1 && D != 256 && tiles <= 80 && whole >= 2 * cus) || int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
         if (together == 4 && whole >= 8 * cus) {
             // fewer workgroups: 256 of 50 to 300 tokens, 32 heads over 8 of 128, 40 us; 52 with a head a workgroup
