@@ -619,7 +619,7 @@ struct KvPlan {
 //   of 128: 1 x 200 tokens 6.1 / 9.1, 1 x 430 9.1 / 9.3, 1 x 777 11.1 / 9.2, 1 x 2000 28.3 / 10.4, 10 x 430 10.0 / 12.6, 10 x 700 13.5 / 13.3,
 //     16 x 500 12.2 / 14.1, 16 x 1000 18.5 / 18.4, 32 x 1000 25.0 / 27.2, 32 x 2000 45.7 / 47.9, 64 x 1000 47.4 / 48.5, 200 of 100 to 2000
 //     181 / 159; 8 heads over 1: 10 x 700 12.1 / 10.1, 32 of 100 to 700 11.7 / 10.4, 128 of them 13.0 / 14.1, 64 of 200 to 1500 20.1 / 13.5,
-//     300 of them 30.7 / 34.3; 32 over 32, 16 of 300 to 1000 38.9 / 36.6
+//     300 of them 30.7 / 34.3; 16 over 2, 60 of 200 to 700 13.2 / 15.6; 32 over 32, 16 of 300 to 1000 38.9 / 36.6
 //   of 64: 1 x 640 7.1 / 8.4, 10 x 700 9.9 / 11.3, 64 x 500 15.7 / 17.7, 64 of 300 to 1000 20.7 / 20.1
 //   of 256: 1 x 200 9.4 / 11.5, 1 x 300 11.6 / 11.6, 1 x 430 14.5 / 11.6, 10 x 300 12.2 / 14.2, 10 x 700 21.2 / 18.5, 30 x 700 30.7 / 36.1.
 // Eight wavefronts of one head have few tiles of a sequence each, so there a share that goes on costs most: 8 heads over 1, 600 of 100 to
@@ -634,8 +634,9 @@ KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {
     const int64_t whole = int64_t(S) * H_KV, cus = fq_host::device_cu_count();
     const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
     KvPlan r = {0, 1, most};
+    // (each of these holds for fewer tiles where it holds for more: the room of a call does not depend on its window)
     const int small = D == 256 ? 10 : D == 128 ? 14 : 24, middle = D == 256 ? 12 : 25;
-    if (tiles <= small || (tiles <= middle && whole * tiles >= most * cus) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
+    if (tiles <= small || (tiles <= middle && 8 * whole >= 3 * cus) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
         (together == 1 && D != 256 && tiles <= 80 && whole >= 2 * cus) || int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
         if (together == 4 && whole >= 8 * cus) {
             // fewer workgroups: 256 of 50 to 300 tokens, 32 heads over 8 of 128, 40 us; 52 with a head a workgroup

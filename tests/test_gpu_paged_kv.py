@@ -709,6 +709,21 @@ def test_decode_has_room_for_every_window(seqs, columns):
     assert torch.equal(outs[5], outs[0]) and all(torch.isfinite(o).all() for o in outs)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads", [1, 2, 8])
+def test_decode_has_room_for_windows_of_every_length(heads, d):
+    """The same where the lines between the ways to divide the work lie: tables and windows of 8 to 90 tiles, 1 to 600 sequences."""
+    g = gen(heads + d)
+    kc, vc, _ = caches("apart", 50, 32, heads, d, BF, g)
+    for seqs in (1, 4, 13, 16, 40, 130, 270, 600):
+        q, lens = torch.randn(seqs, heads, d, generator=g).to(BF).to(DEV), torch.full((seqs,), 5, dtype=torch.int32, device=DEV)
+        for columns in (9, 11, 13, 15, 20, 25, 26, 64, 65, 80, 90):
+            table = torch.zeros(seqs, columns, dtype=torch.int32, device=DEV)
+            want = K.paged_kv_decode(q, kc, vc, table, lens)
+            for tiles in (1, 7, 10, 12, 14, 18, 24, 30, 60, 79):
+                assert torch.allclose(K.paged_kv_decode(q, kc, vc, table, lens, window=32 * tiles), want)
+
+
 def test_decode_joins_two_caches_by_their_normalisers():
     q, kc, vc, table, sl = decode_case([1500], 8, 2, 128, 16, HF, seed=4)
     first = torch.tensor([800], dtype=torch.int32, device=DEV)
