@@ -7,11 +7,12 @@ that it can be captured in a graph."""
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from flashquant_amd.kernels import (paged_kv_decode, paged_schedule, rotary_embedding, rotary_paged_store)
+from flashquant_amd.kernels._native import native
 from flashquant_amd.vllm.impl import TQ4AttentionKernels
 from flashquant_amd.vllm.spec import get_kv_cache_shape
 
@@ -20,13 +21,27 @@ class PagedStep(NamedTuple):
     """A step's tokens: ``slot_mapping`` and ``positions`` (num_tokens,) int64, sequence by sequence; ``seq_lens`` (max_seqs,) and
     ``cu_seqlens`` (max_seqs + 1,) int32; ``block_table`` (max_seqs, max_blocks) int32; ``pages_taken`` (1,) int32: above the number
     of pages where there were too few.  Tokens without a page have slot -1, are not stored, and what their sequences' packed rows
-    give is without meaning; a caller that can run out reads ``pages_taken``."""
+    give is without meaning; a caller that can run out reads ``pages_taken``.
+
+    The tokens are packed: sequences that bring none have none, wherever they are in the table, and what is behind the last token is
+    padding.  ``token_table`` (num_tokens, max_blocks) and ``token_lens`` (num_tokens,) int32 hold, token by token, the pages of its
+    sequence and how many tokens it sees (itself the last; padding: none); None where ``num_tokens`` is above ``max_seqs``."""
     slot_mapping: torch.Tensor
     positions: torch.Tensor
     seq_lens: torch.Tensor
     cu_seqlens: torch.Tensor
     block_table: torch.Tensor
     pages_taken: torch.Tensor
+    token_table: Optional[torch.Tensor] = None
+    token_lens: Optional[torch.Tensor] = None
+
+
+def _rows(q: torch.Tensor, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Pages and lengths for single-token attention of ``q``, row by row (a step made by hand may have them by sequence)."""
+    table, lens = (step.block_table, step.seq_lens) if step.token_table is None else (step.token_table, step.token_lens)
+    if q.shape[0] != table.shape[0]:
+        raise ValueError(f"a step attends one token of every sequence at most: {q.shape[0]} tokens, {table.shape[0]} rows of pages")
+    return table, lens
 
 
 class PageTable:
@@ -51,9 +66,9 @@ class PageTable:
         lengths; ``num_tokens`` is the room for all of them."""
         s = paged_schedule(self.context_lens, query_lens, self.block_table, self.free_blocks, self.block_size, num_tokens,
                            free_start=self.free_start)
-        torch.clamp(s.seq_lens, min=0, out=self.context_lens)
-        torch.clamp(s.free_end, max=self.num_blocks, out=self.free_start)
-        return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end)
+        token_table, token_lens = native().paged_advance(s, self.context_lens, self.free_start, self.block_table, self.num_blocks,
+                                                         self.block_size, num_tokens <= self.block_table.shape[0])
+        return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, token_table, token_lens)
 
     def release(self, seq: int) -> None:
         """Ends sequence ``seq``: its pages are free again (the next to be taken) and its length is 0."""
@@ -86,10 +101,10 @@ class PagedKVLayer:
                                   interleaved=self.interleaved, scale=self.rotary_scale)
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> torch.Tensor:
-        """``store`` of one token of every sequence, then its attention over the sequence: (max_seqs, H_Q, head_dim).  Sequences that
-        bring no token in this step come behind those that do; their rows attend with whatever query they are given."""
-        return paged_kv_decode(self.store(q, k, v, step), self.keys, self.values, step.block_table, step.seq_lens, self.sm_scale,
-                               window=self.window)
+        """``store`` of a step with at most one token of every sequence, then each one's attention over its sequence: (num_tokens, H_Q,
+        head_dim); rows behind the last token are 0."""
+        rows = _rows(q, step)
+        return paged_kv_decode(self.store(q, k, v, step), self.keys, self.values, *rows, self.sm_scale, window=self.window)
 
 
 class PagedTQ4Layer:
@@ -113,9 +128,11 @@ class PagedTQ4Layer:
         return q
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> torch.Tensor:
-        """One token of every sequence stored and attended over the sequence: (max_seqs, H_Q, head_dim)."""
+        """At most one token of every sequence stored and attended over its sequence: (num_tokens, H_Q, head_dim); rows behind the
+        last token are 0."""
+        rows = _rows(q, step)
         q, k = self._rotated(q, k, step)
-        return self.kernels.decode_step(q, k, v, self.cache, step.slot_mapping, step.block_table, step.seq_lens)
+        return self.kernels.decode_step(q, k, v, self.cache, step.slot_mapping, *rows)
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep, max_query_len: int) -> torch.Tensor:
         """Several tokens of the sequences stored and attended, causal: (num_tokens, H_Q, head_dim)."""

@@ -355,6 +355,45 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
     return {slots, positions, lens, cu, end};
 }
 
+// (token_table, token_lens) where rows are asked for; context_lens and free_start are written in place.  `schedule`: what paged_schedule
+// returned, for the same block table.
+std::tuple<MaybeTensor, MaybeTensor> paged_advance(const std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>& schedule,
+                                                   at::Tensor context_lens, at::Tensor free_start, const at::Tensor& block_table,
+                                                   int64_t num_blocks, int64_t block_size, bool rows) {
+    const auto& [slots, positions, lens, cu, end] = schedule;
+    fqbind::require_gpu(context_lens, "context_lens");
+    for (const at::Tensor* t : {&slots, &positions, &lens, &cu, &end, static_cast<const at::Tensor*>(&free_start), &block_table})
+        check_place(*t, context_lens, "every operand");
+    const int64_t S = context_lens.numel(), tokens = positions.numel();
+    auto is = [](const at::Tensor& t, at::ScalarType type, int64_t n) { return t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous(); };
+    check(is(context_lens, at::kInt, S) && is(free_start, at::kInt, 1), "context_lens must be contiguous int32 of shape (num_reqs,), free_start (1,)");
+    check(is(positions, at::kLong, tokens) && is(lens, at::kInt, S) && is(cu, at::kInt, S + 1) && is(end, at::kInt, 1), "schedule must be what paged_schedule returned");
+    check(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && block_table.size(0) == S && block_table.size(1) > 0 &&
+              block_table.size(1) <= 0x7fffffff && block_table.stride(1) == 1 && (S <= 1 || block_table.stride(0) >= block_table.size(1)),
+          "block_table must be int32 of shape (num_reqs, max_blocks) with contiguous rows");
+    check(num_blocks >= 0 && num_blocks <= 0x7fffffff && S <= 0x7fffffff, "too many pages or requests");
+    check_written(context_lens);
+    check_written(free_start);
+    check(!extents_meet_any(context_lens, {&positions, &lens, &cu, &end, &free_start, &block_table}) &&
+              !extents_meet_any(free_start, {&positions, &lens, &cu, &end, &block_table}),
+          "context_lens and free_start must share no memory with the other operands");
+    c10::DeviceGuard guard(context_lens.device());
+    at::Tensor table, token_lens;
+    if (rows) {
+        table = new_tensor({tokens, block_table.size(1)}, at::kInt, context_lens);
+        token_lens = new_tensor({tokens}, at::kInt, context_lens);
+    }
+    const int st = fq_paged_advance(lens.data_ptr<int32_t>(), end.data_ptr<int32_t>(), int(num_blocks), context_lens.data_ptr<int32_t>(),
+                                    free_start.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
+                                    block_table.data_ptr<int32_t>(), S <= 1 ? block_table.size(1) : block_table.stride(0),
+                                    rows ? table.data_ptr<int32_t>() : nullptr, rows ? token_lens.data_ptr<int32_t>() : nullptr, int(S),
+                                    rows ? tokens : 0, int(block_table.size(1)), int(block_size), fqbind::current_stream(context_lens));
+    fqbind::raise_on_error(st, "paged_advance");
+    written(context_lens);
+    written(free_start);
+    return {rows ? MaybeTensor(table) : std::nullopt, rows ? MaybeTensor(token_lens) : std::nullopt};
+}
+
 std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const at::Tensor& key_cache, const at::Tensor& value_cache,
                                                     const at::Tensor& block_table, const at::Tensor& seq_lens, double sm_scale, int64_t window,
                                                     const MaybeTensor& out, bool return_lse, const MaybeTensor& workspace) {
@@ -418,6 +457,9 @@ void bind_paged_kv(py::module_& m) {
     m.def("paged_schedule", &paged_schedule, py::arg("context_lens"), py::arg("query_lens"), py::arg("block_table"), py::arg("free_blocks"),
           py::arg("block_size"), py::arg("num_tokens"), py::arg("free_start") = py::none(), py::arg("out") = py::none(),
           "Pages, slots and positions of a step's new tokens: (slot_mapping, positions, seq_lens, cu_seqlens, free_end); block_table in place");
+    m.def("paged_advance", &paged_advance, py::arg("schedule"), py::arg("context_lens"), py::arg("free_start"), py::arg("block_table"),
+          py::arg("num_blocks"), py::arg("block_size"), py::arg("rows"),
+          "After paged_schedule: context_lens and free_start for the next one, in place; with rows (token_table, token_lens) of its tokens");
     m.def("rotary_embedding", &rotary_embedding, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"),
           py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("inverse") = false, py::arg("q_out") = py::none(),
           py::arg("k_out") = py::none(), "Rotary positions on the first 2 * len(inv_freq) coordinates of every head");

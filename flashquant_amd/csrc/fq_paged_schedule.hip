@@ -158,6 +158,62 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_schedule_kernel(const 
     p.positions[token] = position;
 }
 
+// What follows a schedule, in one launch: lengths and first free page as the next one finds them, and a row of pages and a length
+// for each of the step's tokens.  A schedule packs the tokens and leaves out requests that bring none, so token i is not of request
+// i: attention of single tokens goes by these rows.
+//   What bounds it: latency, and for wide tables the copy.  A workgroup takes up to 2048 entries of one row (64 tokens of 8192 pages:
+// 4 MB over 256 workgroups).  It finds the request with one look at all of `cu`, in as few trips to memory as there are 1024 requests;
+// a search would take a trip for every halving.
+constexpr int kRowEntries = 8 * kScheduleThreads;
+
+struct AdvanceParams {
+    const int32_t* seq_lens;
+    const int32_t* free_end;
+    int32_t* context;
+    int32_t* free_start;
+    const int32_t* cu;
+    const int64_t* positions;
+    const int32_t* table;
+    int32_t* token_table;           // (num_tokens, max_blocks)
+    int32_t* token_lens;
+    int64_t table_row;
+    int S, max_blocks, num_blocks, page_log2;
+    int state_groups, parts;        // workgroups of the state, those of a token's row
+};
+
+__global__ __launch_bounds__(kScheduleThreads) void paged_advance_kernel(const AdvanceParams p) {
+    const int tid = threadIdx.x;
+    if (int(blockIdx.x) < p.state_groups) {
+        const int r = int(blockIdx.x) * kScheduleThreads + tid;
+        if (r < p.S) p.context[r] = p.seq_lens[r];
+        if (r == 0) {
+            const int end = p.free_end[0];
+            p.free_start[0] = end < p.num_blocks ? end : p.num_blocks;
+        }
+        return;
+    }
+    __shared__ int owner;
+    if (tid == 0) owner = -1;
+    __syncthreads();
+    const int token = (int(blockIdx.x) - p.state_groups) / p.parts, part = (int(blockIdx.x) - p.state_groups) % p.parts;
+#pragma unroll 4
+    for (int s = tid; s < p.S; s += kScheduleThreads)
+        if (p.cu[s] <= token && token < p.cu[s + 1]) owner = s;          // of one request at most
+    __syncthreads();
+    const int s = owner;                                                 // none behind the last token: nothing is seen
+    if (part == 0 && tid == 0) {
+        const int64_t room = int64_t(p.max_blocks) << p.page_log2, upto = p.positions[token] + 1;
+        p.token_lens[token] = s < 0 ? 0 : int(upto < room ? upto : room);
+    }
+    const int32_t* from = p.table + int64_t(s < 0 ? 0 : s) * p.table_row;
+    int32_t* to = p.token_table + int64_t(token) * p.max_blocks;
+#pragma unroll
+    for (int k = 0; k < kRowEntries / kScheduleThreads; ++k) {
+        const int i = part * kRowEntries + k * kScheduleThreads + tid;
+        if (i < p.max_blocks) to[i] = s < 0 ? -1 : from[i];
+    }
+}
+
 }  // namespace fq
 
 extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
@@ -185,5 +241,31 @@ extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* que
     // 256 requests: 3.1 us, 3.7 in the form for more; 1500, 36,000 tokens: 5.4 us, 6.9 in the form for few
     if (num_reqs <= fq::kScheduleThreads) fq::paged_schedule_kernel<1><<<grid, fq::kScheduleThreads, 0, s>>>(p);
     else fq::paged_schedule_kernel<fq::kScheduleMost><<<grid, fq::kScheduleThreads, 0, s>>>(p);
+    return fq_host::check_launch();
+}
+
+extern "C" int fq_paged_advance(const int32_t* seq_lens, const int32_t* free_end, int num_blocks, int32_t* context_lens, int32_t* free_start,
+                                const int32_t* cu_seqlens, const int64_t* positions, const int32_t* block_table, int64_t block_table_stride,
+                                int32_t* token_table, int32_t* token_lens, int num_reqs, int64_t num_tokens, int max_blocks_per_seq,
+                                int block_size, void* stream) {
+    if (num_reqs < 0 || num_reqs > (1 << 30) || num_blocks < 0 || num_tokens < 0 || num_tokens > 0x7fffffffLL || max_blocks_per_seq <= 0 ||
+        block_table_stride < max_blocks_per_seq || (num_reqs == 0 && num_tokens > 0))
+        return FQ_ERR_BAD_SHAPE;
+    if (block_size != 8 && block_size != 16 && block_size != 32) return FQ_ERR_UNSUPPORTED_BLOCK;
+    if (int64_t(max_blocks_per_seq) * block_size > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    if (!free_end || !free_start || (num_reqs > 0 && (!seq_lens || !context_lens)) ||
+        (num_tokens > 0 && (!cu_seqlens || !positions || !block_table || !token_table || !token_lens)))
+        return FQ_ERR_NULL_POINTER;
+    fq::AdvanceParams p;
+    p.seq_lens = seq_lens; p.free_end = free_end; p.context = context_lens; p.free_start = free_start;
+    p.cu = cu_seqlens; p.positions = positions; p.table = block_table; p.token_table = token_table; p.token_lens = token_lens;
+    p.table_row = block_table_stride;
+    p.S = num_reqs; p.max_blocks = max_blocks_per_seq; p.num_blocks = num_blocks;
+    p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+    p.state_groups = num_reqs > 0 ? (num_reqs + fq::kScheduleThreads - 1) / fq::kScheduleThreads : 1;
+    p.parts = (max_blocks_per_seq + fq::kRowEntries - 1) / fq::kRowEntries;
+    const int64_t groups = p.state_groups + num_tokens * p.parts;
+    if (groups > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    fq::paged_advance_kernel<<<unsigned(groups), fq::kScheduleThreads, 0, static_cast<hipStream_t>(stream)>>>(p);
     return fq_host::check_launch();
 }

@@ -626,6 +626,20 @@ int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, in
                       int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream);
 
 /*
+ * fq_paged_advance: what follows such a schedule where its lengths and pages live on the GPU, one launch.
+ *   context_lens   (num_reqs,) int32 out: seq_lens; free_start (1,) int32 out: free_end, at most num_blocks
+ *   token_table    (num_tokens, max_blocks_per_seq) int32 out: for token i of the schedule (cu_seqlens, positions: its outputs) the
+ *                  row of block_table of the request that it is of; -1 behind the last token
+ *   token_lens     (num_tokens,) int32 out: position + 1, at most max_blocks_per_seq * block_size; 0 behind the last token
+ * With them as block table and lengths the decodes attend token by token, whichever requests bring none.  num_tokens may be 0
+ * (no rows), and is 0 where num_reqs is.  No output may overlap another operand.
+ */
+int fq_paged_advance(const int32_t* seq_lens, const int32_t* free_end, int num_blocks, int32_t* context_lens, int32_t* free_start,
+                     const int32_t* cu_seqlens, const int64_t* positions, const int32_t* block_table, int64_t block_table_stride,
+                     int32_t* token_table, int32_t* token_lens, int num_reqs, int64_t num_tokens, int max_blocks_per_seq,
+                     int block_size, void* stream);
+
+/*
  * fq_rotary_embedding: pairs (x0, x1) of a head's first 2 * half coordinates become
  *     scale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a),  a = position * inv_freq[i]  (inverse != 0: -a),
  *   pair i = coordinates (i, i + half), or (2 i, 2 i + 1) where interleaved != 0; coordinates from 2 * half on are copied.  With

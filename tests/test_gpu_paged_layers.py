@@ -187,3 +187,130 @@ def test_calls_on_another_stream():
     side.synchronize()
     want = K.paged_kv_decode(K.rotary_paged_store(q, k, v, slot, slot, freq, kc, vc), kc, vc, table, lens)
     assert torch.equal(out, want) and torch.equal(mine[0], kc) and torch.equal(s.slot_mapping, slot)
+
+
+@pytest.mark.parametrize("padded", [True, False])
+@pytest.mark.parametrize("d,page,dtype", [(128, 16, torch.bfloat16), (64, 32, torch.float16), (256, 8, torch.bfloat16)])
+def test_steps_in_which_sequences_are_idle(d, page, dtype, padded):
+    """Sequences without a token first, in the middle and last, ended and not: every token attends over its own sequence, rows behind the
+    last token see nothing."""
+    seqs, g = 5, torch.Generator().manual_seed(d + 1)
+    freq, scale = K.rotary_frequencies(d)
+    table = PageTable(5 * 300 // page + 7, page, seqs, 300 // page + 1)
+    plain, packed = PagedKVLayer(table, HKV, d, freq, scale, dtype=dtype), PagedTQ4Layer(table, HKV, d, freq, scale)
+    told = Told(seqs, d, page, dtype, freq.to(DEV), scale)
+    columns = table.block_table.shape[1]
+    for turn, counts in enumerate([[37, 1, 100, 16, 64], [1, 0, 1, 0, 1], [0, 1, 1, 1, 0], "end 1", [1, 0, 1, 1, 1], [0, 0, 0, 0, 1], "end 4", [0, 0, 1, 1, 0],
+                                   [0, 0, 0, 0, 0], [0, 20, 0, 0, 0], [0, 1, 0, 1, 0], [1, 1, 1, 1, 1]]):
+        if isinstance(counts, str):
+            table.release(int(counts.split()[1]))
+            told.forget(int(counts.split()[1]))
+            continue
+        tokens = sum(counts)
+        room = max(tokens, seqs) if padded else tokens
+        q, k, v = qkv_of(room, d, dtype, g)
+        step = table.schedule(i32(counts), room)
+        qr, kr, slots = told.add(counts, q[:tokens], k[:tokens], v[:tokens])
+        assert torch.equal(step.seq_lens, told.lens()) and torch.equal(step.positions[:tokens], K.paged_schedule(told.lens() - i32(counts), i32(counts), table.block_table.clone(),
+                                                                                                       table.free_blocks, page, tokens).positions)
+        if max(counts) > 1:
+            plain.store(q, k, v, step)
+            packed.store(q, k, v, step)
+            told.kernels.compress_and_store(kr, v[:tokens], told.cache, slots)
+            continue
+        rows = [s for s in range(seqs) if counts[s]]
+        got = plain.step(q, k, v, step)
+        assert got.shape == (room, HQ, d) and not got[tokens:].any()
+        lens = i32([len(told.k[s]) for s in rows] + [0] * (room - tokens))
+        if tokens:
+            n = int(lens.max())
+            kc = torch.zeros(tokens, n, HKV, d, dtype=dtype, device=DEV)
+            vc = torch.zeros_like(kc)
+            for i, s in enumerate(rows):
+                kc[i, :len(told.k[s])], vc[i, :len(told.v[s])] = told.k[s], told.v[s]
+            want, _, tol, _ = attended(qr, kc, vc, torch.arange(tokens, dtype=torch.int32, device=DEV)[:, None], lens[:tokens], 1 / math.sqrt(d))
+            off = (got[:tokens].double() - want).abs() - tol
+            assert (off <= 0).all(), (turn, float(off.max()))
+        got = packed.step(q, k, v, step)
+        # the same rows on the pages that are kept aside
+        pad = [torch.cat([x, torch.zeros(room - tokens, *x.shape[1:], dtype=dtype, device=DEV)]) for x in (qr, kr, v[:tokens])]
+        slots = torch.cat([slots, torch.full((room - tokens,), -1, dtype=torch.int64, device=DEV)])
+        his = told.table[:, :columns][rows + [0] * (room - tokens)].contiguous()
+        if room:
+            want = told.kernels.decode_step(*pad, told.cache, slots, his, lens)
+            assert torch.equal(got, want), turn
+        assert got.shape == (room, HQ, d) and not got[tokens:].any()
+
+
+def test_idle_sequences_in_a_captured_step():
+    """One graph, replayed with other sequences idle each time."""
+    d, seqs, page, dtype = 128, 4, 16, torch.bfloat16
+    freq, _ = K.rotary_frequencies(d)
+
+    def model():
+        table = PageTable(seqs * 60, page, seqs, 60)
+        m = table, PagedKVLayer(table, HKV, d, freq, dtype=dtype), PagedTQ4Layer(table, HKV, d, freq)
+        q, k, v = qkv_of(200, d, dtype, torch.Generator().manual_seed(1))
+        step = table.schedule(i32([100, 1, 60, 39]), 200)
+        m[1].store(q, k, v, step)
+        m[2].store(q, k, v, step)
+        return m
+
+    def run(m, counts, q, k, v):
+        step = m[0].schedule(counts, seqs)
+        return m[1].step(q, k, v, step), m[2].step(q, k, v, step), step.slot_mapping
+
+    eager, captured, warm = model(), model(), model()
+    g = torch.Generator().manual_seed(2)
+    inputs, counts = [x.clone() for x in qkv_of(seqs, d, dtype, g)], i32([1] * seqs)
+    run(warm, counts, *inputs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(captured, counts, *inputs)
+    for turn in range(16):
+        counts.copy_(i32([turn >> b & 1 for b in range(seqs)]))
+        for x, y in zip(inputs, qkv_of(seqs, d, dtype, g)):
+            x.copy_(y)
+        graph.replay()
+        want = run(eager, counts, *inputs)
+        torch.cuda.synchronize()
+        for got, w in zip(out, want):
+            assert torch.equal(got, w), turn
+        n = bin(turn).count("1")
+        assert not out[0][n:].any() and not out[1][n:].any() and (n == 0 or out[0][:n].any())
+    assert torch.equal(captured[0].context_lens, eager[0].context_lens)
+
+
+def test_a_step_of_more_tokens_than_sequences_is_refused_before_it_stores():
+    freq, _ = K.rotary_frequencies(64)
+    table = PageTable(20, 16, 2, 10)
+    q, k, v = qkv_of(3, 64, torch.bfloat16, torch.Generator().manual_seed(1))
+    step = table.schedule(i32([2, 1]), 3)
+    assert step.token_table is None and step.token_lens is None
+    for layer in (PagedKVLayer(table, HKV, 64, freq), PagedTQ4Layer(table, HKV, 64, freq)):
+        with pytest.raises(ValueError, match="one token of every sequence"):
+            layer.step(q, k, v, step)
+        assert not (layer.keys if isinstance(layer, PagedKVLayer) else layer.cache).any()
+
+
+def test_rows_of_tokens_against_loops():
+    """Wide tables, many sequences, more rows than tokens, rows that are full; a table without sequences."""
+    g = torch.Generator().manual_seed(6)
+    for seqs, blocks, page, extra in ((1, 1, 8, 0), (3, 5000, 32, 0), (700, 3, 16, 0), (2500, 40, 8, 13), (300, 2049, 8, 100)):
+        table = PageTable(4 * seqs + 30, page, seqs, blocks)
+        for turn in range(3):
+            before = table.context_lens.tolist()
+            counts = torch.randint(0, 2, (seqs,), generator=g).int().tolist() if turn else [8] * seqs
+            room = min(seqs, sum(counts) + extra) if turn else sum(counts)
+            step = table.schedule(i32(counts), room)
+            if room > seqs:
+                assert step.token_table is None
+                continue
+            rows = [s for s in range(seqs) if counts[s]]
+            lens = [min(before[s] + 1, blocks * page) for s in rows]
+            assert step.token_lens.tolist() == lens + [0] * (room - len(rows))
+            assert torch.equal(step.token_table[:len(rows)], table.block_table[rows]) and (step.token_table[len(rows):] == -1).all()
+            assert step.token_table.shape == (room, blocks) and torch.equal(table.context_lens, step.seq_lens)
+    table = PageTable(4, 16, 0, 3)
+    assert int(table.schedule(i32([]), 2).pages_taken) == 0 and int(table.free_start) == 0

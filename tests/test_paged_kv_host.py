@@ -172,3 +172,18 @@ def test_decode_argument_errors_and_sizes(lib):
     assert need(2, 8, 2, 96, 16, 4000) == 0 and need(0, 8, 2, 128, 16, 4000) == 0
     assert need(1, 8, 2, 128, 16, 4) == 0                                  # a context of one part
     assert need(70000, 8, 8, 64, 32, 1 << 16) > 0                          # more tiles than are counted, fewer with a window
+
+
+def test_advance_argument_errors(lib):
+    f = lib.fq_paged_advance
+    f.argtypes = [P, P, I, P, P, P, P, P, L, P, P, I, L, I, I, P]
+
+    def call(lens=64, end=64, num_blocks=9, context=64, start=64, cu=64, positions=64, table=64, stride=4, rows=64, row_lens=64, reqs=2, tokens=3, blocks=4, page=16):
+        return f(_p(lens), _p(end), num_blocks, _p(context), _p(start), _p(cu), _p(positions), _p(table), stride, _p(rows), _p(row_lens), reqs, tokens, blocks, page, _p(0))
+
+    for bad in (dict(reqs=-1), dict(reqs=0), dict(tokens=-1), dict(tokens=1 << 31), dict(blocks=0), dict(num_blocks=-1), dict(stride=3),
+                dict(blocks=1 << 28, stride=1 << 28), dict(tokens=1 << 30, blocks=1 << 20, stride=1 << 20)):
+        assert call(**bad) == FQ_SHAPE, bad
+    assert call(page=24) == FQ_BLOCK
+    for name in ("lens", "end", "context", "start", "cu", "positions", "table", "rows", "row_lens"):
+        assert call(**{name: 0}) == FQ_NULL, name
