@@ -63,9 +63,10 @@ class PageTable:
 
     def schedule(self, query_lens: torch.Tensor, num_tokens: int) -> PagedStep:
         """Gives ``query_lens[s]`` (int32) new tokens of sequence s their pages, slots and positions and counts them into the
-        lengths; ``num_tokens`` is the room for all of them."""
+        lengths; ``num_tokens`` is the room for all of them.  Tokens that there is no room for are left out: they take no page and
+        count in no length."""
         s = paged_schedule(self.context_lens, query_lens, self.block_table, self.free_blocks, self.block_size, num_tokens,
-                           free_start=self.free_start)
+                           free_start=self.free_start, capped=True)
         token_table, token_lens = native().paged_advance(s, self.context_lens, self.free_start, self.block_table, self.num_blocks,
                                                          self.block_size, num_tokens <= self.block_table.shape[0])
         return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, token_table, token_lens)
@@ -135,5 +136,7 @@ class PagedTQ4Layer:
         return self.kernels.decode_step(q, k, v, self.cache, step.slot_mapping, *rows)
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep, max_query_len: int) -> torch.Tensor:
-        """Several tokens of the sequences stored and attended, causal: (num_tokens, H_Q, head_dim)."""
-        return self.kernels.prefill(self.store(q, k, v, step), step.cu_seqlens, max_query_len, self.cache, step.block_table, step.seq_lens)
+        """Several tokens of the sequences stored and attended, causal: (num_tokens, H_Q, head_dim).  ``max_query_len``: the most
+        tokens of a sequence, those without room among them or not; rows behind the last token are not written."""
+        return self.kernels.prefill(self.store(q, k, v, step), step.cu_seqlens, min(max_query_len, q.shape[0]), self.cache, step.block_table,
+                                    step.seq_lens)

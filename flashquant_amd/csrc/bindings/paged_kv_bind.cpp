@@ -295,7 +295,8 @@ at::Tensor rotary_paged_store(const at::Tensor& q, const at::Tensor& k, const at
 // (slot_mapping, positions, seq_lens, cu_seqlens, free_end); block_table is written in place
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_schedule(
     const at::Tensor& context_lens, const at::Tensor& query_lens, at::Tensor block_table, const at::Tensor& free_blocks, int64_t block_size,
-    int64_t num_tokens, const MaybeTensor& free_start, const std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>>& out) {
+    int64_t num_tokens, const MaybeTensor& free_start, const std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>>& out,
+    bool capped) {
     fqbind::require_gpu(context_lens, "context_lens");
     check_place(query_lens, context_lens, "query_lens");
     check_place(block_table, context_lens, "block_table");
@@ -343,11 +344,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
         end = part_of(all, 2 * longs + 2 * ints, {1}, at::kInt);
     }
     const int64_t row = S <= 1 ? block_table.size(1) : block_table.stride(0);
-    const int st = fq_paged_schedule(context_lens.data_ptr<int32_t>(), query_lens.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(), row,
-                                     free_blocks.data_ptr<int32_t>(), free_blocks.numel(),
-                                     free_start.has_value() ? free_start->data_ptr<int32_t>() : nullptr, end.data_ptr<int32_t>(),
-                                     slots.data_ptr<int64_t>(), positions.data_ptr<int64_t>(), lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(),
-                                     int(S), num_tokens, int(block_table.size(1)), int(block_size), fqbind::current_stream(context_lens));
+    const int st = (capped ? fq_paged_schedule_capped : fq_paged_schedule)(
+        context_lens.data_ptr<int32_t>(), query_lens.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(), row, free_blocks.data_ptr<int32_t>(),
+        free_blocks.numel(), free_start.has_value() ? free_start->data_ptr<int32_t>() : nullptr, end.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
+        positions.data_ptr<int64_t>(), lens.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), int(S), num_tokens, int(block_table.size(1)),
+        int(block_size), fqbind::current_stream(context_lens));
     fqbind::raise_on_error(st, "paged_schedule");
     written(block_table);
     if (out.has_value())
@@ -456,6 +457,7 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
 void bind_paged_kv(py::module_& m) {
     m.def("paged_schedule", &paged_schedule, py::arg("context_lens"), py::arg("query_lens"), py::arg("block_table"), py::arg("free_blocks"),
           py::arg("block_size"), py::arg("num_tokens"), py::arg("free_start") = py::none(), py::arg("out") = py::none(),
+          py::arg("capped") = false,
           "Pages, slots and positions of a step's new tokens: (slot_mapping, positions, seq_lens, cu_seqlens, free_end); block_table in place");
     m.def("paged_advance", &paged_advance, py::arg("schedule"), py::arg("context_lens"), py::arg("free_start"), py::arg("block_table"),
           py::arg("num_blocks"), py::arg("block_size"), py::arg("rows"),

@@ -30,6 +30,7 @@ struct ScheduleParams {
     int64_t table_row;
     int64_t num_tokens;
     int S, max_blocks, num_free, page_log2;
+    int capped;                     // tokens beyond num_tokens do not count
 };
 
 // inclusive sums over the workgroup of two values; `sum` gets those of all threads
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_schedule_kernel(const 
         for (int i = 0; i < MOST; ++i) {
             if (i >= each || r0 + i >= p.S) break;
             int64_t has;
-            const int pages = pages_of(i, has);
+            int pages = pages_of(i, has);
             if (query[i] > 0 && at.x < hi && int64_t(at.x) + query[i] > lo) {      // of the tokens [lo, hi)
                 const int o = int(at.x > lo ? at.x - lo : 0);
                 owner[o] = r0 + i;
@@ -108,11 +109,19 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_schedule_kernel(const 
                 owner_context[o] = context[i];
                 owner_page[o] = at.y;
             }
+            const int64_t left = p.num_tokens - at.x;                              // room for this request's tokens
             at.x += query[i];
+            if (p.capped && left < query[i]) {
+                // only tokens with room take the pages that they begin (those of all requests before this one do)
+                query[i] = left > 0 ? int(left) : 0;
+                pages = pages_of(i, has);
+            }
             at.y += pages;
             if (blockIdx.x == 0) {
                 p.seq_lens[r0 + i] = int(has);
-                p.cu[r0 + i + 1] = at.x;
+                p.cu[r0 + i + 1] = p.capped && at.x > p.num_tokens ? int(p.num_tokens) : at.x;
+                // the request of the last token with room takes the last page
+                if (p.capped && left > 0 && at.x >= p.num_tokens && query[i] > 0) p.free_end[0] = start + at.y;
             }
         }
         before.x += all.x;
@@ -120,7 +129,8 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_schedule_kernel(const 
     }
     if (blockIdx.x == 0 && tid == 0) {
         p.cu[0] = 0;
-        p.free_end[0] = start + before.y;
+        if (!p.capped || before.x < p.num_tokens) p.free_end[0] = start + before.y;
+        else if (p.num_tokens == 0) p.free_end[0] = start;
     }
     __syncthreads();
     // the last request that begins at or before this thread's token
@@ -216,10 +226,11 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_advance_kernel(const A
 
 }  // namespace fq
 
-extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
-                                 const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
-                                 int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
-                                 int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream) {
+namespace {
+
+int schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride, const int32_t* free_blocks,
+             int64_t num_free, const int32_t* free_start, int32_t* free_end, int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens,
+             int32_t* cu_seqlens, int num_reqs, int64_t num_tokens, int max_blocks_per_seq, int block_size, bool capped, void* stream) {
     if (num_reqs < 0 || num_reqs > (1 << 30) || num_tokens < 0 || num_tokens > 0x7fffffffLL || max_blocks_per_seq <= 0 || num_free < 0 || num_free > 0x7fffffffLL ||
         block_table_stride < max_blocks_per_seq)
         return FQ_ERR_BAD_SHAPE;
@@ -235,6 +246,7 @@ extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* que
     p.seq_lens = seq_lens; p.cu = cu_seqlens; p.table_row = block_table_stride; p.num_tokens = num_tokens;
     p.S = num_reqs; p.max_blocks = max_blocks_per_seq; p.num_free = int(num_free);
     p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+    p.capped = capped;
     const int64_t groups = (num_tokens + fq::kScheduleThreads - 1) / fq::kScheduleThreads;
     const unsigned grid = unsigned(groups > 0 ? groups : 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -242,6 +254,24 @@ extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* que
     if (num_reqs <= fq::kScheduleThreads) fq::paged_schedule_kernel<1><<<grid, fq::kScheduleThreads, 0, s>>>(p);
     else fq::paged_schedule_kernel<fq::kScheduleMost><<<grid, fq::kScheduleThreads, 0, s>>>(p);
     return fq_host::check_launch();
+}
+
+}  // namespace
+
+extern "C" int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
+                                 const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
+                                 int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
+                                 int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream) {
+    return schedule(context_lens, query_lens, block_table, block_table_stride, free_blocks, num_free, free_start, free_end, slot_mapping, positions,
+                    seq_lens, cu_seqlens, num_reqs, num_tokens, max_blocks_per_seq, block_size, false, stream);
+}
+
+extern "C" int fq_paged_schedule_capped(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
+                                        const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
+                                        int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
+                                        int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream) {
+    return schedule(context_lens, query_lens, block_table, block_table_stride, free_blocks, num_free, free_start, free_end, slot_mapping, positions,
+                    seq_lens, cu_seqlens, num_reqs, num_tokens, max_blocks_per_seq, block_size, true, stream);
 }
 
 extern "C" int fq_paged_advance(const int32_t* seq_lens, const int32_t* free_end, int num_blocks, int32_t* context_lens, int32_t* free_start,

@@ -30,6 +30,7 @@ def paged_schedule(
     *,
     free_start: Optional[torch.Tensor] = None,
     out: Optional[PagedSchedule] = None,
+    capped: bool = False,
 ) -> PagedSchedule:
     """Pages, slots and positions of a step's new tokens, in one launch and without a look at the lengths from the host.
 
@@ -40,11 +41,12 @@ def paged_schedule(
     -1, and ``free_end`` exceeds ``len(free_blocks)``.
 
     ``num_tokens``: room for the new tokens of all requests (a graph's padded batch); what is behind the last one gets slot -1 and
-    position 0.  ``out``: what an earlier call of these sizes returned, written again; its ``free_end`` must not be this call's
+    position 0.  Tokens that there is no room for get neither slot nor page, but count in ``seq_lens``, ``cu_seqlens`` and ``free_end``;
+    with ``capped`` they count nowhere, as if the requests had not brought them.  ``out``: what an earlier call of these sizes returned, written again; its ``free_end`` must not be this call's
     ``free_start``."""
     require_gpu(context_lens, "context_lens")
     return PagedSchedule(*native().paged_schedule(context_lens, query_lens, block_table, free_blocks, block_size, num_tokens,
-                                                  free_start, out))
+                                                  free_start, out, capped))
 
 
 def paged_kv_decode(

@@ -619,11 +619,18 @@ int fq_split_k_paged_decode_static(const void* q, const uint8_t* kv_cache,
  * Of new tokens beyond num_tokens neither slot nor page is written (seq_lens, cu_seqlens and free_end count them).  No output may
  * overlap an input but block_table itself.  block_size in {8, 16, 32}, num_reqs <= 2^30, num_tokens and
  * max_blocks_per_seq * block_size < 2^31.
+ * fq_paged_schedule_capped: the same, but new tokens beyond num_tokens count nowhere: cu_seqlens ends with num_tokens at most,
+ * seq_lens and free_end are those of the tokens before it.
  */
 int fq_paged_schedule(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
                       const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
                       int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
                       int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream);
+
+int fq_paged_schedule_capped(const int32_t* context_lens, const int32_t* query_lens, int32_t* block_table, int64_t block_table_stride,
+                             const int32_t* free_blocks, int64_t num_free, const int32_t* free_start, int32_t* free_end,
+                             int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens, int32_t* cu_seqlens, int num_reqs,
+                             int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream);
 
 /*
  * fq_paged_advance: what follows such a schedule where its lengths and pages live on the GPU, one launch.

@@ -736,3 +736,23 @@ def test_decode_joins_two_caches_by_their_normalisers():
     # each part is rounded once more, its share of the result
     more = (a.float().abs() * wa + b.float().abs() * wb) / (wa + wb) * torch.finfo(HF).eps
     assert ((joined.double() - o).abs() <= tol * 2 + more).all()
+
+
+@pytest.mark.parametrize("reqs", [1, 2, 5, 200, 256, 257, 700, 3000])
+def test_capped_schedule_is_that_of_the_tokens_with_room(reqs):
+    g = gen(reqs)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    for page, blocks, chunk in ((8, 60, 3), (16, 4, 100), (32, 20, 1)):
+        context = torch.randint(0, 30, (reqs,), generator=g)
+        query = torch.randint(0, chunk + 1, (reqs,), generator=g)
+        free, total = torch.randperm(max(1, int(query.sum())), generator=g).to(**i32), int(query.sum())
+        for room in sorted({0, 1, total // 3, total - 1, total, total + 9} - {-1}):
+            before = torch.cumsum(query, 0) - query
+            with_room = (room - before).clamp(min=0).minimum(query)
+            outs = []
+            for q, capped in ((query, True), (with_room, False)):
+                table = torch.full((reqs, blocks), -1, **i32)
+                s = K.paged_schedule(context.to(**i32), q.to(**i32), table, free, page, room, free_start=torch.tensor([2], **i32), capped=capped)
+                outs.append([table, *s])
+            for name, a, b in zip(("table",) + s._fields, *outs):
+                assert torch.equal(a, b), (name, room, total)

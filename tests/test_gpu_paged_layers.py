@@ -314,3 +314,30 @@ def test_rows_of_tokens_against_loops():
             assert step.token_table.shape == (room, blocks) and torch.equal(table.context_lens, step.seq_lens)
     table = PageTable(4, 16, 0, 3)
     assert int(table.schedule(i32([]), 2).pages_taken) == 0 and int(table.free_start) == 0
+
+
+def test_tokens_beyond_the_room_of_a_step_are_left_out():
+    """They take no page, count in no length, and a prompt's attention does not go beyond the rows that there are."""
+    table = PageTable(20, 16, 4, 10)
+    step = table.schedule(i32([20, 50, 9, 0]), 40)
+    assert step.cu_seqlens.tolist() == [0, 20, 40, 40, 40] and step.seq_lens.tolist() == [20, 20, 0, 0]
+    assert table.context_lens.tolist() == [20, 20, 0, 0] and int(table.free_start) == 4 and int(step.pages_taken) == 4
+    assert step.positions.tolist() == [*range(20), *range(20)] and (step.slot_mapping >= 0).all() and (table.block_table >= 0).sum() == 4
+    step = table.schedule(i32([1, 12, 1, 1]), 14)           # the last one is left out, on the first token of a page
+    assert step.cu_seqlens.tolist() == [0, 1, 13, 14, 14] and step.seq_lens.tolist() == [21, 32, 1, 0] and int(table.free_start) == 5
+    step = table.schedule(i32([3, 1, 1, 1]), 0)
+    assert step.cu_seqlens.tolist() == [0] * 5 and step.seq_lens.tolist() == [21, 32, 1, 0] and int(table.free_start) == 5
+    for s in range(4):
+        table.release(s)
+    assert int(table.free_start) == 0 and sorted(table.free_blocks.tolist()) == list(range(20))
+    d, g = 128, torch.Generator().manual_seed(5)
+    freq, _ = K.rotary_frequencies(d)
+    outs = []
+    for counts in ([20, 300, 700], [20, 230, 0]):
+        table = PageTable(100, 16, 3, 64)
+        layer = PagedTQ4Layer(table, HKV, d, freq)
+        q, k, v = qkv_of(250, d, torch.bfloat16, g.manual_seed(5))
+        step = table.schedule(i32(counts), 250)
+        assert int(step.cu_seqlens[-1]) == 250
+        outs.append(layer.prefill(q, k, v, step, max(counts)))
+    assert torch.equal(*outs)
