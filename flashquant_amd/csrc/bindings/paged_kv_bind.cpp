@@ -220,9 +220,22 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 bool needs_record(const at::Tensor& q, const MaybeTensor& k) {
     return at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad()));
 }
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+bool has_tangent(const MaybeTensor& t) { return t.has_value() && has_tangent(*t); }
 
 std::tuple<at::Tensor, MaybeTensor> rotate_recorded(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions,
                                                     const at::Tensor& inv_freq, bool interleaved, double scale, bool inverse) {
+    const bool dual_q = has_tangent(q), dual_k = has_tangent(k);
+    if (dual_q || dual_k) {
+        // forward mode: the operator is linear, so the tangent of its result is the operator on the tangent
+        auto [yq, yk] = rotate_recorded(q._fw_primal(0), k.has_value() ? MaybeTensor(k->_fw_primal(0)) : std::nullopt, positions, inv_freq,
+                                        interleaved, scale, inverse);
+        const auto [tq, tk] = rotate_recorded(dual_q ? q._fw_grad(0) : k->_fw_grad(0), dual_q && dual_k ? MaybeTensor(k->_fw_grad(0)) : std::nullopt,
+                                              positions, inv_freq, interleaved, scale, inverse);
+        if (dual_q) yq = at::_make_dual(yq, tq, 0);
+        if (dual_k) yk = at::_make_dual(*yk, dual_q ? *tk : tq, 0);
+        return {yq, yk};
+    }
     if (!needs_record(q, k)) return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, std::nullopt, std::nullopt, false);
     const auto r = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, scale, inverse);
     return {r[0], r.size() > 1 ? MaybeTensor(r[1]) : std::nullopt};
@@ -231,7 +244,8 @@ std::tuple<at::Tensor, MaybeTensor> rotate_recorded(const at::Tensor& q, const M
 std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions,
                                                      const at::Tensor& inv_freq, bool interleaved, double scale, bool inverse,
                                                      const MaybeTensor& q_out, const MaybeTensor& k_out) {
-    if (!needs_record(q, k)) return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out, true);
+    if (!needs_record(q, k) && !has_tangent(q) && !has_tangent(k))
+        return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out, true);
     check(!q_out.has_value() && !k_out.has_value(), "out cannot be combined with gradients");
     return rotate_recorded(q, k, positions, inv_freq, interleaved, scale, inverse);
 }

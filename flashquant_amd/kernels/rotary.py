@@ -102,8 +102,8 @@ def rotary_embedding(
     ``rotary_frequencies``.  Rows may be strided (slices of one matrix product).
 
     ``out`` = (q_out, k_out): written instead of new tensors; either may be its input itself.  Differentiable with respect to q and
-    k (any number of times) where ``out`` is not given.  As with torch's own operators, a backward pass is captured in a graph only
-    while no record of the same leaves from outside the capture is alive."""
+    k, any number of times and in forward mode too, where ``out`` is not given.  As with torch's own operators, a backward pass is
+    captured in a graph only while no record of the same leaves from outside the capture is alive."""
     require_gpu(q, "q")
     q_out, k_out = (None, None) if out is None else out
     return native().rotary_embedding(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out)

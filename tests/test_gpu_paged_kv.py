@@ -756,3 +756,62 @@ def test_capped_schedule_is_that_of_the_tokens_with_room(reqs):
                 outs.append([table, *s])
             for name, a, b in zip(("table",) + s._fields, *outs):
                 assert torch.equal(a, b), (name, room, total)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_in_forward_mode(interleaved, dtype):
+    """The map is linear: the tangent is the operator on the tangent; also of a gradient, and beside one."""
+    import torch.autograd.forward_ad as fwAD
+    t, h, d, rot = 19, 3, 64, 48
+    g = gen(11)
+    freq, _ = K.rotary_frequencies(rot, device=DEV)
+    positions = torch.randint(0, 300, (t,), generator=g).to(DEV)
+    q, k, vq, vk, dy, vy = (torch.randn(t, n, d, generator=g).to(dtype).to(DEV) for n in (h, 1, h, 1, h, h))
+    args = dict(interleaved=interleaved, scale=1.5)
+    want = K.rotary_embedding(q, k, positions, freq, **args)
+    for tq, tk, inverse in ((vq, vk, False), (vq, None, False), (None, vk, False), (vq, vk, True)):
+        with fwAD.dual_level():
+            a, b = (x if v is None else fwAD.make_dual(x, v) for x, v in ((q, tq), (k, tk)))
+            outs = K.rotary_embedding(a, b, positions, freq, inverse=inverse, **args)
+            for y, v, w in zip(outs, (tq, tk), want):
+                primal, tangent = fwAD.unpack_dual(y)
+                assert inverse or torch.equal(primal, w)
+                if v is not None:
+                    check_turn(tangent, v, positions, freq, interleaved, 1.5, -1.0 if inverse else 1.0)
+                else:
+                    assert tangent is None or not tangent.any()
+            with pytest.raises(ValueError, match="gradient"):
+                K.rotary_embedding(a, b, positions, freq, out=(torch.empty_like(q), torch.empty_like(k)))
+    with fwAD.dual_level():                                               # alone, of strided rows
+        y, none = K.rotary_embedding(fwAD.make_dual(q[:, 1:], vq[:, 1:]), None, positions, freq, **args)
+        check_turn(fwAD.unpack_dual(y).tangent, vq[:, 1:], positions, freq, interleaved, 1.5)
+        assert none is None
+    # where a gradient is recorded as well: of the result, of its tangent, and the tangent of the gradient
+    leaf, vleaf = q.clone().requires_grad_(), vq.clone().requires_grad_()
+    with fwAD.dual_level():
+        y, _ = K.rotary_embedding(fwAD.make_dual(leaf, vleaf), None, positions, freq, **args)
+        primal, tangent = fwAD.unpack_dual(y)
+        first, = torch.autograd.grad(primal, (leaf,), dy, retain_graph=True)
+        second, = torch.autograd.grad(tangent, (vleaf,), dy, retain_graph=True)
+        check_turn(first, dy, positions, freq, interleaved, 1.5, -1.0)
+        check_turn(second, dy, positions, freq, interleaved, 1.5, -1.0)
+        over, = torch.autograd.grad(primal, (leaf,), fwAD.make_dual(dy, vy))
+        check_turn(fwAD.unpack_dual(over).tangent, vy, positions, freq, interleaved, 1.5, -1.0)
+
+
+def test_rotary_under_function_transforms_is_right_or_refused():
+    g, (freq, _) = gen(12), K.rotary_frequencies(64, device=DEV)
+    q, v = (torch.randn(5, 2, 64, generator=g).to(DEV) for _ in range(2))
+    positions = torch.arange(5, device=DEV)
+
+    def f(x):
+        return K.rotary_embedding(x, None, positions, freq)[0]
+
+    for call, want in ((lambda: torch.func.jvp(f, (q,), (v,))[1], lambda: f(v)), (lambda: torch.func.vmap(f)(torch.stack([q, v])), lambda: torch.stack([f(q), f(v)])),
+                       (lambda: torch.func.grad(lambda x: (f(x) * v).sum())(q), lambda: K.rotary_embedding(v, None, positions, freq, inverse=True)[0])):
+        try:
+            got = call()
+        except RuntimeError:
+            continue
+        assert torch.equal(got, want())
