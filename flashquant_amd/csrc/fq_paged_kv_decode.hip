@@ -35,7 +35,10 @@
 namespace fq {
 
 constexpr int kKvTile = 32;               // keys of a wavefront's step
-constexpr float kKvLift = 10.0f;          // weights are kept times 2^10: their second terms stay normal in fp16
+// Weights are kept times 2^lift.  fp16: up, so that their second terms stay normal.  bf16 has the exponents of float32, and a value may
+// lie near 2^128: down, so that no wavefront's sum of up to 2^20 such values overflows where their average does not (what underflows
+// instead are products below 2^-106).
+template <int DT> constexpr float kKvLift = DT == FQ_F16 ? 10.0f : -20.0f;
 
 struct KvDecodeParams {
     const uint16_t* q;
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
                         for (int e = 0; e < VE; ++e) acc[h][e] *= shrink;
                     m = higher;
                 }
-                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift;
+                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<DT>;
                 uint4v hi, lo;
                 float w[8];
 #pragma unroll
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
                 p.part_m[row + h] = mt;
                 p.part_l[row + h] = lt;
             } else if (p.lse != nullptr) {
-                p.lse[orow + h] = lt == 0.0f ? -__builtin_inff() : (mt - kKvLift + __builtin_amdgcn_logf(lt)) * (1.0f / kLog2e);
+                p.lse[orow + h] = lt == 0.0f ? -__builtin_inff() : (mt - kKvLift<DT> + __builtin_amdgcn_logf(lt)) * (1.0f / kLog2e);
             }
         };
         // lane (g, h) holds coordinates VE (4 g + r) + e of head h
@@ -599,7 +602,7 @@ __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams
         const int64_t out = group * p.G;
         *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(all.x * inv, all.y * inv), round_pair<DT>(all.z * inv, all.w * inv)};
         if (c % D == 0 && p.lse != nullptr)
-            p.lse[out + h] = den == 0.0f ? -__builtin_inff() : (highest - kKvLift + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
+            p.lse[out + h] = den == 0.0f ? -__builtin_inff() : (highest - kKvLift<DT> + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
     }
 }
 

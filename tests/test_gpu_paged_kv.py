@@ -815,3 +815,31 @@ def test_rotary_under_function_transforms_is_right_or_refused():
         except RuntimeError:
             continue
         assert torch.equal(got, want())
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (32, 8, 64), (16, 16, 256), (8, 1, 128)])
+@pytest.mark.parametrize("lens", [[1], [40, 3], [700, 300], [5000], [9000, 20, 4000], [300] * 70])
+def test_decode_of_values_at_the_end_of_bfloat16(lens, hq, hkv, d):
+    """One key has all the weight (the others e^-40 of it) and values go to 2^127: the average is finite, on every path."""
+    q, kc, vc, table, sl = decode_case(lens, hq, hkv, d, 16, BF, seed=d)
+    vc.copy_((vc * 1e38).clamp(-3e38, 3e38))
+    q.fill_(1.0)
+    kc.zero_()
+    for s, n in enumerate(lens):
+        at = (7 * s + n // 3) % n
+        kc[int(table[s, at // 16]), at % 16] = 1.0
+    out, _ = check_decode(q, kc, vc, table, sl, sm=40.0 / d)
+    assert torch.isfinite(out).all() and out.abs().max() > 1e38
+
+
+@pytest.mark.parametrize("lens", [[1], [700, 300], [5000], [9000, 20, 4000], [300] * 70])
+def test_decode_of_equal_weights_over_very_large_and_very_small_values(lens):
+    """All keys weigh the same and all values lie near 2^128: the sum does not overflow where the average does not."""
+    q, kc, vc, table, sl = decode_case(lens, 8, 2, 128, 16, BF, seed=len(lens))
+    vc.fill_(3.2e38)
+    check_decode(q, kc, vc, table, sl, sm=0.0)
+    vc[:, ::3] = -3.2e38
+    check_decode(q, kc, vc, table, sl)
+    vc.copy_(torch.randn(vc.shape, generator=gen(1)) * 1e-30)
+    out, _ = check_decode(q, kc, vc, table, sl)
+    assert out.any()
