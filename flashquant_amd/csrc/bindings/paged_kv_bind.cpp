@@ -253,6 +253,33 @@ std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const 
 struct Cache {
     int64_t s[3];
 };
+// Whether two caches may share rows: false where their addresses do not meet, or where both go on by one step, of blocks, tokens or heads,
+// within which their rows lie side by side (the halves of one tensor, keys and values of a head in one row).
+bool caches_may_meet(const at::Tensor& a, const at::Tensor& b) {
+    if (!Extent(a).meets(Extent(b))) return false;
+    const int64_t size = a.element_size();
+    const int64_t between = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+    if (between % size != 0) return true;
+    // the elements of t within one step, and whether all larger strides are whole steps
+    auto within = [](const at::Tensor& t, int64_t step, int64_t& span) {
+        span = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) {
+            if (t.size(i) == 1) continue;
+            if (t.stride(i) < step) span += (t.size(i) - 1) * t.stride(i);
+            else if (t.stride(i) % step != 0) return false;
+        }
+        return true;
+    };
+    for (int64_t i = 0; i < a.dim(); ++i) {
+        const int64_t step = a.stride(i);
+        int64_t span_a, span_b;
+        if (a.size(i) == 1 || step <= 0 || !within(a, step, span_a) || !within(b, step, span_b)) continue;
+        const int64_t apart = (between / size % step + step) % step;
+        if (span_a <= apart && apart + span_b <= step) return false;
+    }
+    return true;
+}
+
 Cache cache_of(const at::Tensor& cache, const at::Tensor& like, const at::Tensor& rows, const char* name) {
     check_place(cache, like, name);
     check(cache.dim() == 4 && cache.size(3) == rows.size(-1) && cache.scalar_type() == rows.scalar_type(),
@@ -291,7 +318,7 @@ at::Tensor rotary_paged_store(const at::Tensor& q, const at::Tensor& k, const at
         const Extent e(*t);
         check(!e.meets(keys) && !e.meets(values), "the caches must share no memory with the other operands");
     }
-    check(key_cache.numel() == 0 || key_cache.data_ptr() != value_cache.data_ptr(), "keys and values must have a cache each");
+    check(!caches_may_meet(key_cache, value_cache), "keys and values must have a cache each, and share no memory");
     const int64_t qs[2] = {qc.stride(0), qc.stride(1)}, qos[2] = {qo.stride(0), qo.stride(1)};
     const int64_t kst[2] = {kc.stride(0), kc.stride(1)}, vst[2] = {vc.stride(0), vc.stride(1)};
     const int st = fq_rotary_paged_store(qc.data_ptr(), qs, qo.data_ptr(), qos, int(q.size(1)), kc.data_ptr(), kst, vc.data_ptr(), vst,

@@ -843,3 +843,28 @@ def test_decode_of_equal_weights_over_very_large_and_very_small_values(lens):
     vc.copy_(torch.randn(vc.shape, generator=gen(1)) * 1e-30)
     out, _ = check_decode(q, kc, vc, table, sl)
     assert out.any()
+
+
+def test_rotary_store_into_caches_that_share_rows():
+    """Refused; caches whose rows only lie among each other are not."""
+    freq, _ = K.rotary_frequencies(64, device=DEV)
+    x = torch.randn(5, 2, 64, generator=gen(5)).to(BF).to(DEV)
+    t = dict(q=x, k=x.clone(), v=x.clone(), positions=torch.arange(5, device=DEV), slot_mapping=torch.arange(5, device=DEV), inv_freq=freq)
+    buf = torch.zeros(5, 16, 2, 64, dtype=BF, device=DEV)
+    wide = torch.zeros(4, 16, 4, 128, dtype=BF, device=DEV)
+    flat = torch.zeros(8 * 16 * 2 * 64, dtype=BF, device=DEV)
+    for kc, vc in ((buf[:-1], buf[1:]), (buf[1:], buf[:-1]), (wide[:, :, :2, :64], wide[:, :, 1:3, :64]), (wide[..., :2, :64], wide[..., :2, 32:96]),
+                   (flat[:4 * 2048].view(4, 16, 2, 64), flat[1024:1024 + 4 * 2048].view(4, 16, 2, 64)),
+                   (flat[:4 * 2048].view(4, 16, 2, 64), flat[64:64 + 4 * 2048].view(4, 2, 16, 64).transpose(1, 2)),
+                   (flat.view(4, 2, 16, 2, 64)[:, 0], flat[2048:2048 * 5].view(4, 16, 2, 64)), (buf, buf)):
+        with pytest.raises(ValueError, match="share no memory|cache each"):
+            K.rotary_paged_store(**t, key_cache=kc, value_cache=vc)
+    blocks = torch.zeros(4, 2, 16 * 2 * 64, dtype=BF, device=DEV)
+    for whole, kc, vc in ((blocks, blocks[:, 0].view(4, 16, 2, 64), blocks[:, 1].view(4, 2, 16, 64).transpose(1, 2)),        # heads first in one of them
+                          (wide, wide[:, :, :2, :64], wide[:, :, 2:, :64]), (wide, wide[..., :2, :64], wide[..., :2, 64:]),
+                          (wide, wide[:2, :, :2, :64], wide[2:, :, :2, :64]), (wide, wide[::2, :, :2, 64:], wide[1::2, :, :2, :64]),
+                          (flat, flat.view(4, 2, 16, 2, 64)[:, 1], flat.view(4, 2, 16, 2, 64)[:, 0])):
+        whole.zero_()
+        K.rotary_paged_store(**t, key_cache=kc, value_cache=vc)
+        assert torch.equal(kc[0, :5], K.rotary_embedding(t["k"], None, t["positions"], freq)[0]) and torch.equal(vc[0, :5], t["v"])
+        assert int((whole != 0).sum()) == int((kc != 0).sum()) + int((vc != 0).sum())
