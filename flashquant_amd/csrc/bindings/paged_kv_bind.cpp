@@ -2,7 +2,6 @@
 // Tensors are unwrapped, checked and handed to the C ABI on torch's current stream of their device; strided rows go in as
 // they are.  There is no CPU path: a tensor that is not on the GPU is an error.
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
@@ -72,6 +71,25 @@ bool extents_meet_any(const at::Tensor& a, std::initializer_list<const at::Tenso
     return false;
 }
 
+// Whether rows of a tensor that is written lie on each other (expanded ones, windows that slide): taken from the smallest stride up, each
+// has to go past all that lies below it.
+bool rows_meet(const at::Tensor& t) {
+    if (t.is_contiguous() || t.numel() == 0) return false;
+    const auto sizes = t.sizes(), strides = t.strides();
+    uint32_t left = 0;                      // dimensions that are still to be looked at
+    for (size_t i = 0; i < sizes.size(); ++i)
+        if (sizes[i] > 1) left |= 1u << i;
+    for (int64_t span = 1; left != 0;) {
+        size_t low = 0;
+        for (size_t i = 0, found = 0; i < sizes.size(); ++i)
+            if ((left >> i & 1) != 0 && (found == 0 || strides[i] < strides[low])) { low = i; found = 1; }
+        if (strides[low] < span) return true;
+        span += (sizes[low] - 1) * strides[low];
+        left &= ~(1u << low);
+    }
+    return false;
+}
+
 // A tensor that a call writes in place: autograd is told, so that a backward pass which saved what was there before is refused.
 void check_written(const at::Tensor& t) {
     check(!(at::GradMode::is_enabled() && t.requires_grad()), "a tensor that requires a gradient cannot be written in place");
@@ -100,7 +118,7 @@ at::Tensor rows_out(const MaybeTensor& out, const at::Tensor& x, const at::Tenso
     check_place(*out, x, name);
     check(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type(), "out must have the shape and dtype of its input");
     check(out->stride(-1) == 1 || out->size(-1) <= 1, "out must have contiguous rows");
-    check(at::has_internal_overlap(*out) != at::MemOverlap::Yes, "out must not be expanded");
+    check(!rows_meet(*out), "rows of out must not share memory");
     check(same_view(*out, original) || !may_meet(*out, original), "out must be its input itself or share no memory with it");
     check(!other.has_value() || !may_meet(*out, *other), "out must share no memory with the other operands");
     check_written(*out);
@@ -303,8 +321,7 @@ at::Tensor rotary_paged_store(const at::Tensor& q, const at::Tensor& k, const at
           "slot_mapping must be int64 with at most one entry per token");
     const Cache ks = cache_of(key_cache, q, k, "key_cache"), vs = cache_of(value_cache, q, k, "value_cache");
     check(key_cache.size(2) == k.size(1) && value_cache.sizes() == key_cache.sizes(), "the caches must have one shape, with the heads of k");
-    check(at::has_internal_overlap(key_cache) != at::MemOverlap::Yes && at::has_internal_overlap(value_cache) != at::MemOverlap::Yes,
-          "the caches must not be expanded");
+    check(!rows_meet(key_cache) && !rows_meet(value_cache), "rows of a cache must not share memory");
     c10::DeviceGuard guard(q.device());
     const Angles a = angles_of(positions, inv_freq, q);
     const at::Tensor qc = rows_in(q), kc = rows_in(k), vc = rows_in(v), sm = slot_mapping.contiguous();

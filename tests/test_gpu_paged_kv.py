@@ -868,3 +868,26 @@ def test_rotary_store_into_caches_that_share_rows():
         K.rotary_paged_store(**t, key_cache=kc, value_cache=vc)
         assert torch.equal(kc[0, :5], K.rotary_embedding(t["k"], None, t["positions"], freq)[0]) and torch.equal(vc[0, :5], t["v"])
         assert int((whole != 0).sum()) == int((kc != 0).sum()) + int((vc != 0).sum())
+
+
+def test_outputs_whose_own_rows_share_memory_are_refused():
+    freq, _ = K.rotary_frequencies(64, device=DEV)
+    x = torch.randn(5, 2, 64, generator=gen(5)).to(BF).to(DEV)
+    t = dict(q=x, k=x.clone(), v=x.clone(), positions=torch.arange(5, device=DEV), slot_mapping=torch.arange(5, device=DEV), inv_freq=freq,
+             key_cache=torch.zeros(3, 16, 2, 64, dtype=BF, device=DEV), value_cache=torch.zeros(3, 16, 2, 64, dtype=BF, device=DEV))
+    buf = torch.zeros(3 * 16 * 2 * 64, dtype=BF, device=DEV)
+    for sizes, strides in (((5, 2, 64), (64, 64, 1)), ((5, 2, 64), (0, 64, 1)), ((5, 2, 64), (128, 32, 1)), ((5, 2, 64), (96, 64, 1)), ((5, 2, 64), (1, 512, 1))):
+        bad = buf.as_strided(sizes, strides)
+        with pytest.raises(ValueError, match="share memory"):
+            K.rotary_embedding(x, None, t["positions"], freq, out=(bad, None))
+        with pytest.raises(ValueError, match="share memory"):
+            K.rotary_paged_store(**t, out=bad)
+    for strides in ((1024, 128, 64, 1), (2048, 64, 64, 1), (0, 128, 64, 1)):
+        for name in ("key_cache", "value_cache"):
+            with pytest.raises(ValueError, match="share memory"):
+                K.rotary_paged_store(**(t | {name: buf.as_strided((3, 16, 2, 64), strides)}))
+    want = K.rotary_embedding(x, None, t["positions"], freq)[0]
+    for strides in ((128, 64, 1), (64, 320, 1), (200, 64, 1), (64, 777, 1)):  # and these do not
+        out = buf.as_strided((5, 2, 64), strides)
+        K.rotary_embedding(x, None, t["positions"], freq, out=(out, None))
+        assert torch.equal(out, want)
