@@ -31,15 +31,6 @@ at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const at::Ten
     return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
 }
 
-// A contiguous tensor in a piece of memory that several share (a second allocation costs a call half a microsecond).
-at::Tensor part_of(const at::Tensor& memory, int64_t byte, at::IntArrayRef sizes, at::ScalarType dtype) {
-    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(memory.storage()), memory.key_set(), c10::scalarTypeToTypeMeta(dtype));
-    t.unsafeGetTensorImpl()->set_storage_offset(byte / int64_t(c10::elementSize(dtype)));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    return t;
-}
-int64_t room_of(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-
 // rows (..., H, D) of contiguous values, as the kernels take them; others are copied
 at::Tensor rows_in(const at::Tensor& x) { return x.stride(-1) == 1 || x.size(-1) <= 1 ? x : x.contiguous(); }
 
@@ -151,10 +142,8 @@ Angles angles_of(const at::Tensor& positions, const at::Tensor& inv_freq, const 
     return a;
 }
 
-// together: new results share one piece of memory (not those that a gradient is recorded for, or gradients: one may be kept
-// without the other)
 std::tuple<at::Tensor, MaybeTensor> rotate(const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions, const at::Tensor& inv_freq,
-                                           bool interleaved, double scale, bool inverse, const MaybeTensor& q_out, const MaybeTensor& k_out, bool together) {
+                                           bool interleaved, double scale, bool inverse, const MaybeTensor& q_out, const MaybeTensor& k_out) {
     fqbind::require_gpu(q, "q");
     check(q.dim() == 3 || q.dim() == 4, "q must have shape (tokens, H, D) or (batch, tokens, H, D)");
     check(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kFloat, "q must be float16, bfloat16 or float32");
@@ -168,21 +157,14 @@ std::tuple<at::Tensor, MaybeTensor> rotate(const at::Tensor& q, const MaybeTenso
     c10::DeviceGuard guard(q.device());
     const Angles a = angles_of(positions, inv_freq, q);
     const at::Tensor qc = rows_in(q), kc = k.has_value() ? rows_in(*k) : at::Tensor();
-    at::Tensor qo, ko;
-    if (together && k.has_value() && !q_out.has_value() && !k_out.has_value()) {
-        const int64_t size = q.element_size(), first = room_of(q.numel() * size);
-        const at::Tensor all = new_tensor({first + k->numel() * size}, at::kByte, q);
-        qo = part_of(all, 0, q.sizes(), q.scalar_type());
-        ko = part_of(all, first, k->sizes(), q.scalar_type());
-    } else {
-        qo = rows_out(q_out, qc, q, k, "q_out");
-        if (k.has_value()) {
-            ko = rows_out(k_out, kc, *k, q, "k_out");
-            check(!q_out.has_value() || !k_out.has_value() || !may_meet(qo, ko), "the outputs must share no memory");
-        }
-        for (const MaybeTensor* o : {&q_out, &k_out})
-            check(!o->has_value() || !extents_meet_any(**o, {&positions, &inv_freq}), "out must share no memory with the other operands");
+    const at::Tensor qo = rows_out(q_out, qc, q, k, "q_out");
+    at::Tensor ko;
+    if (k.has_value()) {
+        ko = rows_out(k_out, kc, *k, q, "k_out");
+        check(!q_out.has_value() || !k_out.has_value() || !may_meet(qo, ko), "the outputs must share no memory");
     }
+    for (const MaybeTensor* o : {&q_out, &k_out})
+        check(!o->has_value() || !extents_meet_any(**o, {&positions, &inv_freq}), "out must share no memory with the other operands");
     const bool batched = q.dim() == 4;
     const RowStrides qs = strides_of(qc), qos = strides_of(qo);
     RowStrides ks{}, kos{};
@@ -215,7 +197,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["inverse"] = inverse;
         ctx->set_materialize_grads(false);
-        auto [qo, ko] = rotate(q, k, positions, inv_freq, interleaved, scale, inverse, std::nullopt, std::nullopt, false);
+        auto [qo, ko] = rotate(q, k, positions, inv_freq, interleaved, scale, inverse, std::nullopt, std::nullopt);
         torch::autograd::variable_list r = {qo};
         if (ko.has_value()) r.push_back(*ko);
         return r;
@@ -254,7 +236,7 @@ std::tuple<at::Tensor, MaybeTensor> rotate_recorded(const at::Tensor& q, const M
         if (dual_k) yk = at::_make_dual(*yk, dual_q ? *tk : tq, 0);
         return {yq, yk};
     }
-    if (!needs_record(q, k)) return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, std::nullopt, std::nullopt, false);
+    if (!needs_record(q, k)) return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, std::nullopt, std::nullopt);
     const auto r = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, scale, inverse);
     return {r[0], r.size() > 1 ? MaybeTensor(r[1]) : std::nullopt};
 }
@@ -263,7 +245,7 @@ std::tuple<at::Tensor, MaybeTensor> rotary_embedding(const at::Tensor& q, const 
                                                      const at::Tensor& inv_freq, bool interleaved, double scale, bool inverse,
                                                      const MaybeTensor& q_out, const MaybeTensor& k_out) {
     if (!needs_record(q, k) && !has_tangent(q) && !has_tangent(k))
-        return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out, true);
+        return rotate(q, k, positions, inv_freq, interleaved, scale, inverse, q_out, k_out);
     check(!q_out.has_value() && !k_out.has_value(), "out cannot be combined with gradients");
     return rotate_recorded(q, k, positions, inv_freq, interleaved, scale, inverse);
 }
@@ -392,14 +374,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
             for (int j = 0; j < i; ++j) check(!Extent(*outputs[i]).meets(Extent(*outputs[j])), "outputs must share no memory with each other");
         }
     } else {
-        // one piece of memory for all five (five took 2.4 us of a call's 7)
-        const int64_t longs = room_of(8 * num_tokens), ints = room_of(4 * S + 4);
-        const at::Tensor all = new_tensor({2 * longs + 2 * ints + 256}, at::kByte, context_lens);
-        slots = part_of(all, 0, {num_tokens}, at::kLong);
-        positions = part_of(all, longs, {num_tokens}, at::kLong);
-        lens = part_of(all, 2 * longs, {S}, at::kInt);
-        cu = part_of(all, 2 * longs + ints, {S + 1}, at::kInt);
-        end = part_of(all, 2 * longs + 2 * ints, {1}, at::kInt);
+        slots = new_tensor({num_tokens}, at::kLong, context_lens);
+        positions = new_tensor({num_tokens}, at::kLong, context_lens);
+        lens = new_tensor({S}, at::kInt, context_lens);
+        cu = new_tensor({S + 1}, at::kInt, context_lens);
+        end = new_tensor({1}, at::kInt, context_lens);
     }
     const int64_t row = S <= 1 ? block_table.size(1) : block_table.stride(0);
     const int st = (capped ? fq_paged_schedule_capped : fq_paged_schedule)(

@@ -891,3 +891,21 @@ def test_outputs_whose_own_rows_share_memory_are_refused():
         out = buf.as_strided((5, 2, 64), strides)
         K.rotary_embedding(x, None, t["positions"], freq, out=(out, None))
         assert torch.equal(out, want)
+
+
+def test_results_have_memory_of_their_own():
+    """One may be resized, kept or dropped without the others."""
+    freq, _ = K.rotary_frequencies(64, device=DEV)
+    q, k = (torch.randn(8, 4, 64, generator=gen(s)).to(BF).to(DEV) for s in (1, 2))
+    qo, ko = K.rotary_embedding(q, k, torch.arange(8, device=DEV), freq)
+    kept = ko.clone()
+    torch.full((9, 4, 64), 7.0, dtype=BF, device=DEV, out=qo.resize_(0))
+    assert torch.equal(ko, kept)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    lens = torch.arange(64, **i32)
+    s = K.paged_schedule(lens, torch.ones(64, **i32), torch.full((64, 8), -1, **i32), torch.arange(64, **i32), 16, 64)
+    for name in s._fields:
+        kept = {n: t.clone() for n, t in s._asdict().items() if n != name}
+        t = getattr(s, name)
+        t.resize_(t.numel() + 3).fill_(-9)
+        assert all(torch.equal(getattr(s, n), x) for n, x in kept.items()), name
