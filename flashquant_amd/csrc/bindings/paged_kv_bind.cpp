@@ -467,7 +467,7 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const a
     }
     if (return_lse) lse = new_tensor({S, HQ}, at::kFloat, q);
     const int bs = int(key_cache.size(1)), mb = int(block_table.size(1));
-    const size_t bytes = fq_paged_kv_decode_workspace_bytes(int(S), int(HQ), int(HKV), int(D), bs, mb);
+    const size_t bytes = fq_paged_kv_decode_workspace_needed(int(S), int(HQ), int(HKV), int(D), bs, mb, int(window));
     at::Tensor ws;
     if (workspace.has_value()) {
         ws = *workspace;

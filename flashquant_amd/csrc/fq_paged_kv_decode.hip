@@ -631,15 +631,16 @@ struct KvPlan {
 // The workgroup: four heads and two wavefronts of each draw best where there is much (see above); where a call has at most two
 // tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.2 -> 10.1 us,
 // 1 x 4000 13.6 -> 12.0, 8 heads over 1, 4 x 1500 14.6 -> 12.6; but 61 of 500 to 16000 343 -> 355.
+// tables of so many tiles are never divided
+int kv_whole_tiles(int D) { return D == 256 ? 10 : D == 128 ? 14 : 24; }
 KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {
     int64_t tiles = (max_tokens + fq::kKvTile - 1) / fq::kKvTile;
     if (window > 0 && window / fq::kKvTile + 2 < tiles) tiles = window / fq::kKvTile + 2;
     const int64_t whole = int64_t(S) * H_KV, cus = fq_host::device_cu_count();
     const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
     KvPlan r = {0, 1, most};
-    // (each of these holds for fewer tiles where it holds for more: the room of a call does not depend on its window)
-    const int small = D == 256 ? 10 : D == 128 ? 14 : 24, middle = D == 256 ? 12 : 25;
-    if (tiles <= small || (tiles <= middle && 8 * whole >= 3 * cus) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
+    const int middle = D == 256 ? 12 : 25;
+    if (tiles <= kv_whole_tiles(D) || (tiles <= middle && 8 * whole >= 3 * cus) || (tiles <= 64 && whole >= cus / 2 && whole < 2 * cus) ||
         (together == 1 && D != 256 && tiles <= 80 && whole >= 2 * cus) || int64_t(S) * tiles >= (1LL << 31)) {                 // (more tiles than are counted)
         if (together == 4 && whole >= 8 * cus) {
             // fewer workgroups: 256 of 50 to 300 tokens, 32 heads over 8 of 128, 40 us; 52 with a head a workgroup
@@ -723,10 +724,17 @@ int launch_kv_type(const fq::KvDecodeParams& p, const KvPlan& plan, int dtype, h
 
 extern "C" size_t fq_paged_kv_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq) {
     if (check_kv_shape(num_seqs, H_Q, H_KV, D, block_size, max_blocks_per_seq, 1) != FQ_OK || num_seqs == 0) return 0;
-    // (a window only takes tiles away: what needs none without it needs none with it, but for tiles beyond what is counted)
+    // (the calls that need none lie in bands of sizes: a caller who has room for the largest has it for all)
     const int64_t tokens = int64_t(max_blocks_per_seq) * block_size;
-    if (kv_plan(num_seqs, H_KV, D, tokens, 0).shares == 0 && int64_t(num_seqs) * (tokens / fq::kKvTile + 1) < (1LL << 31)) return 0;
+    if ((tokens + fq::kKvTile - 1) / fq::kKvTile <= kv_whole_tiles(D)) return 0;
     return kv_room(num_seqs, H_Q, D, kv_most_shares(H_KV)).all;
+}
+
+extern "C" size_t fq_paged_kv_decode_workspace_needed(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq,
+                                                      int window) {
+    if (check_kv_shape(num_seqs, H_Q, H_KV, D, block_size, max_blocks_per_seq, 1) != FQ_OK || num_seqs == 0 || window < 0) return 0;
+    const KvPlan plan = kv_plan(num_seqs, H_KV, D, int64_t(max_blocks_per_seq) * block_size, window);
+    return kv_room(num_seqs, H_Q, D, plan.shares == 0 ? 0 : kv_most_shares(H_KV)).all;
 }
 
 extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,

@@ -66,12 +66,13 @@ def paged_kv_decode(
     float16 or bfloat16, through ``block_table`` (num_seqs, max_blocks) and ``seq_lens`` (num_seqs,), int32, the new token counted.
 
     ``window``: only so many of a sequence's last tokens are seen (0: all).  Tokens on pages outside the cache (an entry of -1) are
-    not seen; a row that sees none is zero; a seen value that is infinite or NaN makes its coordinate infinite or NaN.  ``return_lse`` adds the float32 logarithm of the softmax's denominator (num_seqs, H_Q),
-    -inf for such rows.  The caches may be strided (halves of one tensor, heads before tokens).  ``workspace``: uint8, at least
-    ``_C.paged_kv_decode_workspace_bytes(...)`` bytes, for callers that allocate nothing; it holds nothing from one call to the next,
-    and calls that may run at the same time (on two streams, in two graphs) need one each.  ``out``: contiguous, apart from the other
-    operands.  No gradient is recorded.  A sequence's last bits may depend on the lengths of the others, which decide where
-    it is divided."""
+    not seen; a row that sees none is zero; a seen value that is infinite or NaN makes its coordinate infinite or NaN.  ``return_lse``
+    adds the float32 logarithm of the softmax's denominator (num_seqs, H_Q), -inf for rows that see nothing.  The caches may be
+    strided (halves of one tensor, heads before tokens).  ``workspace``: uint8, at least ``_C.paged_kv_decode_workspace_bytes(...)``
+    bytes (of the largest call: smaller batches and narrower tables need no more), for callers that allocate nothing; it holds
+    nothing from one call to the next, and calls that may run at the same time (on two streams, in two graphs) need one each.
+    ``out``: contiguous, apart from the other operands.  No gradient is recorded.  A sequence's last bits may depend on the lengths of
+    the others and on the table's width, which decide where it is divided."""
     require_gpu(q, "q")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])

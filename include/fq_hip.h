@@ -689,10 +689,13 @@ int fq_rotary_paged_store(const void* q, const int64_t* q_strides, void* q_out, 
  * Tokens on pages outside [0, num_blocks) are not seen.  A row that sees no token, or whose scores are all -inf, is 0 with an lse of
  * -inf.  Weights keep 16 bits and more, sums and maxima 32.  Long sequences are cut into parts that a second launch joins; the
  * parts follow from all lengths, so the last bits of a row may differ with the batch that it is in.
- *   workspace      fq_paged_kv_decode_workspace_bytes bytes (0: none needed), 256-byte aligned, any contents
+ *   workspace      fq_paged_kv_decode_workspace_bytes bytes (0: none needed), 256-byte aligned, any contents.  That room does not shrink
+ *                  with num_seqs or max_blocks_per_seq, so what suffices for the largest call suffices for all, with any window.  A
+ *                  call that attends to sequences undivided needs none: fq_paged_kv_decode_workspace_needed says what this one must have.
  * D in {64, 128, 256}, block_size in {8, 16, 32}, H_Q / H_KV <= 16, caches 16-byte aligned with strides that are multiples of 8.
  */
 size_t fq_paged_kv_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq);
+size_t fq_paged_kv_decode_workspace_needed(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq, int window);
 int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
                        const void* value_cache, const int64_t* value_strides, const int32_t* block_table, int64_t block_table_stride,
                        const int32_t* seq_lens, void* out, float* lse, int num_seqs, int H_Q, int H_KV, int D, int block_size,

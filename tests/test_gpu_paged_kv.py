@@ -909,3 +909,18 @@ def test_results_have_memory_of_their_own():
         t = getattr(s, name)
         t.resize_(t.numel() + 3).fill_(-9)
         assert all(torch.equal(getattr(s, n), x) for n, x in kept.items()), name
+
+
+def test_decode_in_the_room_of_the_largest_call():
+    """One workspace, of the size that the largest batch asks for, serves all of them."""
+    g = gen(7)
+    kc, vc, _ = caches("apart", 60, 16, 8, 128, BF, g)
+    room = native().paged_kv_decode_workspace_bytes(63, 32, 8, 128, 16, 128)
+    ws = torch.full((room,), 0xff, dtype=torch.uint8, device=DEV)
+    for seqs in (1, 2, 15, 16, 32, 63):
+        for columns in (3, 28, 30, 51, 128):
+            table = torch.randint(0, 60, (seqs, columns), dtype=torch.int32, generator=g).to(DEV)
+            lens = torch.randint(0, 16 * columns + 1, (seqs,), dtype=torch.int32, generator=g).to(DEV)
+            q = torch.randn(seqs, 32, 128, generator=g).to(BF).to(DEV)
+            for window in (0, 200):
+                assert torch.equal(K.paged_kv_decode(q, kc, vc, table, lens, window=window, workspace=ws), K.paged_kv_decode(q, kc, vc, table, lens, window=window))

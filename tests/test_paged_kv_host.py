@@ -187,3 +187,24 @@ def test_advance_argument_errors(lib):
     assert call(page=24) == FQ_BLOCK
     for name in ("lens", "end", "context", "start", "cu", "positions", "table", "rows", "row_lens"):
         assert call(**{name: 0}) == FQ_NULL, name
+
+
+def test_decode_room_does_not_shrink_with_larger_calls(lib):
+    """A workspace for the largest batch and table serves every smaller one, whatever line between the ways to divide lies between."""
+    need = lib.fq_paged_kv_decode_workspace_bytes
+    need.argtypes, need.restype = [I] * 6, Z
+    for hq, hkv, d in ((32, 8, 128), (8, 1, 128), (32, 32, 128), (16, 2, 64), (32, 8, 256), (128, 128, 64)):
+        for page in (8, 16, 32):
+            columns = [1, 2, 5, 9, 10, 14, 15, 24, 25, 26, 40, 64, 65, 80, 81, 128, 200, 512, 5000, 60000]
+            table = [[need(s, hq, hkv, d, page, c) for c in columns] for s in (*range(1, 140), 200, 255, 256, 257, 511, 512, 513, 1000, 2047, 2048, 5000, 70000)]
+            for smaller, larger in zip(table, table[1:]):
+                assert all(a <= b for a, b in zip(smaller, larger)), (hq, hkv, d, page)
+            for row in table:
+                assert row == sorted(row), (hq, hkv, d, page)
+    must = lib.fq_paged_kv_decode_workspace_needed
+    must.argtypes, must.restype = [I] * 7, Z
+    for s in (1, 15, 16, 63, 64, 255, 256, 257, 3000, 70000):
+        for c in (1, 14, 30, 31, 52, 60, 130, 700, 1 << 16):
+            for window in (0, 1, 33, 500, 900, 3000, 1 << 30):
+                assert must(s, 32, 8, 128, 16, c, window) in (0, need(s, 32, 8, 128, 16, c))
+    assert must(0, 32, 8, 128, 16, 9, 0) == 0 and must(1, 32, 8, 96, 16, 9, 0) == 0 and must(1, 32, 8, 128, 16, 9, -1) == 0
