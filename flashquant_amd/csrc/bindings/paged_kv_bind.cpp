@@ -97,7 +97,7 @@ bool may_meet(const at::Tensor& a, const at::Tensor& b) {
     const RowStrides sa = strides_of(a), sb = strides_of(b);
     const int64_t step = sa.s[1], size = a.element_size();
     if (step <= 0 || sb.s[1] != step || sa.s[0] % step != 0 || sb.s[0] % step != 0 || (pb - pa) % size != 0) return true;
-    auto span = [](const at::Tensor& t) { return (t.size(-2) - 1) * t.stride(-2) + t.size(-1); };
+    auto span = [](const at::Tensor& t) { return (t.size(-2) - 1) * t.stride(-2) + (t.size(-1) - 1) * t.stride(-1) + 1; };
     const int64_t apart = ((pb - pa) / size % step + step) % step;
     return span(a) > apart || apart + span(b) > step;
 }

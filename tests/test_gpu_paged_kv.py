@@ -924,3 +924,17 @@ def test_decode_in_the_room_of_the_largest_call():
             q = torch.randn(seqs, 32, 128, generator=g).to(BF).to(DEV)
             for window in (0, 200):
                 assert torch.equal(K.paged_kv_decode(q, kc, vc, table, lens, window=window, workspace=ws), K.paged_kv_decode(q, kc, vc, table, lens, window=window))
+
+
+def test_outputs_in_the_memory_of_transposed_inputs_are_refused():
+    freq, _ = K.rotary_frequencies(64, device=DEV)
+    buf = torch.zeros(5, 512, dtype=BF, device=DEV)
+    x = buf[:, :256].view(5, 64, 4).transpose(1, 2)                        # a row's values lie four apart, over 256
+    positions, apart = torch.arange(5, device=DEV), torch.ones(5, 4, 64, dtype=BF, device=DEV)
+    for at in (0, 128, 255):
+        out = buf.as_strided((5, 4, 64), (512, 64, 1), at)
+        with pytest.raises(ValueError, match="share no memory"):
+            K.rotary_embedding(x, None, positions, freq, out=(out, None))
+        with pytest.raises(ValueError, match="share no memory"):
+            K.rotary_embedding(apart, x, positions, freq, out=(out, torch.empty_like(apart)))
+    K.rotary_embedding(x, None, positions, freq, out=(buf[:, 256:].view(5, 4, 64), None))
