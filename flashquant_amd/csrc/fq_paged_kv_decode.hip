@@ -100,8 +100,8 @@ __device__ __forceinline__ int sum_upto(int v) {
 }
 
 // Where share x begins.  False: there is no such share.  The lengths are read kGroups x 64 at a time, all of them asked for before
-// the first is used, and up to that many only once (4096 sequences of 100 to 1200 tokens, 8 heads over 1: 268 us, and 468 with 64
-// at a time here and in the second kernel; 1 x 777 tokens 9.2, and 9.4 with 512).
+// the first is used, and up to that many only once (4096 sequences of 100 to 1200 tokens in a table for 4096, 8 heads over 1: 266 us,
+// and 468 with 64 at a time here and in the second kernel; 1 x 777 tokens 9.2, and 9.4 with 512).
 template <int kGroups>
 __device__ __forceinline__ bool kv_place(const KvDecodeParams& p, int x, int lane, KvPlace& r) {
     constexpr int kAll = kGroups * kWave;
@@ -616,6 +616,9 @@ struct KvPlan {
     int heads, waves;    // KV heads of a workgroup, wavefronts of each
 };
 
+// The host knows the table's width, not the lengths, and divides for sequences that fill it.  All times below are of tables as wide as
+// the longest sequence; in wider ones short sequences are divided where that costs (tables for 4096 and for 131072 tokens: 1 x 777 8.9 and
+// 10.1 us, 10 x 430 12.2 and 12.2, 16 x 500 13.8 and 13.8, 32 x 1000 26.9 and 27.1).
 // Undivided sequences or shares: a CU takes its tiles at 40 to 60 GB/s, so few long sequences have to be spread, but the second
 // launch costs 3 us, and a share that goes on with another sequence starts from nothing again (3 us; asking for that one's
 // pages ahead was no faster).  In us, undivided / shares, 32 heads over 8, bf16:

@@ -171,9 +171,10 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_schedule_kernel(const 
 // What follows a schedule, in one launch: lengths and first free page as the next one finds them, and a row of pages and a length
 // for each of the step's tokens.  A schedule packs the tokens and leaves out requests that bring none, so token i is not of request
 // i: attention of single tokens goes by these rows.
-//   What bounds it: latency, and for wide tables the copy.  A workgroup takes up to 2048 entries of one row (64 tokens of 8192 pages:
-// 4 MB over 256 workgroups).  It finds the request with one look at all of `cu`, in as few trips to memory as there are 1024 requests;
-// a search would take a trip for every halving.
+//   What bounds it: latency, and for wide tables the copy.  A workgroup takes up to 2048 entries of one row.  It finds the request with
+// one look at all of `cu`, a trip to memory for every 1024 requests, where a search would take one for every halving.  Measured: 64 tokens
+// of 256 pages 3.3 us, of 8192 4.0, 512 of 8192 (34 MB) 6.9 (4.9 TB/s); a whole schedule of 64 sequences in a graph 8.0, and 8.7 with two
+// launches that moved lengths and first page alone.
 constexpr int kRowEntries = 8 * kScheduleThreads;
 
 struct AdvanceParams {
