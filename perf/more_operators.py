@@ -65,7 +65,7 @@ def listed():
 # (query heads, KV heads, dimension): whole models and their tensor-parallel shards
 HEADS = ((32, 8, 128), (64, 8, 128), (32, 4, 128), (16, 2, 128), (8, 1, 128), (32, 32, 128), (32, 8, 64), (16, 4, 64), (32, 8, 256),
          (16, 4, 256), (8, 1, 256))
-MAX_VALUES = 700 << 20           # keys that one drawn decode gathers, in values, padded
+MAX_VALUES = 450 << 20           # keys that one drawn decode gathers, in values, padded
 
 
 def _log(rng, lo, hi):
