@@ -11,6 +11,7 @@ PYBIND11_MODULE(_C, m) {
     m.attr("abi_version") = fq_abi_version();
     bind_kernels(m);
     bind_paged_kv(m);
+    bind_paged_kv8(m);
     bind_codebook(m);
     bind_quantizer(m);
     bind_quantizer_classes(m);

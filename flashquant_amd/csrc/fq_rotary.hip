@@ -11,7 +11,7 @@
 // of these tokens use them.  The product and its reduction are in 64 bits: in 32 an angle at position 10^6 is off by 0.03.
 // Measured: 16384 tokens of 32 + 8 heads of 128, bf16, 54.4 us (6.2 TB/s; a copy 5.9); 3001 of 16 + 4 heads of 256, 64 of them
 // turned, fp16, 11.7 us; with the store 12000 tokens of 32 + 8 + 8 49.6 us (5.9 TB/s); 32 tokens 3.1 us.
-#include "fq_device.hpp"
+#include "fq_rotary.hpp"
 
 namespace fq {
 
@@ -44,23 +44,6 @@ struct RotaryParams {
     uint32_t units_magic, heads_magic;          // ceil(2^32 / .)
     float scale, sign;                          // sign -1: negative angles
 };
-
-// i / d for i d < 2^32, with magic = ceil(2^32 / d)
-__device__ __forceinline__ uint32_t divide(uint32_t i, uint32_t d, uint32_t magic) { return d == 1 ? i : __umulhi(i, magic); }
-
-// cos and sin of 2 pi x: the nearest quarter turn is taken off exactly and the rest, at most an eighth of a turn, turned into
-// radians in 64 bits; then the Taylor series in 32, whose next terms are below 2^-28.  sin as t + t (t^2 ...), cos as 1 + t^2 ...,
-// so that the roundings inside count little: within 1.6 2^-24.
-__device__ __forceinline__ float2v turn_cos_sin(double x) {
-    const double quarter = __builtin_rint(4.0 * x);
-    const float t = float(__builtin_fma(-0.25, quarter, x) * 6.283185307179586476925287);
-    const float z = t * t;
-    const float s = __builtin_fmaf(t, z * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), t);
-    const float c = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
-    const int k = int(quarter - 4.0 * __builtin_floor(0.25 * quarter));      // 0 .. 3
-    const float a = (k & 1) ? s : c, b = (k & 1) ? c : s;
-    return float2v{k == 1 || k == 2 ? -a : a, k >= 2 ? -b : b};
-}
 
 // VEC elements as they lie in memory, and as float32
 template <typename T, int VEC> struct Piece {
@@ -96,17 +79,8 @@ template <typename T, int VEC, bool STREAM> __device__ __forceinline__ void stor
     }
 }
 
-// (x0, x1) turned.  Which product is rounded is spelled out: the same bits at every alignment.
-__device__ __forceinline__ float2v turned_pair(float x0, float x1, float2v cs) {
-    return float2v{__builtin_fmaf(x0, cs.x, -(x1 * cs.y)), __builtin_fmaf(x1, cs.x, x0 * cs.y)};
-}
-
 // The eight pairs of two 16-byte parts of 16-bit values, a word at a time: words of `a` and `d` hold two elements of a part each.
 // `first`, `later`: angles of pairs 0 to 3 and of pairs 4 to 7.
-template <int DT> __device__ __forceinline__ uint32_t rounded_words(float x, float y) {
-    if constexpr (DT == FQ_F16) asm("" : "+v"(x), "+v"(y));      // (as in from_float)
-    return round_pair<DT>(x, y);
-}
 template <int DT, bool INTERLEAVED, typename P>
 __device__ __forceinline__ void turn_words(const float2v* first, const float2v* later, P& pa, P& pd) {
     uint4v a = __builtin_bit_cast(uint4v, pa), d = __builtin_bit_cast(uint4v, pd);
@@ -245,16 +219,6 @@ __global__ __launch_bounds__(kRotaryThreads, 6) void rotary_kernel(const RotaryP
 
 namespace {
 
-uint32_t magic_of(int d) { return uint32_t(((uint64_t(1) << 32) + uint32_t(d) - 1) / uint32_t(d)); }
-
-// whether rows at `ptr` with these strides can be read and written 16 bytes at a time
-bool wide_rows(const void* ptr, const int64_t* strides, int n, int vec) {
-    if (!fq_host::aligned(ptr, 16)) return false;
-    for (int i = 0; i < n; ++i)
-        if (strides[i] % vec != 0) return false;
-    return true;
-}
-
 template <int DT, typename T, int VEC, bool STORE, bool STREAM>
 void launch_rows(const fq::RotaryParams& p, bool interleaved, unsigned groups, hipStream_t s) {
     if (interleaved) fq::rotary_kernel<DT, T, VEC, true, STORE, STREAM><<<groups, fq::kRotaryThreads, 0, s>>>(p);
@@ -290,20 +254,6 @@ int launch_rotary(fq::RotaryParams& p, int64_t tokens, bool wide, bool interleav
     else if (stream) launch_rows<DT, T, VEC, STORE, true>(p, interleaved, n, s);
     else launch_rows<DT, T, VEC, STORE, false>(p, interleaved, n, s);
     return fq_host::check_launch();
-}
-
-int check_rotary(int64_t tokens, int H_Q, int H_K, int half, int D, int position_bytes) {
-    if (tokens < 0 || H_Q < 0 || H_K < 0 || H_Q + int64_t(H_K) == 0 || H_Q > 4096 || H_K > 4096) return FQ_ERR_BAD_SHAPE;
-    if (half < 1 || D < 2 * half || D > 1024) return FQ_ERR_BAD_SHAPE;
-    if (position_bytes != 4 && position_bytes != 8) return FQ_ERR_UNSUPPORTED_DTYPE;
-    return FQ_OK;
-}
-
-// strides but those of a batch or a block are 32-bit in the kernel
-bool fits(const int64_t* strides, int n) {
-    for (int i = 0; i < n; ++i)
-        if (strides[i] > 0x7fffffffLL || strides[i] < -0x7fffffffLL) return false;
-    return true;
 }
 
 fq::RotaryRows rows_of(const void* src, const int64_t* in, void* dst, const int64_t* out, int heads) {

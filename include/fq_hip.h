@@ -702,6 +702,53 @@ int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_
                        int max_blocks_per_seq, int64_t num_blocks, float sm_scale, int window, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/*
+ * A paged cache of 8-bit rows on the same tables and slots.  A row, the D values of a token and KV head, is D e4m3 codes (OCP: four
+ * significant bits, up to 448, no infinities) and one E8M0 byte: value = code * 2^(byte - 127).
+ *   codes    addressed by three strides in bytes, host arrays {block, token, head}; the D codes of a row are contiguous
+ *   scales   two strides {block, head}; the bytes of a page's tokens are contiguous
+ *
+ * fq_rotary_paged_store8: fq_rotary_paged_store into such a cache.  Of a row's float32 values (keys: as rotated, not rounded to 16
+ *   bits first) the largest finite magnitude a gives the power, floor(log2 a) - 8, one more where a > 1.75 * 2^floor(log2 a), not
+ *   below -118 (a row of zeros: that) or above 120; the codes are rounded to nearest even.  Infinite values become NaN.
+ *   D in {64, 128, 256}.  Fastest where half is a multiple of 8 and rows lie at multiples of 16 bytes.
+ *
+ * fq_paged_kv8_read: tokens back as 16-bit rows, code * 2^(byte - 127) rounded to fp16 or bf16 (bf16: exact from 2^-126 on).
+ *   cu_seqlens     (num_seqs + 1,) int32, not decreasing: sequence s gives tokens starts[s] (int32; NULL: 0) and on to rows
+ *                  cu_seqlens[s] .. cu_seqlens[s + 1] of the outputs
+ *   keys, values   (num_tokens, H_KV, D) out.  Rows of tokens that are not on a page of the cache, or before the sequence's first or
+ *                  beyond its max_blocks_per_seq pages, are 0; rows behind the last sequence are 0 with fill != 0 and left as they were
+ *                  without; sequences' rows beyond num_tokens are not written
+ *   Codes 16-byte aligned with strides that are multiples of 16.
+ *
+ * fq_paged_kv8_decode: fq_paged_kv_decode over such a cache; q, out fp16 or bf16.  The codes are multiplied as they are and the powers
+ *   applied in float32, so nothing is rounded that was not in the cache.  Scale bytes 1 to 254.  Codes aligned as above, scales 8
+ *   bytes with strides that are multiples of 8.  Workspace as there.
+ */
+int fq_rotary_paged_store8(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int H_Q, const void* k,
+                           const int64_t* k_strides, const void* v, const int64_t* v_strides, int H_KV, const void* positions,
+                           int position_bytes, const double* inv_freq, int half, int interleaved, float scale,
+                           const int64_t* slot_mapping, int64_t num_mapped, uint8_t* key_cache, const int64_t* key_strides,
+                           uint8_t* value_cache, const int64_t* value_strides, uint8_t* key_scales, const int64_t* key_scale_strides,
+                           uint8_t* value_scales, const int64_t* value_scale_strides, int block_size, int64_t num_blocks, int64_t tokens,
+                           int D, int dtype, void* stream);
+
+int fq_paged_kv8_read(const uint8_t* key_cache, const int64_t* key_strides, const uint8_t* value_cache, const int64_t* value_strides,
+                      const uint8_t* key_scales, const int64_t* key_scale_strides, const uint8_t* value_scales,
+                      const int64_t* value_scale_strides, const int32_t* block_table, int64_t block_table_stride,
+                      const int32_t* cu_seqlens, const int32_t* starts, void* keys, void* values, int fill, int num_seqs,
+                      int64_t num_tokens, int H_KV, int D, int block_size, int max_blocks_per_seq, int64_t num_blocks, int dtype,
+                      void* stream);
+
+size_t fq_paged_kv8_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq);
+size_t fq_paged_kv8_decode_workspace_needed(int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq, int window);
+int fq_paged_kv8_decode(const void* q, const int64_t* q_strides, const uint8_t* key_cache, const int64_t* key_strides,
+                        const uint8_t* value_cache, const int64_t* value_strides, const uint8_t* key_scales,
+                        const int64_t* key_scale_strides, const uint8_t* value_scales, const int64_t* value_scale_strides,
+                        const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens, void* out, float* lse,
+                        int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                        float sm_scale, int window, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
