@@ -1,4 +1,4 @@
-// Bindings of the operators around an 8-bit paged cache: rotary store, read and decode.  Rows are e4m3 (num_blocks, block_size, H_KV,
+// Bindings of the operators around an 8-bit paged cache (rotary store, read and decode) and of decode over shared prefixes.  Rows are e4m3 (num_blocks, block_size, H_KV,
 // D), their powers of two E8M0 (num_blocks, H_KV, block_size).  There is no CPU path: a tensor that is not on the GPU is an error.
 
 #include "paged_common.h"
@@ -222,6 +222,54 @@ std::tuple<at::Tensor, MaybeTensor> paged_kv8_decode(const at::Tensor& q, const 
     return {c.out, return_lse ? MaybeTensor(c.lse) : std::nullopt};
 }
 
+// 16-bit caches, or 8-bit ones with their scales
+std::tuple<at::Tensor, MaybeTensor> paged_prefix_decode(const at::Tensor& q, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                                                        const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& prefix_ids,
+                                                        const at::Tensor& prefix_lens, double sm_scale, const MaybeTensor& key_scales,
+                                                        const MaybeTensor& value_scales, const MaybeTensor& out, bool return_lse,
+                                                        const MaybeTensor& workspace) {
+    fqbind::require_gpu(q, "q");
+    check(q.dim() == 3 && (q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16), "q must be float16 or bfloat16 of shape (num_seqs, H_Q, D)");
+    check(key_scales.has_value() == value_scales.has_value(), "key_scales and value_scales belong together");
+    const bool f8 = key_scales.has_value();
+    Side ks = {}, vs = {};
+    if (f8) {
+        ks = side_of(key_cache, *key_scales, q, q.size(2));
+        vs = side_of(value_cache, *value_scales, q, q.size(2));
+    } else {
+        const Cache k = cache_of(key_cache, q, q, "key_cache"), v = cache_of(value_cache, q, q, "value_cache");
+        for (int i = 0; i < 3; ++i) {
+            ks.s[i] = key_cache.size(i) > 1 ? k.s[i] : 0;
+            vs.s[i] = value_cache.size(i) > 1 ? v.s[i] : 0;
+        }
+    }
+    check_alike(key_cache, value_cache);
+    DecodeCall c;
+    check_decode(c, q, key_cache, block_table, seq_lens);
+    check_place(prefix_ids, q, "prefix_ids");
+    check_place(prefix_lens, q, "prefix_lens");
+    check(prefix_ids.dim() == 1 && prefix_ids.scalar_type() == at::kInt && prefix_ids.size(0) == c.S, "prefix_ids must be int32 of shape (num_seqs,)");
+    check(prefix_lens.dim() == 1 && prefix_lens.scalar_type() == at::kInt && prefix_lens.size(0) <= 1024,
+          "prefix_lens must be int32 of one dimension, of 1024 prefixes at most");
+    c10::DeviceGuard guard(q.device());
+    const at::Tensor ids = prefix_ids.contiguous(), lens = prefix_lens.contiguous();
+    const size_t bytes = fq_paged_prefix_decode_workspace_bytes(int(c.S), int(c.HQ), int(c.HKV), int(c.D), int(lens.size(0)));
+    set_up_decode(c, q, seq_lens,
+                  {&key_cache, &value_cache, f8 ? &*key_scales : &key_cache, f8 ? &*value_scales : &value_cache, &block_table, &seq_lens, &prefix_ids, &prefix_lens},
+                  out, return_lse, bytes, workspace, "workspace must be a contiguous uint8 GPU tensor of at least paged_prefix_decode_workspace_bytes(...) bytes");
+    const int64_t qs[2] = {c.q.stride(0), c.q.stride(1)};
+    const int st = fq_paged_prefix_decode(c.q.data_ptr(), qs, key_cache.data_ptr(), ks.s, value_cache.data_ptr(), vs.s, ks.scales, ks.ss, vs.scales, vs.ss,
+                                          block_table.data_ptr<int32_t>(), block_table.stride(0), c.lens.data_ptr<int32_t>(),
+                                          ids.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), int(lens.size(0)), c.out.data_ptr(),
+                                          return_lse ? c.lse.data_ptr<float>() : nullptr, int(c.S), int(c.HQ), int(c.HKV), int(c.D), c.block_size,
+                                          c.max_blocks, key_cache.size(0), float(sm_scale), fqbind::dtype_code(q.scalar_type(), "paged_prefix_decode"),
+                                          c.ws.defined() ? c.ws.data_ptr() : nullptr, c.ws.defined() ? size_t(c.ws.numel()) : 0,
+                                          fqbind::current_stream(q));
+    fqbind::raise_on_error(st, "paged_prefix_decode");
+    if (out.has_value()) written(c.out);
+    return {c.out, return_lse ? MaybeTensor(c.lse) : std::nullopt};
+}
+
 }  // namespace
 
 void bind_paged_kv8(py::module_& m) {
@@ -238,4 +286,10 @@ void bind_paged_kv8(py::module_& m) {
           "Attention of one query per sequence over an 8-bit paged cache: (out, lse or None)");
     m.def("paged_kv8_decode_workspace_bytes", &fq_paged_kv8_decode_workspace_bytes, py::arg("num_seqs"), py::arg("H_Q"), py::arg("H_KV"),
           py::arg("head_dim"), py::arg("block_size"), py::arg("max_blocks_per_seq"));
+    m.def("paged_prefix_decode", &paged_prefix_decode, py::arg("q"), py::arg("key_cache"), py::arg("value_cache"), py::arg("block_table"),
+          py::arg("seq_lens"), py::arg("prefix_ids"), py::arg("prefix_lens"), py::arg("sm_scale"), py::arg("key_scales") = py::none(),
+          py::arg("value_scales") = py::none(), py::arg("out") = py::none(), py::arg("return_lse") = false, py::arg("workspace") = py::none(),
+          "Attention of one query per sequence where sequences begin with the same pages: (out, lse or None)");
+    m.def("paged_prefix_decode_workspace_bytes", &fq_paged_prefix_decode_workspace_bytes, py::arg("num_seqs"), py::arg("H_Q"), py::arg("H_KV"),
+          py::arg("head_dim"), py::arg("num_prefixes"));
 }

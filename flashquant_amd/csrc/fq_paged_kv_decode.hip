@@ -38,10 +38,6 @@ extern "C" int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const
     const int st = set_up_call(call, q, q_strides, block_table, block_table_stride, seq_lens, out, lse, num_seqs, H_Q, H_KV, D, block_size,
                                max_blocks_per_seq, num_blocks, sm_scale, window, workspace, workspace_bytes);
     if (st != FQ_OK) return st;
-    fq::KvDecodeParams& p = call.p;
-    p.kc = key_cache;
-    p.vc = value_cache;
-    p.k_block = key_strides[0]; p.k_token = key_strides[1]; p.k_head = key_strides[2];
-    p.v_block = value_strides[0]; p.v_token = value_strides[1]; p.v_head = value_strides[2];
-    return launch_kv_any<false>(p, call.plan, D, dtype, static_cast<hipStream_t>(stream));
+    set_rows(call.p, key_cache, key_strides, value_cache, value_strides);
+    return launch_kv_any<false>(call.p, call.plan, D, dtype, static_cast<hipStream_t>(stream));
 }

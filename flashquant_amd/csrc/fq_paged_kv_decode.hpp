@@ -839,7 +839,25 @@ int launch_kv_any(const fq::KvDecodeParams& p, const KvPlan& plan, int D, int dt
     }
 }
 
-// What the entries for both kinds of rows check and set up alike; the caches' own operands are the caller's.
+// What the entries for both kinds of rows set up alike; the caches' own operands are the caller's, and room for parts.
+void set_up_params(fq::KvDecodeParams& p, const void* q, const int64_t* q_strides, const int32_t* block_table, int64_t block_table_stride,
+                   const int32_t* seq_lens, void* out, float* lse, int S, int H_Q, int H_KV, int block_size, int max_blocks, int64_t num_blocks,
+                   float sm_scale, int window, const KvPlan& plan) {
+    p = {};
+    p.q = static_cast<const uint16_t*>(q);
+    p.table = block_table;
+    p.lens = seq_lens;
+    p.out = static_cast<uint16_t*>(out);
+    p.lse = lse;
+    p.q_seq = q_strides[0]; p.q_head = q_strides[1];
+    p.table_row = block_table_stride;
+    p.S = S; p.H_KV = H_KV; p.G = H_Q / H_KV;
+    p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
+    p.max_blocks = max_blocks; p.num_blocks = int(num_blocks); p.window = window;
+    p.shares = plan.shares; p.min_tiles = plan.waves;        // a tile a wavefront
+    p.scale_log2 = sm_scale * fq::kLog2e;
+}
+
 struct KvCall {
     KvPlan plan;
     fq::KvDecodeParams p;
@@ -856,27 +874,21 @@ int set_up_call(KvCall& call, const void* q, const int64_t* q_strides, const int
         if (!fq_host::aligned(workspace, 256)) return FQ_ERR_MISALIGNED;
     }
     fq::KvDecodeParams& p = call.p;
-    p = {};
-    p.q = static_cast<const uint16_t*>(q);
-    p.table = block_table;
-    p.lens = seq_lens;
-    p.out = static_cast<uint16_t*>(out);
-    p.lse = lse;
+    set_up_params(p, q, q_strides, block_table, block_table_stride, seq_lens, out, lse, S, H_Q, H_KV, block_size, max_blocks, num_blocks, sm_scale,
+                  window, call.plan);
     char* ws = static_cast<char*>(workspace);
     p.part_o = reinterpret_cast<float*>(ws);
     p.part_m = reinterpret_cast<float*>(ws + room.o);
     p.part_l = reinterpret_cast<float*>(ws + room.o + room.m);
     p.place = reinterpret_cast<int2*>(ws + room.o + 2 * room.m);
-    p.q_seq = q_strides[0]; p.q_head = q_strides[1];
-    p.table_row = block_table_stride;
-    p.S = S; p.H_KV = H_KV; p.G = H_Q / H_KV;
-    p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;
-    p.max_blocks = max_blocks; p.num_blocks = int(num_blocks); p.window = window;
-    p.shares = call.plan.shares; p.min_tiles = call.plan.waves;        // a tile a wavefront
-    p.scale_log2 = sm_scale * fq::kLog2e;
     return FQ_OK;
 }
 
+void set_rows(fq::KvDecodeParams& p, const void* key_cache, const int64_t* key_strides, const void* value_cache, const int64_t* value_strides) {
+    p.kc = key_cache; p.vc = value_cache;
+    p.k_block = key_strides[0]; p.k_token = key_strides[1]; p.k_head = key_strides[2];
+    p.v_block = value_strides[0]; p.v_token = value_strides[1]; p.v_head = value_strides[2];
+}
 // Codes are read 16 bytes at a time, the powers of eight tokens 8.
 bool codes_aligned(const void* codes, const int64_t* strides, const void* scales, const int64_t* scale_strides) {
     return fq_host::aligned(codes, 16) && strides[0] % 16 == 0 && strides[1] % 16 == 0 && strides[2] % 16 == 0 && fq_host::aligned(scales, 8) &&

@@ -1,0 +1,595 @@
+// Attention of one new token per sequence where sequences begin with the same pages: the keys of a shared prefix are read once for all
+// queries that see them, what every sequence has behind it is read as in fq_paged_kv_decode.hpp, and the parts are joined by their
+// maxima and sums:
+//
+//   o = (sum_{j in prefix} p_j v_j + sum_{j behind} p_j v_j) / (sum_{j in prefix} p_j + sum_{j behind} p_j)
+//
+// Members of prefix i are the sequences whose id it is and that are as long as it; no lists of them are asked for.
+#include "fq_paged_kv_decode.hpp"
+
+namespace fq {
+
+struct PrefixParams {
+    KvDecodeParams kv;
+    int4* place;                          // (S): first piece of a member's prefix, pieces, row in each, unused
+    int64_t first_row;                    // of the prefixes' partial results, behind those of the sequences' own tokens
+    int shares, min_tiles;                // among which a KV head's work is divided
+    int members;                          // of a workgroup's rows
+};
+
+constexpr int kPrefixRows = 128;
+constexpr int kPrefixMost = 1024;         // prefixes of a call
+
+template <int D> struct PrefixCfg {
+    static constexpr int TT = 8192 / D;                    // tokens of a tile
+    static constexpr int NB = TT / 32, NKS = D / 16, NOB = D / 32, NU = TT / 16, NG = TT / 8;
+    static constexpr int SIDE = TT * D * 2;                // bytes of a tile's keys or values: 16 KB
+    static constexpr int LDS = 4 * SIDE + 2 * TT * 4 + 2 * NG * 4 + kPrefixRows * 4 + 2 * kPrefixMost * 4;
+};
+
+// Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
+__device__ __forceinline__ int coord_of_row(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
+
+// Where a key's 16-byte pieces lie in its row of LDS, so that lanes that read one piece of 16 neighbouring keys reach all banks.
+template <int D> __device__ __forceinline__ int key_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+
+template <int DT> __device__ __forceinline__ float16v wide_mfma(uint4v a, uint4v b, float16v c) {
+    if constexpr (DT == FQ_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16v8, a), __builtin_bit_cast(bf16v8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d, kWave);
+    return v;
+}
+__device__ __forceinline__ int64_t wave_scan64(int64_t v, int lane) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int64_t u = __shfl_up(v, d, kWave);
+        if (lane >= d) v += u;
+    }
+    return v;
+}
+
+// The members of a prefix, 128 rows (member, query head of the KV head) of them a workgroup, against a share of its keys.
+template <int D, int DT, bool F8>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(const PrefixParams pp) {
+    using C = PrefixCfg<D>;
+    using Elem = std::conditional_t<F8, uint8_t, uint16_t>;
+    constexpr int TT = C::TT, NB = C::NB, NKS = C::NKS, NOB = C::NOB, NU = C::NU, NG = C::NG;
+    constexpr int PT = F8 ? FQ_BF16 : DT;                  // of weights and values in the second product
+    constexpr bool TWO_TERMS = F8 && DT == FQ_F16;         // one bf16 term would show in an fp16 result
+    constexpr int KR = F8 ? 4 : 8;                         // keys of a thread's piece of a tile
+    const KvDecodeParams& p = pp.kv;
+    extern __shared__ __attribute__((aligned(256))) uint8_t prefix_lds[];
+    uint8_t* lds = prefix_lds;
+    uint8_t *lk = lds, *lv = lds + 2 * C::SIDE;
+    float* lscale = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, TT): what a key's score is multiplied by
+    int* lvalid = reinterpret_cast<int*>(lscale + 2 * TT);                // (2, NG): whether eight keys are on a page of the cache
+    int* list = lvalid + 2 * NG;                                          // the sequences of the rows
+    const int tid = threadIdx.x, lane = tid & 63, m32 = lane & 31, hf = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = blockIdx.x % p.H_KV, x = blockIdx.x / p.H_KV, G = p.G;
+
+    // ---- the share: members of every prefix, tiles of all, where this one begins -----------------------------------------------
+    int* count = list + kPrefixRows;
+    int* shared_len = count + kPrefixMost;
+    for (int i = tid; i < p.num_prefixes; i += 256) {
+        count[i] = 0;
+        const int n = p.prefix_lens[i] >> p.page_log2 << p.page_log2;
+        shared_len[i] = n > 0 ? n : 0;
+    }
+    __syncthreads();
+    auto member_of = [&](int s) {                          // the prefix that sequence s shares, or -1
+        const int id = p.prefix_ids[s], len = kv_length(p, s);
+        if (uint32_t(id) >= uint32_t(p.num_prefixes)) return -1;
+        const int n = shared_len[id];
+        return n > 0 && n <= len ? id : -1;
+    };
+    for (int s = tid; s < p.S; s += 256) {
+        const int id = member_of(s);
+        if (id >= 0) atomicAdd(&count[id], 1);
+    }
+    __syncthreads();
+    auto tiles_of = [&](int i) { return (shared_len[i] + TT - 1) / TT; };
+    auto groups_of = [&](int i) { return (count[i] + pp.members - 1) / pp.members; };
+    int64_t total = 0;
+    for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) {
+        const int i = i0 + lane;
+        total += wave_sum64(i < p.num_prefixes ? int64_t(tiles_of(i)) * groups_of(i) : 0);
+    }
+    int64_t size = (total + pp.shares - 1) / pp.shares;
+    if (size < pp.min_tiles) size = pp.min_tiles;
+    const int64_t wanted = int64_t(x) * size;
+    if (wanted >= total) return;
+    int64_t left = total - wanted < size ? total - wanted : size;
+    int prefix = 0, group = 0, tile0 = 0, piece = x;       // piece: the share and the groups of rows before this one
+    {
+        int64_t before = 0;
+        for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) {
+            const int i = i0 + lane;
+            const int gs = i < p.num_prefixes && shared_len[i] > 0 ? groups_of(i) : 0;
+            const int64_t units = i < p.num_prefixes ? int64_t(tiles_of(i)) * gs : 0, upto = before + wave_scan64(units, lane);
+            const uint64_t past = __ballot(upto > wanted);
+            const int groups_upto = sum_upto(gs);
+            if (past != 0) {
+                const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                prefix = i0 + at;
+                const int64_t inside = wanted - (__shfl(upto, at, kWave) - __shfl(units, at, kWave));
+                const int tiles = tiles_of(prefix);
+                group = int(inside / tiles);
+                tile0 = int(inside - int64_t(group) * tiles);
+                piece += __builtin_amdgcn_readlane(groups_upto, at) - __builtin_amdgcn_readlane(gs, at) + group;
+                break;
+            }
+            piece += __builtin_amdgcn_readlane(groups_upto, kWave - 1);
+            before = __shfl(upto, kWave - 1, kWave);
+        }
+    }
+    prefix = __builtin_amdgcn_readfirstlane(prefix);
+    group = __builtin_amdgcn_readfirstlane(group);
+    tile0 = __builtin_amdgcn_readfirstlane(tile0);
+    piece = __builtin_amdgcn_readfirstlane(piece);
+
+    // ---- what this thread brings of a tile: the first half of them values, eight tokens of eight coordinates in the order of the
+    // scores' registers; the others keys -----------------------------------------------------------------------------------------
+    const bool brings_values = tid < 128;
+    const int item = tid & 127;
+    const int vgroup = item / (D / 8), vc = item % (D / 8);                              // tokens 16 (vgroup / 2) + 4 (vgroup % 2) + 0 .. 3, + 8
+    const int kpiece = F8 ? item % (D / 16) : item % (D / 8), krow = KR * (F8 ? item / (D / 16) : item / (D / 8));
+    const int page_mask = (1 << p.page_log2) - 1;
+    const int vtoken = 16 * (vgroup >> 1) + 4 * (vgroup & 1);
+    const Elem* kbase = static_cast<const Elem*>(p.kc) + head * p.k_head + (F8 ? 16 : 8) * kpiece;
+    const Elem* vbase = static_cast<const Elem*>(p.vc) + head * p.v_head + 8 * vc;
+
+    for (;;) {
+        const int n_members = count[prefix], shared = shared_len[prefix], tiles = tiles_of(prefix), groups = groups_of(prefix);
+        const int here = left < tiles - tile0 ? int(left) : tiles - tile0, end = tile0 + here;
+        // the group's members, in the order of the sequences
+        if (w == 0) {
+            int rank = 0;
+            const int first = group * pp.members;
+            for (int s0 = 0; s0 < p.S && rank < first + pp.members; s0 += kWave) {
+                const int s = s0 + lane;
+                const bool mine = s < p.S && member_of(s) == prefix;
+                const uint64_t all = __ballot(mine);
+                const int at = rank + __popcll(all & ((uint64_t(1) << lane) - 1)) - first;
+                if (mine && at >= 0 && at < pp.members) list[at] = s;
+                rank += __popcll(all);
+            }
+        }
+        __syncthreads();
+        const int members = n_members - group * pp.members < pp.members ? n_members - group * pp.members : pp.members;
+        const int rows = members * G, blocks = shared >> p.page_log2;
+        const int32_t* table = p.table + int64_t(list[0]) * p.table_row;
+        if (tile0 == 0 && head == 0 && tid < members) pp.place[list[tid]] = int4{piece, int(1 + (tiles - here + size - 1) / size), tid * G, 0};
+        const int row = 32 * w + m32;
+        const bool live = 32 * w < rows;
+        uint4v qb[NKS];
+        {
+            const int r = row < rows ? row : 0;
+            const uint16_t* src = p.q + int64_t(list[r / G]) * p.q_seq + int64_t(head * G + r % G) * p.q_head + 8 * hf;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) qb[ks] = *reinterpret_cast<const uint4v*>(src + 16 * ks);
+        }
+
+        // pages of this thread's tokens in a tile; -1: none of the cache
+        auto page_of = [&](int tile, int token) {
+            const int b = (tile * TT + token) >> p.page_log2;
+            const int block = b < blocks ? table[b] : -1;
+            return uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
+        };
+        int page0, page1 = -1;
+        auto look_up = [&](int tile) {
+            if (brings_values) {
+                page0 = page_of(tile, vtoken);
+                page1 = page_of(tile, vtoken + 8);
+            } else {
+                page0 = page_of(tile, krow);
+            }
+        };
+        constexpr int NW = F8 ? 4 : 8;                     // 16-byte words of a thread's part of a tile
+        uint4v part[NW];
+        uint32_t scales[2];
+        int got0, got1;                                    // the pages that `part` is of
+        auto load = [&](int tile) {
+            got0 = page0;
+            got1 = page1;
+            if (brings_values) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int block = h ? got1 : got0, b = block < 0 ? 0 : block, t = (tile * TT + vtoken + 8 * h) & page_mask;
+                    const Elem* src = vbase + int64_t(b) * p.v_block + int64_t(t) * p.v_token;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (F8) {
+                            const uint2v v = *reinterpret_cast<const uint2v*>(src);
+                            part[2 * h + i / 2][2 * (i & 1)] = v.x;
+                            part[2 * h + i / 2][2 * (i & 1) + 1] = v.y;
+                        } else {
+                            part[4 * h + i] = *reinterpret_cast<const uint4v*>(src);
+                        }
+                        src += p.v_token;
+                    }
+                    if constexpr (F8) scales[h] = *reinterpret_cast<const uint32_t*>(p.vs + head * p.vs_head + int64_t(b) * p.vs_block + t);
+                }
+            } else {
+                const int b = got0 < 0 ? 0 : got0, t = (tile * TT + krow) & page_mask;
+                const Elem* src = kbase + int64_t(b) * p.k_block + int64_t(t) * p.k_token;
+#pragma unroll
+                for (int i = 0; i < KR; ++i) {
+                    part[i] = *reinterpret_cast<const uint4v*>(src);
+                    src += p.k_token;
+                }
+                if constexpr (F8) scales[0] = *reinterpret_cast<const uint32_t*>(p.ks + head * p.ks_head + int64_t(b) * p.ks_block + t);
+            }
+        };
+        auto keep = [&](int buffer) {                      // into LDS, as the products read them
+            if (brings_values) {
+                uint32_t word[8][4];                       // a token's eight coordinates
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                    const bool there = (t < 4 ? got0 : got1) >= 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (F8) {
+                            const uint32_t codes = part[t / 2][2 * (t & 1) + i / 2];
+                            const uint32_t bits = scales[t >> 2];
+                            const float up = (t & 3) == 0 ? row_scale<0>(bits) : (t & 3) == 1 ? row_scale<1>(bits) : (t & 3) == 2 ? row_scale<2>(bits) : row_scale<3>(bits);
+                            word[t][i] = i & 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, true))
+                                               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, false));
+                        } else {
+                            word[t][i] = part[t][i];
+                        }
+                        word[t][i] = there ? word[t][i] : 0u;
+                    }
+                }
+                uint8_t* dst = lv + buffer * C::SIDE + ((vgroup >> 1) * NOB + (vc >> 2)) * 1024 + (vgroup & 1) * 512 + (vc & 3) * 128;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint4v o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[i] = __builtin_amdgcn_perm(word[2 * i + 1][c / 2], word[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                    *reinterpret_cast<uint4v*>(dst + 16 * (c ^ (vc & 7))) = o;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < KR; ++i) {
+                    const int r = krow + i, swizzle = key_swizzle<D>(r);
+                    uint8_t* dst = lk + buffer * C::SIDE + r * (2 * D);
+                    if constexpr (F8) {
+                        const uint4v c = part[i];
+                        *reinterpret_cast<uint4v*>(dst + 16 * ((2 * kpiece) ^ swizzle)) =
+                            uint4v{codes_pair<DT, false>(c.x), codes_pair<DT, true>(c.x), codes_pair<DT, false>(c.y), codes_pair<DT, true>(c.y)};
+                        *reinterpret_cast<uint4v*>(dst + 16 * ((2 * kpiece + 1) ^ swizzle)) =
+                            uint4v{codes_pair<DT, false>(c.z), codes_pair<DT, true>(c.z), codes_pair<DT, false>(c.w), codes_pair<DT, true>(c.w)};
+                    } else {
+                        *reinterpret_cast<uint4v*>(dst + 16 * (kpiece ^ swizzle)) = part[i];
+                    }
+                }
+                if (kpiece == 0) {
+                    if (krow % 8 == 0) lvalid[buffer * NG + krow / 8] = got0 >= 0 ? 1 : 0;
+                    if constexpr (F8)
+                        *reinterpret_cast<float4v*>(lscale + buffer * TT + krow) =
+                            float4v{row_scale<0>(scales[0]), row_scale<1>(scales[0]), row_scale<2>(scales[0]), row_scale<3>(scales[0])} * p.scale_log2;
+                }
+            }
+        };
+
+        float16v O[NOB];
+#pragma unroll
+        for (int ob = 0; ob < NOB; ++ob)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) O[ob][e] = 0.0f;
+        float m = -__builtin_inff(), l = 0.0f;
+        const uint8_t* kread = lk + m32 * (2 * D);
+        const int kswizzle = 16 * (hf ^ key_swizzle<D>(m32));
+        const int cr = coord_of_row(m32);
+        const uint8_t* vread[2];                           // of even and odd blocks of 32 coordinates
+#pragma unroll
+        for (int o = 0; o < 2; ++o) vread[o] = lv + 512 * hf + 16 * ((cr & 24) + ((cr & 7) ^ (4 * o + (cr >> 3))));
+
+        look_up(tile0);
+        load(tile0);
+        look_up(tile0 + 1);
+        for (int tile = tile0; tile < end; ++tile) {
+            const int buffer = (tile - tile0) & 1;
+            keep(buffer);
+            if (tile + 1 < end) {
+                load(tile + 1);
+                look_up(tile + 2);
+            }
+            __syncthreads();
+            if (live) {
+                const uint64_t valid = __ballot(lane < NG && lvalid[buffer * NG + (lane < NG ? lane : 0)] != 0);
+                float16v S[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    S[b] = float16v{};
+#pragma unroll
+                    for (int ks = 0; ks < NKS; ++ks)
+                        S[b] = wide_mfma<DT>(*reinterpret_cast<const uint4v*>(kread + buffer * C::SIDE + b * (64 * D) + ((32 * ks) ^ kswizzle)), qb[ks], S[b]);
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if constexpr (F8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4v c = *reinterpret_cast<const float4v*>(lscale + buffer * TT + 32 * b + 8 * i + 4 * hf);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) S[b][4 * i + e] *= c[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) S[b][e] *= p.scale_log2;
+                    }
+                }
+                if (valid != (uint64_t(1) << NG) - 1) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (((valid >> (4 * b + e / 4)) & 1) == 0) S[b][e] = -__builtin_inff();
+                }
+                float top = S[0][0];
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, S[b][e]);
+                top = max_xor32(top);
+                // The reference moves only where a score would lead it by more than 2^4: rarely.
+                const float higher = top > m + 4.0f ? top : m;
+                if (__any(higher != m)) {
+                    const float shrink = m == higher ? 1.0f : __builtin_amdgcn_exp2f(m - higher);
+                    l *= shrink;
+#pragma unroll
+                    for (int ob = 0; ob < NOB; ++ob)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) O[ob][e] *= shrink;
+                    m = higher;
+                }
+                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<PT>;
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    uint4v hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float a = __builtin_amdgcn_exp2f(S[u / 2][8 * (u & 1) + 2 * i] - ref);
+                        const float b = __builtin_amdgcn_exp2f(S[u / 2][8 * (u & 1) + 2 * i + 1] - ref);
+                        sum += a + b;
+                        hi[i] = round_pair<PT>(a, b);
+                        if constexpr (TWO_TERMS) lo[i] = round_pair<PT>(a - low_value<PT>(hi[i]), b - high_value<PT>(hi[i]));
+                    }
+#pragma unroll
+                    for (int ob = 0; ob < NOB; ++ob) {
+                        const uint4v v = *reinterpret_cast<const uint4v*>(vread[ob & 1] + buffer * C::SIDE + (u * NOB + ob) * 1024);
+                        O[ob] = wide_mfma<PT>(v, hi, O[ob]);
+                        if constexpr (TWO_TERMS) O[ob] = wide_mfma<PT>(v, lo, O[ob]);
+                    }
+                }
+                l += sum;
+            }
+        }
+        l = sum_xor32(l);
+        if (row < rows) {
+            const int64_t at = pp.first_row + (int64_t(piece) * p.H_KV + head) * kPrefixRows + row;
+#pragma unroll
+            for (int ob = 0; ob < NOB; ++ob)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4v*>(p.part_o + at * D + 32 * ob + 16 * (e / 8) + 8 * hf + e % 8) =
+                        float4v{O[ob][e], O[ob][e + 1], O[ob][e + 2], O[ob][e + 3]};
+            if (hf == 0) {
+                p.part_m[at] = m;
+                p.part_l[at] = l;
+            }
+        }
+        left -= here;
+        if (left <= 0) break;
+        // the next group of rows
+        ++piece;
+        tile0 = 0;
+        if (++group == groups) {
+            group = 0;
+            do ++prefix;
+            while (prefix < p.num_prefixes && count[prefix] == 0);
+            if (prefix == p.num_prefixes) break;           // (not reached: the shares end with the last tile)
+        }
+    }
+}
+
+// Joins the pieces of a sequence, of its own tokens and of its prefix.  A workgroup takes 4 Q neighbouring values of the G rows of one
+// sequence and KV head, 256 / Q pieces at a time, each thread with a maximum and a sum of its own.
+template <int D, int DT, int PT, int Q>
+__global__ __launch_bounds__(256) void paged_prefix_join_kernel(const PrefixParams pp) {
+    constexpr int R = 256 / Q;
+    const KvDecodeParams& p = pp.kv;
+    __shared__ __align__(16) float4v rows[R][Q];
+    __shared__ float2v sums[R][Q];
+    const int columns = p.G * D / (4 * Q);
+    const int64_t unit = blockIdx.x / columns;                           // sequence and KV head
+    const int seq = int(unit / p.H_KV), head = int(unit - int64_t(seq) * p.H_KV);
+    const int c = 4 * (int(blockIdx.x % columns) * Q + threadIdx.x % Q), r0 = threadIdx.x / Q, h = c / D;
+    const int len = kv_length(p, seq), shared = kv_shared(p, seq, len);
+    const int2 own = len > shared ? p.place[seq] : int2{0, 0};           // (of sequences without tokens nothing is written)
+    const int4 before = shared > 0 ? pp.place[seq] : int4{0, 0, 0, 0};
+    const int pieces = own.y + before.y;
+    auto row_of = [&](int i) {
+        return i < own.y ? (int64_t(own.x + seq + i) * p.H_KV + head) * p.G + h
+                         : pp.first_row + (int64_t(before.x + i - own.y) * p.H_KV + head) * kPrefixRows + before.z + h;
+    };
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    float top = -__builtin_inff(), sum = 0.0f;
+    auto take = [&](float4v v, float m, float l) {
+        const float higher = __builtin_fmaxf(top, m);
+        const float a = piece_weight(top, sum, higher), b = piece_weight(m, l, higher);
+        o = o * a + v * b;
+        sum = sum * a + l * b;
+        top = higher;
+    };
+    const int in_row = c - h * D;
+    for (int i = r0; i < pieces; i += 4 * R) {                           // four pieces a trip
+        float4v v[4];
+        float m[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t row = row_of(i + k * R < pieces ? i + k * R : i);
+            v[k] = *reinterpret_cast<const float4v*>(p.part_o + row * D + in_row);
+            m[k] = p.part_m[row];
+            l[k] = p.part_l[row];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * R < pieces) take(v[k], m[k], l[k]);
+    }
+    const int q = threadIdx.x % Q;
+    sums[r0][q] = float2v{top, sum};
+    __syncthreads();
+    float highest = -__builtin_inff(), den = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) highest = __builtin_fmaxf(highest, sums[r][q].x);
+#pragma unroll
+    for (int r = 0; r < R; ++r) den += sums[r][q].y * piece_weight(sums[r][q].x, sums[r][q].y, highest);
+    rows[r0][q] = o * piece_weight(top, sum, highest);
+    __syncthreads();
+    if (threadIdx.x < Q) {
+        float4v all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < R; ++r) all += rows[r][q];
+        const float inv = inverse_sum(den);
+        const int64_t out = unit * p.G;
+        *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(all.x * inv, all.y * inv), round_pair<DT>(all.z * inv, all.w * inv)};
+        if (in_row == 0 && p.lse != nullptr)
+            p.lse[out + h] = den == 0.0f ? -__builtin_inff() : (highest - kKvLift<PT> + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
+    }
+}
+
+}  // namespace fq
+
+namespace {
+
+// How a call is divided: the sequences' own tokens as in a decode that is cut into shares, the prefixes' tiles into equal shares.
+struct PrefixPlan {
+    KvPlan own;
+    int shares, min_tiles, members, most_pieces;
+};
+PrefixPlan prefix_plan(int S, int H_KV, int G, int D, int num_prefixes) {
+    const int64_t cus = fq_host::device_cu_count();
+    PrefixPlan r;
+    const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
+    r.own = {int((cus * together + H_KV - 1) / H_KV), together, most / together};
+    r.shares = int(((D == 256 ? 1 : 2) * cus + H_KV - 1) / H_KV);
+    r.min_tiles = 2;
+    r.members = fq::kPrefixRows / G;
+    const int64_t groups = int64_t(S) / r.members + (num_prefixes < S ? num_prefixes : S);
+    r.most_pieces = r.shares + int(groups < S ? groups : S);
+    return r;
+}
+
+struct PrefixRoom {
+    size_t o, m, place, prefix_place, all;
+    int64_t first_row;
+};
+PrefixRoom prefix_room(const PrefixPlan& plan, int S, int H_Q, int H_KV, int D) {
+    PrefixRoom r;
+    r.first_row = (int64_t(S) + kv_most_shares(H_KV)) * H_Q;
+    const size_t rows = size_t(r.first_row) + size_t(plan.most_pieces) * size_t(H_KV) * fq::kPrefixRows;
+    r.o = round_up(rows * size_t(D) * 4);
+    r.m = round_up(rows * 4);
+    r.place = round_up(size_t(S) * sizeof(int2));
+    r.prefix_place = round_up(size_t(S) * sizeof(int4));
+    r.all = r.o + 2 * r.m + r.place + r.prefix_place;
+    return r;
+}
+
+template <int D, int DT, bool F8>
+int launch_prefix(const fq::PrefixParams& pp, const PrefixPlan& plan, hipStream_t s) {
+    constexpr int PT = F8 ? FQ_BF16 : DT;
+    auto kernel = fq::paged_prefix_kernel<D, DT, F8>;
+    constexpr size_t lds = fq::PrefixCfg<D>::LDS;
+    if (!fq_host::lds_limit_raised(reinterpret_cast<const void*>(kernel), lds)) return FQ_ERR_LAUNCH;
+    kernel<<<unsigned(plan.shares) * unsigned(pp.kv.H_KV), 256, lds, s>>>(pp);
+    const int st = launch_shares<D, DT, F8, true>(pp.kv, plan.own, s);
+    if (st != FQ_OK) return st;
+    const int64_t values = int64_t(pp.kv.S) * pp.kv.H_KV * pp.kv.G * D;
+    fq::paged_prefix_join_kernel<D, DT, PT, 16><<<unsigned(values / 64), 256, 0, s>>>(pp);
+    return fq_host::check_launch();
+}
+
+template <int D>
+int launch_prefix_type(const fq::PrefixParams& pp, const PrefixPlan& plan, bool f8, int dtype, hipStream_t s) {
+    if (dtype == FQ_BF16) return f8 ? launch_prefix<D, FQ_BF16, true>(pp, plan, s) : launch_prefix<D, FQ_BF16, false>(pp, plan, s);
+    return f8 ? launch_prefix<D, FQ_F16, true>(pp, plan, s) : launch_prefix<D, FQ_F16, false>(pp, plan, s);
+}
+
+}  // namespace
+
+extern "C" size_t fq_paged_prefix_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int num_prefixes) {
+    if (check_kv_shape(num_seqs, H_Q, H_KV, D, 16, 1, 1) != FQ_OK || num_seqs == 0 || num_prefixes < 0 || num_prefixes > fq::kPrefixMost) return 0;
+    return prefix_room(prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes), num_seqs, H_Q, H_KV, D).all;
+}
+
+extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
+                                      const void* value_cache, const int64_t* value_strides, const uint8_t* key_scales,
+                                      const int64_t* key_scale_strides, const uint8_t* value_scales, const int64_t* value_scale_strides,
+                                      const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens,
+                                      const int32_t* prefix_ids, const int32_t* prefix_lens, int num_prefixes, void* out, float* lse,
+                                      int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                                      float sm_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const int bad = check_kv_shape(num_seqs, H_Q, H_KV, D, block_size, max_blocks_per_seq, num_blocks);
+    if (bad != FQ_OK) return bad;
+    if (dtype != FQ_F16 && dtype != FQ_BF16) return FQ_ERR_UNSUPPORTED_DTYPE;
+    if (block_table_stride < 0 || num_prefixes < 0 || num_prefixes > fq::kPrefixMost) return FQ_ERR_BAD_SHAPE;
+    if (num_seqs == 0) return FQ_OK;
+    const bool f8 = key_scales != nullptr || value_scales != nullptr;
+    if (!q || !q_strides || !key_cache || !key_strides || !value_cache || !value_strides || !block_table || !seq_lens || !prefix_ids || !out ||
+        (num_prefixes > 0 && !prefix_lens) || !workspace ||
+        (f8 && (!key_scales || !key_scale_strides || !value_scales || !value_scale_strides)))
+        return FQ_ERR_NULL_POINTER;
+    const int unit = f8 ? 16 : 8;
+    for (int i = 0; i < 3; ++i)
+        if (key_strides[i] % unit != 0 || value_strides[i] % unit != 0 || (i < 2 && q_strides[i] % 8 != 0)) return FQ_ERR_MISALIGNED;
+    if (!fq_host::aligned(q, 16) || !fq_host::aligned(key_cache, 16) || !fq_host::aligned(value_cache, 16) || !fq_host::aligned(out, 16) ||
+        (f8 && !(codes_aligned(key_cache, key_strides, key_scales, key_scale_strides) &&
+                 codes_aligned(value_cache, value_strides, value_scales, value_scale_strides))))
+        return FQ_ERR_MISALIGNED;
+    const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes);
+    const PrefixRoom room = prefix_room(plan, num_seqs, H_Q, H_KV, D);
+    if (room.o / (size_t(D) * 4) * size_t(D / 32) > size_t(0x7fffffff)) return FQ_ERR_BAD_SHAPE;
+    if (workspace_bytes < room.all) return FQ_ERR_WORKSPACE;
+    if (!fq_host::aligned(workspace, 256)) return FQ_ERR_MISALIGNED;
+    fq::PrefixParams pp = {};
+    fq::KvDecodeParams& p = pp.kv;
+    set_up_params(p, q, q_strides, block_table, block_table_stride, seq_lens, out, lse, num_seqs, H_Q, H_KV, block_size, max_blocks_per_seq,
+                  num_blocks, sm_scale, 0, plan.own);
+    char* ws = static_cast<char*>(workspace);
+    p.part_o = reinterpret_cast<float*>(ws);
+    p.part_m = reinterpret_cast<float*>(ws + room.o);
+    p.part_l = reinterpret_cast<float*>(ws + room.o + room.m);
+    p.place = reinterpret_cast<int2*>(ws + room.o + 2 * room.m);
+    pp.place = reinterpret_cast<int4*>(ws + room.o + 2 * room.m + room.place);
+    p.prefix_ids = prefix_ids;
+    p.prefix_lens = prefix_lens;
+    p.num_prefixes = num_prefixes;
+    pp.first_row = room.first_row;
+    pp.shares = plan.shares;
+    pp.min_tiles = plan.min_tiles;
+    pp.members = plan.members;
+    if (f8) {
+        set_codes(p, static_cast<const uint8_t*>(key_cache), key_strides, static_cast<const uint8_t*>(value_cache), value_strides, key_scales,
+                  key_scale_strides, value_scales, value_scale_strides);
+    } else {
+        set_rows(p, key_cache, key_strides, value_cache, value_strides);
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (D) {
+        case 64: return launch_prefix_type<64>(pp, plan, f8, dtype, s);
+        case 128: return launch_prefix_type<128>(pp, plan, f8, dtype, s);
+        default: return launch_prefix_type<256>(pp, plan, f8, dtype, s);
+    }
+}

@@ -749,6 +749,27 @@ int fq_paged_kv8_decode(const void* q, const int64_t* q_strides, const uint8_t* 
                         int num_seqs, int H_Q, int H_KV, int D, int block_size, int max_blocks_per_seq, int64_t num_blocks,
                         float sm_scale, int window, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * fq_paged_prefix_decode: fq_paged_kv_decode (scales NULL) or fq_paged_kv8_decode (with scales) for sequences that begin with the same
+ *   pages: those are read once for all of them, and the result is that of these entries up to rounding.
+ *   prefix_ids     (num_seqs,) int32: the prefix of a sequence; outside [0, num_prefixes): none
+ *   prefix_lens    (num_prefixes,) int32 tokens, of which whole pages are taken.  Of the sequences of one prefix whose length is at
+ *                  least that, the rows of block_table begin with the same pages (one of the rows is read for all); a shorter one
+ *                  is attended to by itself.  num_prefixes <= 1024
+ *   workspace      fq_paged_prefix_decode_workspace_bytes bytes (does not shrink with num_seqs or num_prefixes), 256-byte aligned, any
+ *                  contents
+ * No window.  Weights over shared tokens keep 11 bits (fp16 pages), 8 (bf16) or, with scales, 8 and for fp16 queries 16; over a
+ * sequence's own as in the decodes.  Maxima and sums are 32-bit.
+ */
+size_t fq_paged_prefix_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int num_prefixes);
+int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
+                           const void* value_cache, const int64_t* value_strides, const uint8_t* key_scales,
+                           const int64_t* key_scale_strides, const uint8_t* value_scales, const int64_t* value_scale_strides,
+                           const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens, const int32_t* prefix_ids,
+                           const int32_t* prefix_lens, int num_prefixes, void* out, float* lse, int num_seqs, int H_Q, int H_KV, int D,
+                           int block_size, int max_blocks_per_seq, int64_t num_blocks, float sm_scale, int dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
