@@ -233,7 +233,7 @@ __device__ __forceinline__ float scale_of(const uint2v& w, int k) {
 // HW heads of a workgroup, TW wavefronts of each; SHARED: a share of all tiles, else one sequence.  F8: rows of codes.  OWN (with
 // SHARED): the tokens behind a shared prefix, left as partial results.
 template <int D, int DT, bool F8, int HW, int TW, bool SHARED, bool OWN>
-__global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const KvDecodeParams p) {
+__device__ __forceinline__ void kv_decode_workgroup(const KvDecodeParams& p, int workgroup, float* lds) {
     using Elem = std::conditional_t<F8, uint8_t, uint16_t>;
     constexpr int PT = F8 ? FQ_BF16 : DT;            // of weights and values in the second product
     constexpr bool LINES = !F8 || D >= 128;          // a key is lines of 128 bytes (of 64 codes: half a line)
@@ -245,12 +245,12 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
     constexpr int VE = (F8 ? 4 : 2) * VW;            // its coordinates
     constexpr int W = HW * TW;
     static_assert(SHARED || !OWN);
-    extern __shared__ __align__(16) float lds[];     // (W, G, D), then (W, 2, 16), then (HW, 16)
+    // lds: (W, G, D), then (W, 2, 16), then (HW, 16)
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n = lane & 15, g = lane >> 4, kgroup = (n >> 2) & 1;
     const int G = p.G;
     const int groups = p.H_KV / HW;                  // of HW neighbouring heads
-    const int x = blockIdx.x / groups, head = (blockIdx.x - x * groups) * HW + wave % HW, turn = wave / HW;
+    const int x = workgroup / groups, head = (workgroup - x * groups) * HW + wave % HW, turn = wave / HW;
 
     const Elem* kbase = static_cast<const Elem*>(p.kc) + head * p.k_head + EL * (LINES ? g + 4 * (n >> 3) : g) + int64_t(n & 3) * p.k_token;
     const Elem* vbase = static_cast<const Elem*>(p.vc) + head * p.v_head + VE * n;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
         }
 
         const bool complete = !OWN && (!SHARED || count == span.tiles);
-        if (SHARED && offset == 0 && threadIdx.x == 0 && int(blockIdx.x) == x * groups)
+        if (SHARED && offset == 0 && threadIdx.x == 0 && workgroup == x * groups)
             p.place[seq] = int2{x, 1 + (span.tiles - count + at.size - 1) / at.size};
         const int64_t row = (int64_t(x + seq) * p.H_KV + head) * G;      // of the partial results
         const int64_t orow = (int64_t(seq) * p.H_KV + head) * G;         // of the outputs
@@ -636,6 +636,12 @@ __global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const 
             }
         }
     } while (SHARED && left > 0 && seq < p.S);
+}
+
+template <int D, int DT, bool F8, int HW, int TW, bool SHARED>
+__global__ __launch_bounds__(HW * TW * kWave) void paged_kv_decode_kernel(const KvDecodeParams p) {
+    extern __shared__ __align__(16) float kv_lds[];
+    kv_decode_workgroup<D, DT, F8, HW, TW, SHARED, false>(p, int(blockIdx.x), kv_lds);
 }
 
 // Joins the pieces of the sequences that several shares hold, and writes the rows of those that have no tokens.  A workgroup
@@ -790,23 +796,13 @@ KvRoom kv_room(int S, int H_Q, int D, int shares) {
     return r;
 }
 
-template <int D, int DT, bool F8, int HW, int TW, bool SHARED, bool OWN = false>
+template <int D, int DT, bool F8, int HW, int TW, bool SHARED>
 int launch_attend(const fq::KvDecodeParams& p, hipStream_t s) {
     const size_t lds = TW == 1 ? 0 : (size_t(HW * TW) * p.G * D + HW * TW * 32 + HW * 16) * 4;
-    auto kernel = fq::paged_kv_decode_kernel<D, DT, F8, HW, TW, SHARED, OWN>;
+    auto kernel = fq::paged_kv_decode_kernel<D, DT, F8, HW, TW, SHARED>;
     if (lds > 32768 && !fq_host::lds_limit_raised(reinterpret_cast<const void*>(kernel), lds)) return FQ_ERR_LAUNCH;
     kernel<<<unsigned(SHARED ? p.shares : p.S) * unsigned(p.H_KV / HW), HW * TW * 64, lds, s>>>(p);
     return FQ_OK;
-}
-
-// the shares of a plan
-template <int D, int DT, bool F8, bool OWN>
-int launch_shares(const fq::KvDecodeParams& p, const KvPlan& plan, hipStream_t s) {
-    constexpr int W = D == 256 ? 4 : 8;
-    if (plan.heads == 4) return launch_attend<D, DT, F8, 4, W / 4, true, OWN>(p, s);
-    if (plan.heads == 2)
-        return plan.waves == W / 2 ? launch_attend<D, DT, F8, 2, W / 2, true, OWN>(p, s) : launch_attend<D, DT, F8, 2, 2, true, OWN>(p, s);
-    return plan.waves == W ? launch_attend<D, DT, F8, 1, W, true, OWN>(p, s) : launch_attend<D, DT, F8, 1, 4, true, OWN>(p, s);
 }
 
 template <int D, int DT, bool F8>
@@ -814,7 +810,9 @@ int launch_kv(const fq::KvDecodeParams& p, const KvPlan& plan, hipStream_t s) {
     constexpr int W = D == 256 ? 4 : 8, PT = F8 ? FQ_BF16 : DT;
     int st;
     if (plan.shares > 0) {
-        st = launch_shares<D, DT, F8, false>(p, plan, s);
+        if (plan.heads == 4) st = launch_attend<D, DT, F8, 4, W / 4, true>(p, s);
+        else if (plan.heads == 2) st = plan.waves == W / 2 ? launch_attend<D, DT, F8, 2, W / 2, true>(p, s) : launch_attend<D, DT, F8, 2, 2, true>(p, s);
+        else st = plan.waves == W ? launch_attend<D, DT, F8, 1, W, true>(p, s) : launch_attend<D, DT, F8, 1, 4, true>(p, s);
         if (st != FQ_OK) return st;
         // as many values a workgroup as leave enough workgroups
         const int64_t values = int64_t(p.S) * p.H_KV * p.G * D;

@@ -19,12 +19,14 @@ struct PrefixParams {
 
 constexpr int kPrefixRows = 128;
 constexpr int kPrefixMost = 1024;         // prefixes of a call
+constexpr int kPrefixSeqs = 1024;         // sequences whose prefixes are kept in LDS (the others' are read again)
 
 template <int D> struct PrefixCfg {
     static constexpr int TT = 8192 / D;                    // tokens of a tile
     static constexpr int NB = TT / 32, NKS = D / 16, NOB = D / 32, NU = TT / 16, NG = TT / 8;
+    template <bool F8> static constexpr int depth() { return F8 ? 2 : 1; }   // tiles that are on their way
     static constexpr int SIDE = TT * D * 2;                // bytes of a tile's keys or values: 16 KB
-    static constexpr int LDS = 4 * SIDE + 2 * TT * 4 + 2 * NG * 4 + kPrefixRows * 4 + 2 * kPrefixMost * 4;
+    static constexpr int LDS = 4 * SIDE + 2 * TT * 4 + 2 * NG * 4 + kPrefixRows * 4 + 2 * kPrefixMost * 4 + kPrefixSeqs * 2;
 };
 
 // Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
@@ -40,121 +42,118 @@ template <int DT> __device__ __forceinline__ float16v wide_mfma(uint4v a, uint4v
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d, kWave);
-    return v;
-}
-__device__ __forceinline__ int64_t wave_scan64(int64_t v, int lane) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int64_t u = __shfl_up(v, d, kWave);
-        if (lane >= d) v += u;
-    }
-    return v;
-}
-
 // The members of a prefix, 128 rows (member, query head of the KV head) of them a workgroup, against a share of its keys.
 template <int D, int DT, bool F8>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(const PrefixParams pp) {
+__device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int workgroup, uint8_t* lds) {
     using C = PrefixCfg<D>;
     using Elem = std::conditional_t<F8, uint8_t, uint16_t>;
     constexpr int TT = C::TT, NB = C::NB, NKS = C::NKS, NOB = C::NOB, NU = C::NU, NG = C::NG;
     constexpr int PT = F8 ? FQ_BF16 : DT;                  // of weights and values in the second product
     constexpr bool TWO_TERMS = F8 && DT == FQ_F16;         // one bf16 term would show in an fp16 result
-    constexpr int KR = F8 ? 4 : 8;                         // keys of a thread's piece of a tile
+    constexpr bool TABLE = F8 && DT == FQ_F16;             // keys as fp16 codes, their powers applied to the scores (as bf16 they are in the keys)
+    constexpr int kDepth = PrefixCfg<D>::template depth<F8>();
     const KvDecodeParams& p = pp.kv;
-    extern __shared__ __attribute__((aligned(256))) uint8_t prefix_lds[];
-    uint8_t* lds = prefix_lds;
     uint8_t *lk = lds, *lv = lds + 2 * C::SIDE;
     float* lscale = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, TT): what a key's score is multiplied by
     int* lvalid = reinterpret_cast<int*>(lscale + 2 * TT);                // (2, NG): whether eight keys are on a page of the cache
     int* list = lvalid + 2 * NG;                                          // the sequences of the rows
     const int tid = threadIdx.x, lane = tid & 63, m32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int head = blockIdx.x % p.H_KV, x = blockIdx.x / p.H_KV, G = p.G;
+    const int head = workgroup % p.H_KV, x = workgroup / p.H_KV, G = p.G;
 
     // ---- the share: members of every prefix, tiles of all, where this one begins -----------------------------------------------
+    // (all lengths and ids are asked for at once; what the sequences share is kept in LDS for the lists of members)
     int* count = list + kPrefixRows;
     int* shared_len = count + kPrefixMost;
+    int16_t* shares_of = reinterpret_cast<int16_t*>(shared_len + kPrefixMost);
+    constexpr int kAhead = 4;
+    int ids[kAhead], lens[kAhead];
+    auto ask = [&](int s0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int s = s0 + 256 * j + tid;
+            ids[j] = -1;
+            lens[j] = 0;
+            if (s < p.S) {
+                ids[j] = p.prefix_ids[s];
+                lens[j] = p.lens[s];
+            }
+        }
+    };
+    ask(0);
     for (int i = tid; i < p.num_prefixes; i += 256) {
         count[i] = 0;
         const int n = p.prefix_lens[i] >> p.page_log2 << p.page_log2;
         shared_len[i] = n > 0 ? n : 0;
     }
     __syncthreads();
-    auto member_of = [&](int s) {                          // the prefix that sequence s shares, or -1
-        const int id = p.prefix_ids[s], len = kv_length(p, s);
+    const int64_t room = int64_t(p.max_blocks) << p.page_log2;
+    auto prefix_of = [&](int id, int len) {                // that a sequence shares, or -1
         if (uint32_t(id) >= uint32_t(p.num_prefixes)) return -1;
         const int n = shared_len[id];
-        return n > 0 && n <= len ? id : -1;
+        return n > 0 && n <= (len > room ? room : int64_t(len)) ? id : -1;
     };
-    for (int s = tid; s < p.S; s += 256) {
-        const int id = member_of(s);
-        if (id >= 0) atomicAdd(&count[id], 1);
+    for (int s0 = 0; s0 < p.S; s0 += 256 * kAhead) {
+        if (s0 > 0) ask(s0);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int s = s0 + 256 * j + tid, id = prefix_of(ids[j], lens[j]);
+            if (s < kPrefixSeqs && s < p.S) shares_of[s] = int16_t(id);
+            if (id >= 0) atomicAdd(&count[id], 1);
+        }
     }
     __syncthreads();
     auto tiles_of = [&](int i) { return (shared_len[i] + TT - 1) / TT; };
-    auto groups_of = [&](int i) { return (count[i] + pp.members - 1) / pp.members; };
-    int64_t total = 0;
-    for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) {
-        const int i = i0 + lane;
-        total += wave_sum64(i < p.num_prefixes ? int64_t(tiles_of(i)) * groups_of(i) : 0);
-    }
-    int64_t size = (total + pp.shares - 1) / pp.shares;
+    auto groups_of = [&](int i) { return int(uint32_t(count[i] + pp.members - 1) / uint32_t(pp.members)); };
+    auto units_of = [&](int i) { return i < p.num_prefixes ? tiles_of(i) * groups_of(i) : 0; };      // (the host bounds their sum)
+    uint32_t total = 0;
+    for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) total += wave_sum(uint32_t(units_of(i0 + lane)));
+    int size = int((total + uint32_t(pp.shares) - 1) / uint32_t(pp.shares));
     if (size < pp.min_tiles) size = pp.min_tiles;
-    const int64_t wanted = int64_t(x) * size;
-    if (wanted >= total) return;
-    int64_t left = total - wanted < size ? total - wanted : size;
+    if (int64_t(x) * size >= int64_t(total)) return;
+    const int wanted = x * size;
+    int left = int(total) - wanted < size ? int(total) - wanted : size;
     int prefix = 0, group = 0, tile0 = 0, piece = x;       // piece: the share and the groups of rows before this one
-    {
-        int64_t before = 0;
-        for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) {
-            const int i = i0 + lane;
-            const int gs = i < p.num_prefixes && shared_len[i] > 0 ? groups_of(i) : 0;
-            const int64_t units = i < p.num_prefixes ? int64_t(tiles_of(i)) * gs : 0, upto = before + wave_scan64(units, lane);
-            const uint64_t past = __ballot(upto > wanted);
-            const int groups_upto = sum_upto(gs);
-            if (past != 0) {
-                const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-                prefix = i0 + at;
-                const int64_t inside = wanted - (__shfl(upto, at, kWave) - __shfl(units, at, kWave));
-                const int tiles = tiles_of(prefix);
-                group = int(inside / tiles);
-                tile0 = int(inside - int64_t(group) * tiles);
-                piece += __builtin_amdgcn_readlane(groups_upto, at) - __builtin_amdgcn_readlane(gs, at) + group;
-                break;
-            }
-            piece += __builtin_amdgcn_readlane(groups_upto, kWave - 1);
-            before = __shfl(upto, kWave - 1, kWave);
+    for (int i0 = 0, before = 0; i0 < p.num_prefixes; i0 += kWave) {
+        const int units = units_of(i0 + lane), gs = units > 0 ? groups_of(i0 + lane) : 0;
+        const int upto = before + sum_upto(units), groups_upto = sum_upto(gs);
+        const uint64_t past = __ballot(upto > wanted);
+        if (past != 0) {
+            const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            prefix = i0 + at;
+            const int inside = wanted - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(units, at));
+            const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(prefix));
+            group = inside / tiles;
+            tile0 = inside - group * tiles;
+            piece += __builtin_amdgcn_readlane(groups_upto, at) - __builtin_amdgcn_readlane(gs, at) + group;
+            break;
         }
+        piece += __builtin_amdgcn_readlane(groups_upto, kWave - 1);
+        before = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
-    prefix = __builtin_amdgcn_readfirstlane(prefix);
-    group = __builtin_amdgcn_readfirstlane(group);
-    tile0 = __builtin_amdgcn_readfirstlane(tile0);
-    piece = __builtin_amdgcn_readfirstlane(piece);
 
-    // ---- what this thread brings of a tile: the first half of them values, eight tokens of eight coordinates in the order of the
-    // scores' registers; the others keys -----------------------------------------------------------------------------------------
-    const bool brings_values = tid < 128;
-    const int item = tid & 127;
-    const int vgroup = item / (D / 8), vc = item % (D / 8);                              // tokens 16 (vgroup / 2) + 4 (vgroup % 2) + 0 .. 3, + 8
-    const int kpiece = F8 ? item % (D / 16) : item % (D / 8), krow = KR * (F8 ? item / (D / 16) : item / (D / 8));
+    // ---- what this thread brings of a tile: eight coordinates of eight tokens; the first two wavefronts values, in the order of the
+    // scores' registers, the others keys -----------------------------------------------------------------------------------------
+    const bool brings_values = w < 2;
+    const int item = tid & 127, igroup = item / (D / 8), ic = item % (D / 8);
+    const int token0 = brings_values ? 16 * (igroup >> 1) + 4 * (igroup & 1) : 8 * igroup, token1 = token0 + (brings_values ? 8 : 4);    // four from each
     const int page_mask = (1 << p.page_log2) - 1;
-    const int vtoken = 16 * (vgroup >> 1) + 4 * (vgroup & 1);
-    const Elem* kbase = static_cast<const Elem*>(p.kc) + head * p.k_head + (F8 ? 16 : 8) * kpiece;
-    const Elem* vbase = static_cast<const Elem*>(p.vc) + head * p.v_head + 8 * vc;
+    const Elem* base = static_cast<const Elem*>(brings_values ? p.vc : p.kc) + head * (brings_values ? p.v_head : p.k_head) + 8 * ic;
+    const int64_t block_step = brings_values ? p.v_block : p.k_block, token_step = brings_values ? p.v_token : p.k_token;
+    const uint8_t* scale_base = F8 ? (brings_values ? p.vs + head * p.vs_head : p.ks + head * p.ks_head) : nullptr;
+    const int64_t scale_block = brings_values ? p.vs_block : p.ks_block;
 
     for (;;) {
-        const int n_members = count[prefix], shared = shared_len[prefix], tiles = tiles_of(prefix), groups = groups_of(prefix);
-        const int here = left < tiles - tile0 ? int(left) : tiles - tile0, end = tile0 + here;
+        const int n_members = __builtin_amdgcn_readfirstlane(count[prefix]), shared = __builtin_amdgcn_readfirstlane(shared_len[prefix]);
+        const int tiles = (shared + TT - 1) / TT, groups = int(uint32_t(n_members + pp.members - 1) / uint32_t(pp.members));
+        const int here = left < tiles - tile0 ? left : tiles - tile0, end = tile0 + here;
         // the group's members, in the order of the sequences
         if (w == 0) {
             int rank = 0;
             const int first = group * pp.members;
             for (int s0 = 0; s0 < p.S && rank < first + pp.members; s0 += kWave) {
                 const int s = s0 + lane;
-                const bool mine = s < p.S && member_of(s) == prefix;
+                const bool mine = s < p.S && (s < kPrefixSeqs ? int(shares_of[s]) : prefix_of(p.prefix_ids[s], p.lens[s])) == prefix;
                 const uint64_t all = __ballot(mine);
                 const int at = rank + __popcll(all & ((uint64_t(1) << lane) - 1)) - first;
                 if (mine && at >= 0 && at < pp.members) list[at] = s;
@@ -165,7 +164,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(con
         const int members = n_members - group * pp.members < pp.members ? n_members - group * pp.members : pp.members;
         const int rows = members * G, blocks = shared >> p.page_log2;
         const int32_t* table = p.table + int64_t(list[0]) * p.table_row;
-        if (tile0 == 0 && head == 0 && tid < members) pp.place[list[tid]] = int4{piece, int(1 + (tiles - here + size - 1) / size), tid * G, 0};
+        if (tile0 == 0 && head == 0 && tid < members) pp.place[list[tid]] = int4{piece, 1 + (tiles - here + size - 1) / size, tid * G, 0};
         const int row = 32 * w + m32;
         const bool live = 32 * w < rows;
         uint4v qb[NKS];
@@ -179,103 +178,96 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(con
         // pages of this thread's tokens in a tile; -1: none of the cache
         auto page_of = [&](int tile, int token) {
             const int b = (tile * TT + token) >> p.page_log2;
-            const int block = b < blocks ? table[b] : -1;
+            const int block = tile < end && b < blocks ? table[b] : -1;
             return uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
         };
-        int page0, page1 = -1;
+        int page0, page1;                                  // of the tile that is asked for next
         auto look_up = [&](int tile) {
-            if (brings_values) {
-                page0 = page_of(tile, vtoken);
-                page1 = page_of(tile, vtoken + 8);
-            } else {
-                page0 = page_of(tile, krow);
-            }
+            page0 = page_of(tile, token0);
+            page1 = page_of(tile, token1);
         };
-        constexpr int NW = F8 ? 4 : 8;                     // 16-byte words of a thread's part of a tile
-        uint4v part[NW];
-        uint32_t scales[2];
-        int got0, got1;                                    // the pages that `part` is of
-        auto load = [&](int tile) {
-            got0 = page0;
-            got1 = page1;
-            if (brings_values) {
+        constexpr int NW = F8 ? 2 : 4;                     // words of eight coordinates
+        struct Part {
+            uint32_t word[8][NW];
+            uint32_t scales[2];
+            int page0, page1;
+        };
+        Part parts[kDepth];
+        auto load = [&](Part& part, int tile) {            // (no branch round the loads, so that nothing waits for them here)
+            part.page0 = page0;
+            part.page1 = page1;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int block = h ? got1 : got0, b = block < 0 ? 0 : block, t = (tile * TT + vtoken + 8 * h) & page_mask;
-                    const Elem* src = vbase + int64_t(b) * p.v_block + int64_t(t) * p.v_token;
+            for (int h = 0; h < 2; ++h) {
+                const int block = h ? page1 : page0, b = block < 0 ? 0 : block, t = (tile * TT + (h ? token1 : token0)) & page_mask;
+                const Elem* src = base + int64_t(b) * block_step + int64_t(t) * token_step;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (F8) {
-                            const uint2v v = *reinterpret_cast<const uint2v*>(src);
-                            part[2 * h + i / 2][2 * (i & 1)] = v.x;
-                            part[2 * h + i / 2][2 * (i & 1) + 1] = v.y;
-                        } else {
-                            part[4 * h + i] = *reinterpret_cast<const uint4v*>(src);
-                        }
-                        src += p.v_token;
+                for (int i = 4 * h; i < 4 * h + 4; ++i) {
+                    if constexpr (F8) {
+                        const uint2v v = *reinterpret_cast<const uint2v*>(src);
+                        part.word[i][0] = v.x; part.word[i][1] = v.y;
+                    } else {
+                        const uint4v v = *reinterpret_cast<const uint4v*>(src);
+                        part.word[i][0] = v.x; part.word[i][1] = v.y; part.word[i][2] = v.z; part.word[i][3] = v.w;
                     }
-                    if constexpr (F8) scales[h] = *reinterpret_cast<const uint32_t*>(p.vs + head * p.vs_head + int64_t(b) * p.vs_block + t);
+                    src += token_step;
                 }
-            } else {
-                const int b = got0 < 0 ? 0 : got0, t = (tile * TT + krow) & page_mask;
-                const Elem* src = kbase + int64_t(b) * p.k_block + int64_t(t) * p.k_token;
-#pragma unroll
-                for (int i = 0; i < KR; ++i) {
-                    part[i] = *reinterpret_cast<const uint4v*>(src);
-                    src += p.k_token;
-                }
-                if constexpr (F8) scales[0] = *reinterpret_cast<const uint32_t*>(p.ks + head * p.ks_head + int64_t(b) * p.ks_block + t);
+                if constexpr (F8) part.scales[h] = *reinterpret_cast<const uint32_t*>(scale_base + int64_t(b) * scale_block + t);
             }
         };
-        auto keep = [&](int buffer) {                      // into LDS, as the products read them
-            if (brings_values) {
-                uint32_t word[8][4];                       // a token's eight coordinates
+        auto keep = [&](const Part& part, int buffer) {    // into LDS, as the products read them
+            uint32_t word[8][4];
+            if constexpr (F8) {
 #pragma unroll
                 for (int t = 0; t < 8; ++t) {
-                    const bool there = (t < 4 ? got0 : got1) >= 0;
+                    const uint32_t bits = part.scales[t >> 2];
+                    const float up = (t & 3) == 0 ? row_scale<0>(bits) : (t & 3) == 1 ? row_scale<1>(bits) : (t & 3) == 2 ? row_scale<2>(bits) : row_scale<3>(bits);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (F8) {
-                            const uint32_t codes = part[t / 2][2 * (t & 1) + i / 2];
-                            const uint32_t bits = scales[t >> 2];
-                            const float up = (t & 3) == 0 ? row_scale<0>(bits) : (t & 3) == 1 ? row_scale<1>(bits) : (t & 3) == 2 ? row_scale<2>(bits) : row_scale<3>(bits);
-                            word[t][i] = i & 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, true))
-                                               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, false));
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t codes = part.word[t][i];
+                        if (DT == FQ_BF16 || brings_values) {
+                            word[t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, false));
+                            word[t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, true));
                         } else {
-                            word[t][i] = part[t][i];
+                            word[t][2 * i] = codes_pair<FQ_F16, false>(codes);
+                            word[t][2 * i + 1] = codes_pair<FQ_F16, true>(codes);
                         }
-                        word[t][i] = there ? word[t][i] : 0u;
                     }
                 }
-                uint8_t* dst = lv + buffer * C::SIDE + ((vgroup >> 1) * NOB + (vc >> 2)) * 1024 + (vgroup & 1) * 512 + (vc & 3) * 128;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) word[t][i] = part.word[t][i % NW];
+            }
+            if (brings_values) {
+                if ((part.page0 | part.page1) < 0) {
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) word[t][i] = (t < 4 ? part.page0 : part.page1) < 0 ? 0u : word[t][i];
+                }
+                uint8_t* dst = lv + buffer * C::SIDE + ((igroup >> 1) * NOB + (ic >> 2)) * 1024 + (igroup & 1) * 512 + (ic & 3) * 128;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint4v o;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         o[i] = __builtin_amdgcn_perm(word[2 * i + 1][c / 2], word[2 * i][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-                    *reinterpret_cast<uint4v*>(dst + 16 * (c ^ (vc & 7))) = o;
+                    *reinterpret_cast<uint4v*>(dst + 16 * (c ^ (ic & 7))) = o;
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < KR; ++i) {
-                    const int r = krow + i, swizzle = key_swizzle<D>(r);
-                    uint8_t* dst = lk + buffer * C::SIDE + r * (2 * D);
-                    if constexpr (F8) {
-                        const uint4v c = part[i];
-                        *reinterpret_cast<uint4v*>(dst + 16 * ((2 * kpiece) ^ swizzle)) =
-                            uint4v{codes_pair<DT, false>(c.x), codes_pair<DT, true>(c.x), codes_pair<DT, false>(c.y), codes_pair<DT, true>(c.y)};
-                        *reinterpret_cast<uint4v*>(dst + 16 * ((2 * kpiece + 1) ^ swizzle)) =
-                            uint4v{codes_pair<DT, false>(c.z), codes_pair<DT, true>(c.z), codes_pair<DT, false>(c.w), codes_pair<DT, true>(c.w)};
-                    } else {
-                        *reinterpret_cast<uint4v*>(dst + 16 * (kpiece ^ swizzle)) = part[i];
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const int r = token0 + i;
+                    *reinterpret_cast<uint4v*>(lk + buffer * C::SIDE + r * (2 * D) + 16 * (ic ^ key_swizzle<D>(r))) = uint4v{word[i][0], word[i][1], word[i][2], word[i][3]};
                 }
-                if (kpiece == 0) {
-                    if (krow % 8 == 0) lvalid[buffer * NG + krow / 8] = got0 >= 0 ? 1 : 0;
-                    if constexpr (F8)
-                        *reinterpret_cast<float4v*>(lscale + buffer * TT + krow) =
-                            float4v{row_scale<0>(scales[0]), row_scale<1>(scales[0]), row_scale<2>(scales[0]), row_scale<3>(scales[0])} * p.scale_log2;
+                if (ic == 0) {
+                    lvalid[buffer * NG + igroup] = part.page0 >= 0 ? 1 : 0;
+                    if constexpr (TABLE)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            *reinterpret_cast<float4v*>(lscale + buffer * TT + token0 + 4 * h) =
+                                float4v{row_scale<0>(part.scales[h]), row_scale<1>(part.scales[h]), row_scale<2>(part.scales[h]), row_scale<3>(part.scales[h])} * p.scale_log2;
                 }
             }
         };
@@ -293,16 +285,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(con
 #pragma unroll
         for (int o = 0; o < 2; ++o) vread[o] = lv + 512 * hf + 16 * ((cr & 24) + ((cr & 7) ^ (4 * o + (cr >> 3))));
 
-        look_up(tile0);
-        load(tile0);
-        look_up(tile0 + 1);
-        for (int tile = tile0; tile < end; ++tile) {
-            const int buffer = (tile - tile0) & 1;
-            keep(buffer);
-            if (tile + 1 < end) {
-                load(tile + 1);
-                look_up(tile + 2);
-            }
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            look_up(tile0 + d);
+            load(parts[d], tile0 + d);
+        }
+        look_up(tile0 + kDepth);
+        int buffer = 0;
+        auto step = [&](int tile, Part& part) __attribute__((always_inline)) {
+            keep(part, buffer);
+            load(part, tile + kDepth);                     // (of tiles behind the last: some page's, not used)
+            look_up(tile + kDepth + 1);
             __syncthreads();
             if (live) {
                 const uint64_t valid = __ballot(lane < NG && lvalid[buffer * NG + (lane < NG ? lane : 0)] != 0);
@@ -316,7 +309,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(con
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    if constexpr (F8) {
+                    if constexpr (TABLE) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float4v c = *reinterpret_cast<const float4v*>(lscale + buffer * TT + 32 * b + 8 * i + 4 * hf);
@@ -374,6 +367,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(con
                 }
                 l += sum;
             }
+            buffer ^= 1;
+        };
+        for (int tile = tile0; tile < end; tile += kDepth) {
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d)
+                if (tile + d < end) step(tile + d, parts[d]);
         }
         l = sum_xor32(l);
         if (row < rows) {
@@ -401,6 +400,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(con
             if (prefix == p.num_prefixes) break;           // (not reached: the shares end with the last tile)
         }
     }
+}
+
+// The first workgroups take the prefixes, the others what the sequences have behind them: those wait for the matrix cores, these for
+// memory, so a CU has one of each.
+template <int D, int DT, bool F8, int HW>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(const PrefixParams pp) {
+    extern __shared__ __attribute__((aligned(256))) uint8_t prefix_lds[];
+    const int first = pp.shares * pp.kv.H_KV;
+    if (int(blockIdx.x) < first) prefix_workgroup<D, DT, F8>(pp, int(blockIdx.x), prefix_lds);
+    else kv_decode_workgroup<D, DT, F8, HW, 4 / HW, true, true>(pp.kv, int(blockIdx.x) - first, reinterpret_cast<float*>(prefix_lds));
 }
 
 // Joins the pieces of a sequence, of its own tokens and of its prefix.  A workgroup takes 4 Q neighbouring values of the G rows of one
@@ -481,9 +490,9 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(int S, int H_KV, int G, int D, int num_prefixes) {
     const int64_t cus = fq_host::device_cu_count();
     PrefixPlan r;
-    const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, most = D == 256 ? 4 : 8;
-    r.own = {int((cus * together + H_KV - 1) / H_KV), together, most / together};
-    r.shares = int(((D == 256 ? 1 : 2) * cus + H_KV - 1) / H_KV);
+    const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, each = D == 256 ? 1 : 2;       // workgroups that a CU has at a time
+    r.own = {int((each * cus * together + H_KV - 1) / H_KV), together, 4 / together};
+    r.shares = int((cus + H_KV - 1) / H_KV);
     r.min_tiles = 2;
     r.members = fq::kPrefixRows / G;
     const int64_t groups = int64_t(S) / r.members + (num_prefixes < S ? num_prefixes : S);
@@ -497,7 +506,7 @@ struct PrefixRoom {
 };
 PrefixRoom prefix_room(const PrefixPlan& plan, int S, int H_Q, int H_KV, int D) {
     PrefixRoom r;
-    r.first_row = (int64_t(S) + kv_most_shares(H_KV)) * H_Q;
+    r.first_row = (int64_t(S) + plan.own.shares) * H_Q;
     const size_t rows = size_t(r.first_row) + size_t(plan.most_pieces) * size_t(H_KV) * fq::kPrefixRows;
     r.o = round_up(rows * size_t(D) * 4);
     r.m = round_up(rows * 4);
@@ -507,17 +516,26 @@ PrefixRoom prefix_room(const PrefixPlan& plan, int S, int H_Q, int H_KV, int D) 
     return r;
 }
 
+template <int D, int DT, bool F8, int HW>
+int launch_attend_prefix(const fq::PrefixParams& pp, const PrefixPlan& plan, hipStream_t s) {
+    auto kernel = fq::paged_prefix_kernel<D, DT, F8, HW>;
+    const size_t own = HW == 4 ? 0 : (size_t(4) * pp.kv.G * D + 4 * 32 + HW * 16) * 4, lds = own > fq::PrefixCfg<D>::LDS ? own : fq::PrefixCfg<D>::LDS;
+    if (!fq_host::lds_limit_raised(reinterpret_cast<const void*>(kernel), lds)) return FQ_ERR_LAUNCH;
+    kernel<<<unsigned(plan.shares) * unsigned(pp.kv.H_KV) + unsigned(plan.own.shares) * unsigned(pp.kv.H_KV / HW), 256, lds, s>>>(pp);
+    return FQ_OK;
+}
+
 template <int D, int DT, bool F8>
 int launch_prefix(const fq::PrefixParams& pp, const PrefixPlan& plan, hipStream_t s) {
     constexpr int PT = F8 ? FQ_BF16 : DT;
-    auto kernel = fq::paged_prefix_kernel<D, DT, F8>;
-    constexpr size_t lds = fq::PrefixCfg<D>::LDS;
-    if (!fq_host::lds_limit_raised(reinterpret_cast<const void*>(kernel), lds)) return FQ_ERR_LAUNCH;
-    kernel<<<unsigned(plan.shares) * unsigned(pp.kv.H_KV), 256, lds, s>>>(pp);
-    const int st = launch_shares<D, DT, F8, true>(pp.kv, plan.own, s);
+    const int st = plan.own.heads == 4 ? launch_attend_prefix<D, DT, F8, 4>(pp, plan, s)
+                   : plan.own.heads == 2 ? launch_attend_prefix<D, DT, F8, 2>(pp, plan, s) : launch_attend_prefix<D, DT, F8, 1>(pp, plan, s);
     if (st != FQ_OK) return st;
     const int64_t values = int64_t(pp.kv.S) * pp.kv.H_KV * pp.kv.G * D;
-    fq::paged_prefix_join_kernel<D, DT, PT, 16><<<unsigned(values / 64), 256, 0, s>>>(pp);
+    if (pp.kv.G * D % 256 == 0 && values / 256 >= 2 * fq_host::device_cu_count())
+        fq::paged_prefix_join_kernel<D, DT, PT, 64><<<unsigned(values / 256), 256, 0, s>>>(pp);
+    else
+        fq::paged_prefix_join_kernel<D, DT, PT, 16><<<unsigned(values / 64), 256, 0, s>>>(pp);
     return fq_host::check_launch();
 }
 
@@ -560,6 +578,8 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
         return FQ_ERR_MISALIGNED;
     const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes);
     const PrefixRoom room = prefix_room(plan, num_seqs, H_Q, H_KV, D);
+    // (units of work are counted in 32 bits)
+    if ((int64_t(num_seqs) / plan.members + num_prefixes) * (int64_t(max_blocks_per_seq) * block_size / (8192 / D) + 1) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if (room.o / (size_t(D) * 4) * size_t(D / 32) > size_t(0x7fffffff)) return FQ_ERR_BAD_SHAPE;
     if (workspace_bytes < room.all) return FQ_ERR_WORKSPACE;
     if (!fq_host::aligned(workspace, 256)) return FQ_ERR_MISALIGNED;
