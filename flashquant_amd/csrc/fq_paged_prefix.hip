@@ -26,7 +26,7 @@ template <int D> struct PrefixCfg {
     static constexpr int NB = TT / 32, NKS = D / 16, NOB = D / 32, NU = TT / 16, NG = TT / 8;
     template <bool F8> static constexpr int depth() { return F8 ? 2 : 1; }   // tiles that are on their way
     static constexpr int SIDE = TT * D * 2;                // bytes of a tile's keys or values: 16 KB
-    static constexpr int LDS = 4 * SIDE + 2 * TT * 4 + 2 * NG * 4 + kPrefixRows * 4 + 2 * kPrefixMost * 4 + kPrefixSeqs * 2;
+    static constexpr int LDS = 4 * SIDE + 2 * 3 * (TT / 4) * 4 + kPrefixRows * 4 + 2 * kPrefixMost * 4 + kPrefixSeqs * 2;
 };
 
 // Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
@@ -48,15 +48,12 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
     using C = PrefixCfg<D>;
     using Elem = std::conditional_t<F8, uint8_t, uint16_t>;
     constexpr int TT = C::TT, NB = C::NB, NKS = C::NKS, NOB = C::NOB, NU = C::NU, NG = C::NG;
-    constexpr int PT = F8 ? FQ_BF16 : DT;                  // of weights and values in the second product
-    constexpr bool TWO_TERMS = F8 && DT == FQ_F16;         // one bf16 term would show in an fp16 result
-    constexpr bool TABLE = F8 && DT == FQ_F16;             // keys as fp16 codes, their powers applied to the scores (as bf16 they are in the keys)
-    constexpr int kDepth = PrefixCfg<D>::template depth<F8>();
+    constexpr bool POWERS = F8 && DT == FQ_F16;            // fp16 has no room for the powers of the rows: see below
+    constexpr int kDepth = C::template depth<F8>();
     const KvDecodeParams& p = pp.kv;
     uint8_t *lk = lds, *lv = lds + 2 * C::SIDE;
-    float* lscale = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, TT): what a key's score is multiplied by
-    int* lvalid = reinterpret_cast<int*>(lscale + 2 * TT);                // (2, NG): whether eight keys are on a page of the cache
-    int* list = lvalid + 2 * NG;                                          // the sequences of the rows
+    float* powers = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, 3, TT / 4), see keep()
+    int* list = reinterpret_cast<int*>(powers + 2 * 3 * (TT / 4));        // the sequences of the rows
     const int tid = threadIdx.x, lane = tid & 63, m32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = workgroup % p.H_KV, x = workgroup / p.H_KV, G = p.G;
@@ -173,32 +170,35 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
             const uint16_t* src = p.q + int64_t(list[r / G]) * p.q_seq + int64_t(head * G + r % G) * p.q_head + 8 * hf;
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) qb[ks] = *reinterpret_cast<const uint4v*>(src + 16 * ks);
+            // scores are compared before they are scaled: a negative scale goes to the query, one of zero makes it zero
+            if (!POWERS && !(p.scale_log2 > 0.0f)) {
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) qb[ks] = p.scale_log2 == 0.0f ? uint4v{0u, 0u, 0u, 0u} : qb[ks] ^ 0x80008000u;
+            }
         }
+        const float scale = p.scale_log2 == 0.0f ? 1.0f : __builtin_fabsf(p.scale_log2);
 
-        // pages of this thread's tokens in a tile; -1: none of the cache
-        auto page_of = [&](int tile, int token) {
-            const int b = (tile * TT + token) >> p.page_log2;
-            const int block = tile < end && b < blocks ? table[b] : -1;
+        // The pages of kAhead tiles, lane NG j + i that of the j-th tile's i-th eight tokens (-1: none of the cache), and those of the next ones.
+        constexpr int kAhead = kWave / NG;
+        auto pages_of = [&](int tile) {
+            const int at = tile + lane / NG, b = (at * TT + 8 * (lane % NG)) >> p.page_log2;
+            const int block = at < end && b < blocks ? table[b] : -1;
             return uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
         };
-        int page0, page1;                                  // of the tile that is asked for next
-        auto look_up = [&](int tile) {
-            page0 = page_of(tile, token0);
-            page1 = page_of(tile, token1);
-        };
+        int pages = pages_of(tile0), next_pages = pages_of(tile0 + kAhead), asked = 0;      // asked: the number in `pages` of the tile asked for next
         constexpr int NW = F8 ? 2 : 4;                     // words of eight coordinates
         struct Part {
             uint32_t word[8][NW];
             uint32_t scales[2];
-            int page0, page1;
+            uint32_t there;                                // which eights of the tile are in the cache
         };
         Part parts[kDepth];
-        auto load = [&](Part& part, int tile) {            // (no branch round the loads, so that nothing waits for them here)
-            part.page0 = page0;
-            part.page1 = page1;
+        auto load = [&](Part& part, int tile) __attribute__((always_inline)) {      // (no branch round the loads, so that nothing waits for them here)
+            part.there = uint32_t(__ballot(pages >= 0) >> (NG * asked)) & ((1u << NG) - 1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int block = h ? page1 : page0, b = block < 0 ? 0 : block, t = (tile * TT + (h ? token1 : token0)) & page_mask;
+                const int token = h ? token1 : token0, block = __builtin_amdgcn_ds_bpermute(4 * (NG * asked + token / 8), pages);
+                const int b = block < 0 ? 0 : block, t = (tile * TT + token) & page_mask;
                 const Elem* src = base + int64_t(b) * block_step + int64_t(t) * token_step;
 #pragma unroll
                 for (int i = 4 * h; i < 4 * h + 4; ++i) {
@@ -213,25 +213,45 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                 }
                 if constexpr (F8) part.scales[h] = *reinterpret_cast<const uint32_t*>(scale_base + int64_t(b) * scale_block + t);
             }
+            if (++asked == kAhead) {
+                asked = 0;
+                pages = next_pages;
+                next_pages = pages_of(tile + 1 + kAhead);
+            }
         };
-        auto keep = [&](const Part& part, int buffer) {    // into LDS, as the products read them
+        // Into LDS, as the products read them.  Codes become bfloat16 with the powers of their rows, exactly; to fp16 they go with their
+        // power relative to the highest, E, of four neighbouring tokens (exact within 2^15 of it), and what is left, 2^E, is applied in
+        // float32: to the scores (keys) and to the weights (values), where it is added to the score before the reference is chosen
+        // and taken out of the sum of weights again.
+        auto keep = [&](const Part& part, int buffer) __attribute__((always_inline)) {
             uint32_t word[8][4];
+            int power[2] = {0, 0};
             if constexpr (F8) {
 #pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    const uint32_t bits = part.scales[t >> 2];
-                    const float up = (t & 3) == 0 ? row_scale<0>(bits) : (t & 3) == 1 ? row_scale<1>(bits) : (t & 3) == 2 ? row_scale<2>(bits) : row_scale<3>(bits);
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t bits = part.scales[h];
+                    float up[4] = {row_scale<0>(bits), row_scale<1>(bits), row_scale<2>(bits), row_scale<3>(bits)};
+                    if constexpr (POWERS) {
+                        float most = __builtin_fmaxf(__builtin_fmaxf(up[0], up[1]), __builtin_fmaxf(up[2], up[3]));
+                        // (values below 2^-31 are 0 in an fp16 result)
+                        if (brings_values) most = __builtin_fmaxf(most, 0x1p-40f);
+                        power[h] = int(float_to_bits(most) >> 23) - 127;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t codes = part.word[t][i];
-                        if (DT == FQ_BF16 || brings_values) {
-                            word[t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, false));
-                            word[t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up, true));
-                        } else {
-                            word[t][2 * i] = codes_pair<FQ_F16, false>(codes);
-                            word[t][2 * i + 1] = codes_pair<FQ_F16, true>(codes);
-                        }
+                        for (int t = 0; t < 4; ++t) up[t] = __builtin_ldexpf(up[t], -power[h]);
                     }
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t codes = part.word[4 * h + t][i];
+                            if constexpr (DT == FQ_BF16) {
+                                word[4 * h + t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up[t], false));
+                                word[4 * h + t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up[t], true));
+                            } else {
+                                word[4 * h + t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, up[t], false));
+                                word[4 * h + t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, up[t], true));
+                            }
+                        }
                 }
             } else {
 #pragma unroll
@@ -240,11 +260,11 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     for (int i = 0; i < 4; ++i) word[t][i] = part.word[t][i % NW];
             }
             if (brings_values) {
-                if ((part.page0 | part.page1) < 0) {
+                if (part.there != (1u << NG) - 1) {        // (a weight of 0 times what lies there must be 0)
 #pragma unroll
                     for (int t = 0; t < 8; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) word[t][i] = (t < 4 ? part.page0 : part.page1) < 0 ? 0u : word[t][i];
+                        for (int i = 0; i < 4; ++i) word[t][i] = (part.there >> ((t < 4 ? token0 : token1) / 8)) & 1 ? word[t][i] : 0u;
                 }
                 uint8_t* dst = lv + buffer * C::SIDE + ((igroup >> 1) * NOB + (ic >> 2)) * 1024 + (igroup & 1) * 512 + (ic & 3) * 128;
 #pragma unroll
@@ -261,13 +281,21 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     const int r = token0 + i;
                     *reinterpret_cast<uint4v*>(lk + buffer * C::SIDE + r * (2 * D) + 16 * (ic ^ key_swizzle<D>(r))) = uint4v{word[i][0], word[i][1], word[i][2], word[i][3]};
                 }
+            }
+            if constexpr (POWERS) {
+                // tables by four tokens, 8 i + 4 hf + 0 .. 3 at place (hf, i): of keys, of values, and of values inverted
                 if (ic == 0) {
-                    lvalid[buffer * NG + igroup] = part.page0 >= 0 ? 1 : 0;
-                    if constexpr (TABLE)
+                    float* to = powers + buffer * 3 * (TT / 4);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            *reinterpret_cast<float4v*>(lscale + buffer * TT + token0 + 4 * h) =
-                                float4v{row_scale<0>(part.scales[h]), row_scale<1>(part.scales[h]), row_scale<2>(part.scales[h]), row_scale<3>(part.scales[h])} * p.scale_log2;
+                    for (int h = 0; h < 2; ++h) {
+                        const int four = (h ? token1 : token0) / 4, at = (four & 1) * NG + (four >> 1);
+                        if (brings_values) {
+                            to[TT / 4 + at] = float(power[h]);
+                            to[TT / 2 + at] = __builtin_ldexpf(1.0f, -power[h]);
+                        } else {
+                            to[at] = __builtin_ldexpf(p.scale_log2, power[h]);
+                        }
+                    }
                 }
             }
         };
@@ -286,19 +314,14 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
         for (int o = 0; o < 2; ++o) vread[o] = lv + 512 * hf + 16 * ((cr & 24) + ((cr & 7) ^ (4 * o + (cr >> 3))));
 
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            look_up(tile0 + d);
-            load(parts[d], tile0 + d);
-        }
-        look_up(tile0 + kDepth);
+        for (int d = 0; d < kDepth; ++d) load(parts[d], tile0 + d);
         int buffer = 0;
         auto step = [&](int tile, Part& part) __attribute__((always_inline)) {
+            const uint32_t there = part.there;
             keep(part, buffer);
             load(part, tile + kDepth);                     // (of tiles behind the last: some page's, not used)
-            look_up(tile + kDepth + 1);
             __syncthreads();
             if (live) {
-                const uint64_t valid = __ballot(lane < NG && lvalid[buffer * NG + (lane < NG ? lane : 0)] != 0);
                 float16v S[NB];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -307,26 +330,21 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     for (int ks = 0; ks < NKS; ++ks)
                         S[b] = wide_mfma<DT>(*reinterpret_cast<const uint4v*>(kread + buffer * C::SIDE + b * (64 * D) + ((32 * ks) ^ kswizzle)), qb[ks], S[b]);
                 }
+                const float4v* table = reinterpret_cast<const float4v*>(powers + buffer * 3 * (TT / 4) + hf * NG);
+                if constexpr (POWERS) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if constexpr (TABLE) {
+                    for (int b = 0; b < NB; ++b) {
+                        const float4v times = table[b], plus = table[NG / 2 + b];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float4v c = *reinterpret_cast<const float4v*>(lscale + buffer * TT + 32 * b + 8 * i + 4 * hf);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) S[b][4 * i + e] *= c[e];
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) S[b][e] *= p.scale_log2;
+                        for (int e = 0; e < 16; ++e) S[b][e] = __builtin_fmaf(S[b][e], times[e / 4], plus[e / 4]);
                     }
                 }
-                if (valid != (uint64_t(1) << NG) - 1) {
+                if (there != (1u << NG) - 1) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (((valid >> (4 * b + e / 4)) & 1) == 0) S[b][e] = -__builtin_inff();
+                            if (((there >> (4 * b + e / 4)) & 1) == 0) S[b][e] = -__builtin_inff();
                 }
                 float top = S[0][0];
 #pragma unroll
@@ -334,6 +352,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, S[b][e]);
                 top = max_xor32(top);
+                if constexpr (!POWERS) top *= scale;
                 // The reference moves only where a score would lead it by more than 2^4: rarely.
                 const float higher = top > m + 4.0f ? top : m;
                 if (__any(higher != m)) {
@@ -345,24 +364,24 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                         for (int e = 0; e < 16; ++e) O[ob][e] *= shrink;
                     m = higher;
                 }
-                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<PT>;
+                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<DT>;
                 float sum = 0.0f;
+                uint4v P[NU];
 #pragma unroll
                 for (int u = 0; u < NU; ++u) {
-                    uint4v hi, lo;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float a = __builtin_amdgcn_exp2f(S[u / 2][8 * (u & 1) + 2 * i] - ref);
-                        const float b = __builtin_amdgcn_exp2f(S[u / 2][8 * (u & 1) + 2 * i + 1] - ref);
-                        sum += a + b;
-                        hi[i] = round_pair<PT>(a, b);
-                        if constexpr (TWO_TERMS) lo[i] = round_pair<PT>(a - low_value<PT>(hi[i]), b - high_value<PT>(hi[i]));
+                        const float sa = S[u / 2][8 * (u & 1) + 2 * i], sb = S[u / 2][8 * (u & 1) + 2 * i + 1];
+                        const float a = __builtin_amdgcn_exp2f(POWERS ? sa - ref : __builtin_fmaf(sa, scale, -ref));
+                        const float b = __builtin_amdgcn_exp2f(POWERS ? sb - ref : __builtin_fmaf(sb, scale, -ref));
+                        P[u][i] = round_pair<DT>(a, b);
+                        if constexpr (POWERS) sum = __builtin_fmaf(a + b, table[NG + u / 2][2 * (u & 1) + i / 2], sum);
+                        else sum += a + b;
                     }
 #pragma unroll
                     for (int ob = 0; ob < NOB; ++ob) {
                         const uint4v v = *reinterpret_cast<const uint4v*>(vread[ob & 1] + buffer * C::SIDE + (u * NOB + ob) * 1024);
-                        O[ob] = wide_mfma<PT>(v, hi, O[ob]);
-                        if constexpr (TWO_TERMS) O[ob] = wide_mfma<PT>(v, lo, O[ob]);
+                        O[ob] = wide_mfma<DT>(v, P[u], O[ob]);
                     }
                 }
                 l += sum;
@@ -384,7 +403,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     *reinterpret_cast<float4v*>(p.part_o + at * D + 32 * ob + 16 * (e / 8) + 8 * hf + e % 8) =
                         float4v{O[ob][e], O[ob][e + 1], O[ob][e + 2], O[ob][e + 3]};
             if (hf == 0) {
-                p.part_m[at] = m;
+                p.part_m[at] = POWERS ? m + (kKvLift<FQ_BF16> - kKvLift<FQ_F16>) : m;      // (as the parts of the own tokens have it)
                 p.part_l[at] = l;
             }
         }

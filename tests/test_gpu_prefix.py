@@ -54,7 +54,7 @@ def wanted(q, cache, table, lens, ids, prefixes, sm):
     kc, vc, ks, vs = cache
     keys, values = (c.double() if s is None else stood_for(c, s) for c, s in ((kc, ks), (vc, vs)))
     o, l, to, tl = attended(q, keys, values, table, lens, sm)
-    weight = 2.0 ** -16 if ks is not None and q.dtype == HF else torch.finfo(BF if ks is not None else q.dtype).eps / 2
+    weight = torch.finfo(q.dtype).eps / 2
     # sum of weights times sizes, with the size of values as the value
     size, _, _, _ = attended(q, keys, values.abs(), table, lens, sm)
     most = values[torch.isfinite(values)].abs().max()
