@@ -180,12 +180,15 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
 
         // The pages of kAhead tiles, lane NG j + i that of the j-th tile's i-th eight tokens (-1: none of the cache), and those of the next ones.
         constexpr int kAhead = kWave / NG;
-        auto pages_of = [&](int tile) {
-            const int at = tile + lane / NG, b = (at * TT + 8 * (lane % NG)) >> p.page_log2;
-            const int block = at < end && b < blocks ? table[b] : -1;
-            return uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
+        auto entry_of = [&](int tile) { return ((tile + lane / NG) * TT + 8 * (lane % NG)) >> p.page_log2; };
+        auto read_entries = [&](int tile) {
+            const int b = entry_of(tile);
+            return table[b < blocks ? b : blocks - 1];
         };
-        int pages = pages_of(tile0), next_pages = pages_of(tile0 + kAhead), asked = 0;      // asked: the number in `pages` of the tile asked for next
+        auto pages_of = [&](int tile, int block) {
+            return tile + lane / NG < end && entry_of(tile) < blocks && uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
+        };
+        int pages = pages_of(tile0, read_entries(tile0)), next = read_entries(tile0 + kAhead), asked = 0;      // asked: the number in `pages` of the tile asked for next
         constexpr int NW = F8 ? 2 : 4;                     // words of eight coordinates
         struct Part {
             uint32_t word[8][NW];
@@ -215,8 +218,8 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
             }
             if (++asked == kAhead) {
                 asked = 0;
-                pages = next_pages;
-                next_pages = pages_of(tile + 1 + kAhead);
+                pages = pages_of(tile + 1, next);
+                next = read_entries(tile + 1 + kAhead);
             }
         };
         // Into LDS, as the products read them.  Codes become bfloat16 with the powers of their rows, exactly; to fp16 they go with their
@@ -443,9 +446,11 @@ __global__ __launch_bounds__(256) void paged_prefix_join_kernel(const PrefixPara
     const int64_t unit = blockIdx.x / columns;                           // sequence and KV head
     const int seq = int(unit / p.H_KV), head = int(unit - int64_t(seq) * p.H_KV);
     const int c = 4 * (int(blockIdx.x % columns) * Q + threadIdx.x % Q), r0 = threadIdx.x / Q, h = c / D;
+    int2 own = p.place[seq];
+    int4 before = pp.place[seq];
     const int len = kv_length(p, seq), shared = kv_shared(p, seq, len);
-    const int2 own = len > shared ? p.place[seq] : int2{0, 0};           // (of sequences without tokens nothing is written)
-    const int4 before = shared > 0 ? pp.place[seq] : int4{0, 0, 0, 0};
+    if (len <= shared) own = int2{0, 0};                                 // (of sequences without tokens nothing is written)
+    if (shared == 0) before = int4{0, 0, 0, 0};
     const int pieces = own.y + before.y;
     auto row_of = [&](int i) {
         return i < own.y ? (int64_t(own.x + seq + i) * p.H_KV + head) * p.G + h
@@ -505,12 +510,17 @@ namespace {
 struct PrefixPlan {
     KvPlan own;
     int shares, min_tiles, members, most_pieces;
+    int most_own;            // shares of the own tokens in any table
 };
-PrefixPlan prefix_plan(int S, int H_KV, int G, int D, int num_prefixes) {
+PrefixPlan prefix_plan(int S, int H_KV, int G, int D, int num_prefixes, int64_t max_tokens) {
     const int64_t cus = fq_host::device_cu_count();
     PrefixPlan r;
-    const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1, each = D == 256 ? 1 : 2;       // workgroups that a CU has at a time
-    r.own = {int((each * cus * together + H_KV - 1) / H_KV), together, 4 / together};
+    const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1;
+    auto own_shares = [&](int each) { return int((each * cus * together + H_KV - 1) / H_KV); };
+    // Workgroups for the sequences' own tokens: one a CU, beside one of the prefixes', and two where the table is too narrow for much of
+    // either (us, one / two: 96 sequences of 50 to 1200 tokens behind 6000 63 / 74, 64 of up to 300 behind 512 23.0 / 20.5).
+    r.most_own = own_shares(2);
+    r.own = {max_tokens <= 1024 ? r.most_own : own_shares(1), together, 4 / together};
     r.shares = int((cus + H_KV - 1) / H_KV);
     r.min_tiles = 2;
     r.members = fq::kPrefixRows / G;
@@ -525,7 +535,7 @@ struct PrefixRoom {
 };
 PrefixRoom prefix_room(const PrefixPlan& plan, int S, int H_Q, int H_KV, int D) {
     PrefixRoom r;
-    r.first_row = (int64_t(S) + plan.own.shares) * H_Q;
+    r.first_row = (int64_t(S) + plan.most_own) * H_Q;
     const size_t rows = size_t(r.first_row) + size_t(plan.most_pieces) * size_t(H_KV) * fq::kPrefixRows;
     r.o = round_up(rows * size_t(D) * 4);
     r.m = round_up(rows * 4);
@@ -568,7 +578,7 @@ int launch_prefix_type(const fq::PrefixParams& pp, const PrefixPlan& plan, bool 
 
 extern "C" size_t fq_paged_prefix_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int num_prefixes) {
     if (check_kv_shape(num_seqs, H_Q, H_KV, D, 16, 1, 1) != FQ_OK || num_seqs == 0 || num_prefixes < 0 || num_prefixes > fq::kPrefixMost) return 0;
-    return prefix_room(prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes), num_seqs, H_Q, H_KV, D).all;
+    return prefix_room(prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes, 0), num_seqs, H_Q, H_KV, D).all;
 }
 
 extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
@@ -595,7 +605,7 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
         (f8 && !(codes_aligned(key_cache, key_strides, key_scales, key_scale_strides) &&
                  codes_aligned(value_cache, value_strides, value_scales, value_scale_strides))))
         return FQ_ERR_MISALIGNED;
-    const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes);
+    const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes, int64_t(max_blocks_per_seq) * block_size);
     const PrefixRoom room = prefix_room(plan, num_seqs, H_Q, H_KV, D);
     // (units of work are counted in 32 bits)
     if ((int64_t(num_seqs) / plan.members + num_prefixes) * (int64_t(max_blocks_per_seq) * block_size / (8192 / D) + 1) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
