@@ -1,5 +1,6 @@
-"""Paged storage driven from the GPU: one table of pages for all layers, and layers that keep their keys and values at 16 bits or
-packed (TQ4) on those pages, with rotary positions applied on the way in.
+"""Paged storage driven from the GPU: one table of pages for all layers, and layers that keep their keys and values at 16 bits, at 8
+bits or packed (TQ4) on those pages, with rotary positions applied on the way in.  Sequences may begin with the same pages; single
+tokens then attend to these once for all.
 
 The reference has the packed pages (src/flashquant/vllm/impl.py:132-138, 220-263) and leaves tables, positions and 16-bit layers to
 vLLM; here a decode step is ``PageTable.schedule`` once and ``step`` per layer, without a look at lengths or pages from the host, so
@@ -7,11 +8,12 @@ that it can be captured in a graph."""
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 
-from flashquant_amd.kernels import (paged_kv_decode, paged_schedule, rotary_embedding, rotary_paged_store)
+from flashquant_amd.kernels import (paged_kv8_decode, paged_kv8_read, paged_kv_decode, paged_prefix_decode, paged_schedule, rotary_embedding,
+                                    rotary_paged_store, rotary_paged_store8)
 from flashquant_amd.kernels._native import native
 from flashquant_amd.vllm.impl import TQ4AttentionKernels
 from flashquant_amd.vllm.spec import get_kv_cache_shape
@@ -25,7 +27,8 @@ class PagedStep(NamedTuple):
 
     The tokens are packed: sequences that bring none have none, wherever they are in the table, and what is behind the last token is
     padding.  ``token_table`` (num_tokens, max_blocks) and ``token_lens`` (num_tokens,) int32 hold, token by token, the pages of its
-    sequence and how many tokens it sees (itself the last; padding: none); None where ``num_tokens`` is above ``max_seqs``."""
+    sequence and how many tokens it sees (itself the last; padding: none); None where ``num_tokens`` is above ``max_seqs``.  Where the
+    table has prefixes, ``token_prefix`` (num_tokens,) int32 is the one of a token's sequence (or -1) and ``prefix_lens`` their tokens."""
     slot_mapping: torch.Tensor
     positions: torch.Tensor
     seq_lens: torch.Tensor
@@ -34,6 +37,8 @@ class PagedStep(NamedTuple):
     pages_taken: torch.Tensor
     token_table: Optional[torch.Tensor] = None
     token_lens: Optional[torch.Tensor] = None
+    token_prefix: Optional[torch.Tensor] = None
+    prefix_lens: Optional[torch.Tensor] = None
 
 
 def _rows(q: torch.Tensor, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -45,12 +50,15 @@ def _rows(q: torch.Tensor, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]
 
 
 class PageTable:
-    """Block tables, lengths and the list of free pages of ``max_seqs`` sequences, all on the GPU."""
+    """Block tables, lengths and the list of free pages of ``max_seqs`` sequences, all on the GPU, and up to ``max_prefixes`` prefixes
+    that sequences share: whole pages that belong to the prefix and not to a sequence."""
 
     def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_blocks_per_seq: int,
-                 device: Optional[torch.device] = None) -> None:
+                 device: Optional[torch.device] = None, *, max_prefixes: int = 0) -> None:
         if device is None:
             device = torch.device("cuda")
+        if not 0 <= max_prefixes <= 1024:
+            raise ValueError(f"max_prefixes must be 0 to 1024, got {max_prefixes}")
         self.num_blocks = num_blocks
         self.block_size = block_size
         i32 = dict(dtype=torch.int32, device=device)
@@ -60,6 +68,12 @@ class PageTable:
         self._pages = torch.arange(num_blocks + 1, **i32)
         self.free_blocks = self._pages[:num_blocks]
         self.free_start = torch.zeros(1, **i32)
+        # pages and tokens of the prefixes, the prefix of every sequence; on the host which sequences share one, and which there are
+        self.prefix_ids = torch.full((max_seqs,), -1, **i32)
+        self.prefix_lens = torch.zeros(max_prefixes, **i32)
+        self._prefix_table = torch.full((max_prefixes, max_blocks_per_seq), -1, **i32)
+        self._prefix_of: List[int] = [-1] * max_seqs
+        self._made: List[bool] = [False] * max_prefixes
 
     def schedule(self, query_lens: torch.Tensor, num_tokens: int) -> PagedStep:
         """Gives ``query_lens[s]`` (int32) new tokens of sequence s their pages, slots and positions and counts them into the
@@ -67,21 +81,75 @@ class PageTable:
         count in no length."""
         s = paged_schedule(self.context_lens, query_lens, self.block_table, self.free_blocks, self.block_size, num_tokens,
                            free_start=self.free_start, capped=True)
-        token_table, token_lens = native().paged_advance(s, self.context_lens, self.free_start, self.block_table, self.num_blocks,
-                                                         self.block_size, num_tokens <= self.block_table.shape[0])
-        return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, token_table, token_lens)
+        rows = num_tokens <= self.block_table.shape[0]
+        state = s, self.context_lens, self.free_start, self.block_table, self.num_blocks, self.block_size, rows
+        if not any(self._made):
+            return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, *native().paged_advance(*state))
+        token_table, token_lens, token_prefix = native().paged_advance_prefix(*state, self.prefix_ids)
+        return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, token_table, token_lens, token_prefix,
+                         self.prefix_lens if rows else None)
+
+    def make_prefix(self, seq: int, prefix: int) -> None:
+        """The whole pages that sequence ``seq`` has by now become prefix ``prefix`` (below ``max_prefixes``, not in use), which the
+        sequence shares from now on."""
+        self._check(seq, prefix, made=False)
+        tokens = self.context_lens[seq] // self.block_size * self.block_size
+        row = self.block_table[seq]
+        self.prefix_lens[prefix] = tokens
+        self._prefix_table[prefix] = torch.where(torch.arange(row.shape[0], device=row.device) < tokens // self.block_size, row, -1)
+        self._made[prefix] = True
+        self._share(seq, prefix)
+
+    def join_prefix(self, seq: int, prefix: int) -> None:
+        """Sequence ``seq``, which has no tokens, begins with those of ``prefix``."""
+        self._check(seq, prefix, made=True)
+        self.block_table[seq] = self._prefix_table[prefix]
+        self.context_lens[seq] = self.prefix_lens[prefix]
+        self._share(seq, prefix)
+
+    def drop_prefix(self, prefix: int) -> None:
+        """Ends ``prefix``, which no sequence shares any more: its pages are free again."""
+        if not self._made[prefix]:
+            raise ValueError(f"prefix {prefix} is not in use")
+        if prefix in self._prefix_of:
+            raise ValueError(f"sequence {self._prefix_of.index(prefix)} still shares prefix {prefix}")
+        self._free(self._prefix_table[prefix] >= 0, self._prefix_table[prefix])
+        self._prefix_table[prefix] = -1
+        self.prefix_lens[prefix] = 0
+        self._made[prefix] = False
 
     def release(self, seq: int) -> None:
-        """Ends sequence ``seq``: its pages are free again (the next to be taken) and its length is 0."""
-        row = self.block_table[seq]
+        """Ends sequence ``seq``: its pages, but those of a prefix that it shares, are free again (the next to be taken) and its length is
+        0."""
+        row, prefix = self.block_table[seq], self._prefix_of[seq]
         held = (self.context_lens[seq] + self.block_size - 1) // self.block_size
-        mine = (row >= 0) & (torch.arange(row.shape[0], device=row.device) < held)
+        column = torch.arange(row.shape[0], device=row.device)
+        mine = (row >= 0) & (column < held)
+        if prefix >= 0:
+            mine &= column >= self.prefix_lens[prefix] // self.block_size
+            self.prefix_ids[seq] = -1
+            self._prefix_of[seq] = -1
+        self._free(mine, row)
+        self.block_table[seq] = -1
+        self.context_lens[seq] = 0
+
+    def _check(self, seq: int, prefix: int, made: bool) -> None:
+        if not 0 <= seq < len(self._prefix_of) or not 0 <= prefix < len(self._made):
+            raise ValueError(f"no sequence {seq} or no prefix {prefix}")
+        if self._prefix_of[seq] >= 0:
+            raise ValueError(f"sequence {seq} shares prefix {self._prefix_of[seq]} already")
+        if self._made[prefix] != made:
+            raise ValueError(f"prefix {prefix} is {'not ' if made else ''}in use")
+
+    def _share(self, seq: int, prefix: int) -> None:
+        self.prefix_ids[seq] = prefix
+        self._prefix_of[seq] = prefix
+
+    def _free(self, mine: torch.Tensor, row: torch.Tensor) -> None:
         count = mine.sum(dtype=torch.int32)
         place = torch.where(mine, self.free_start - count + torch.cumsum(mine, 0) - 1, self.num_blocks)
         self._pages[place] = row
         self.free_start -= count
-        self.block_table[seq] = -1
-        self.context_lens[seq] = 0
 
 
 class PagedKVLayer:
@@ -105,7 +173,48 @@ class PagedKVLayer:
         """``store`` of a step with at most one token of every sequence, then each one's attention over its sequence: (num_tokens, H_Q,
         head_dim); rows behind the last token are 0."""
         rows = _rows(q, step)
-        return paged_kv_decode(self.store(q, k, v, step), self.keys, self.values, *rows, self.sm_scale, window=self.window)
+        q = self.store(q, k, v, step)
+        if step.token_prefix is not None and self.window == 0:
+            return paged_prefix_decode(q, self.keys, self.values, *rows, step.token_prefix, step.prefix_lens, self.sm_scale)
+        return paged_kv_decode(q, self.keys, self.values, *rows, self.sm_scale, window=self.window)
+
+
+class PagedKV8Layer:
+    """The same at 8 bits: e4m3 rows (num_blocks, block_size, heads, head_dim) with a power of two each (num_blocks, heads, block_size).
+    ``dtype``: of queries, of keys and values on the way in, and of rows read back."""
+
+    def __init__(self, table: PageTable, heads: int, head_dim: int, inv_freq: torch.Tensor, rotary_scale: float = 1.0, *,
+                 interleaved: bool = False, window: int = 0, sm_scale: Optional[float] = None, dtype: torch.dtype = torch.bfloat16) -> None:
+        device = table.block_table.device
+        self.table = table
+        rows = torch.zeros(2, table.num_blocks, table.block_size, heads, head_dim, dtype=torch.uint8, device=device)
+        scales = torch.zeros(2, table.num_blocks, heads, table.block_size, dtype=torch.uint8, device=device)
+        self.keys, self.values = rows.view(torch.float8_e4m3fn)
+        self.key_scales, self.value_scales = scales.view(torch.float8_e8m0fnu)
+        self.inv_freq, self.rotary_scale, self.interleaved = inv_freq.to(device), rotary_scale, interleaved
+        self.window, self.dtype = window, dtype
+        self.sm_scale = 1.0 / math.sqrt(head_dim) if sm_scale is None else sm_scale
+
+    def store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> torch.Tensor:
+        """The step's keys and values, rotated and quantised, into their slots; returns the rotated queries (num_tokens, H_Q, head_dim)."""
+        return rotary_paged_store8(q, k, v, step.positions, step.slot_mapping, self.inv_freq, self.keys, self.values, self.key_scales,
+                                   self.value_scales, interleaved=self.interleaved, scale=self.rotary_scale)
+
+    def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> torch.Tensor:
+        """``store`` of a step with at most one token of every sequence, then each one's attention over its sequence: (num_tokens, H_Q,
+        head_dim); rows behind the last token are 0."""
+        rows = _rows(q, step)
+        q = self.store(q, k, v, step)
+        if step.token_prefix is not None and self.window == 0:
+            return paged_prefix_decode(q, self.keys, self.values, *rows, step.token_prefix, step.prefix_lens, self.sm_scale,
+                                       key_scales=self.key_scales, value_scales=self.value_scales)
+        return paged_kv8_decode(q, self.keys, self.values, self.key_scales, self.value_scales, *rows, self.sm_scale, window=self.window)
+
+    def read(self, cu_seqlens: torch.Tensor, num_tokens: int, starts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys (rotated) and values of the table's sequences, (num_tokens, heads, head_dim) each: of sequence s its tokens from
+        ``starts[s]`` (0 without) on, to rows ``cu_seqlens[s]`` .. ``cu_seqlens[s + 1]``; what the attention of a prompt's next chunk takes."""
+        return paged_kv8_read(self.keys, self.values, self.key_scales, self.value_scales, self.table.block_table, cu_seqlens, num_tokens,
+                              starts=starts, dtype=self.dtype)
 
 
 class PagedTQ4Layer:

@@ -221,11 +221,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_sch
     return {slots, positions, lens, cu, end};
 }
 
-// (token_table, token_lens) where rows are asked for; context_lens and free_start are written in place.  `schedule`: what paged_schedule
-// returned, for the same block table.
-std::tuple<MaybeTensor, MaybeTensor> paged_advance(const std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>& schedule,
-                                                   at::Tensor context_lens, at::Tensor free_start, const at::Tensor& block_table,
-                                                   int64_t num_blocks, int64_t block_size, bool rows) {
+using Schedule = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+// (token_table, token_lens, token_prefix) where rows are asked for, the last with prefix_ids; context_lens and free_start are written in
+// place.  `schedule`: what paged_schedule returned, for the same block table.
+std::tuple<MaybeTensor, MaybeTensor, MaybeTensor> advance(const Schedule& schedule, at::Tensor context_lens, at::Tensor free_start,
+                                                          const at::Tensor& block_table, int64_t num_blocks, int64_t block_size, bool rows,
+                                                          const MaybeTensor& prefix_ids) {
     const auto& [slots, positions, lens, cu, end] = schedule;
     fqbind::require_gpu(context_lens, "context_lens");
     for (const at::Tensor* t : {&slots, &positions, &lens, &cu, &end, static_cast<const at::Tensor*>(&free_start), &block_table})
@@ -238,26 +240,40 @@ std::tuple<MaybeTensor, MaybeTensor> paged_advance(const std::tuple<at::Tensor, 
               block_table.size(1) <= 0x7fffffff && block_table.stride(1) == 1 && (S <= 1 || block_table.stride(0) >= block_table.size(1)),
           "block_table must be int32 of shape (num_reqs, max_blocks) with contiguous rows");
     check(num_blocks >= 0 && num_blocks <= 0x7fffffff && S <= 0x7fffffff, "too many pages or requests");
+    if (prefix_ids.has_value()) {
+        check_place(*prefix_ids, context_lens, "prefix_ids");
+        check(is(*prefix_ids, at::kInt, S), "prefix_ids must be contiguous int32 of shape (num_reqs,)");
+        check(!extents_meet_any(*prefix_ids, {&context_lens, &free_start}), "context_lens and free_start must share no memory with the other operands");
+    }
     check_written(context_lens);
     check_written(free_start);
     check(!extents_meet_any(context_lens, {&positions, &lens, &cu, &end, &free_start, &block_table}) &&
               !extents_meet_any(free_start, {&positions, &lens, &cu, &end, &block_table}),
           "context_lens and free_start must share no memory with the other operands");
     c10::DeviceGuard guard(context_lens.device());
-    at::Tensor table, token_lens;
+    at::Tensor table, token_lens, token_prefix;
+    const bool prefixes = rows && prefix_ids.has_value();
     if (rows) {
         table = new_tensor({tokens, block_table.size(1)}, at::kInt, context_lens);
         token_lens = new_tensor({tokens}, at::kInt, context_lens);
     }
-    const int st = fq_paged_advance(lens.data_ptr<int32_t>(), end.data_ptr<int32_t>(), int(num_blocks), context_lens.data_ptr<int32_t>(),
-                                    free_start.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
-                                    block_table.data_ptr<int32_t>(), S <= 1 ? block_table.size(1) : block_table.stride(0),
-                                    rows ? table.data_ptr<int32_t>() : nullptr, rows ? token_lens.data_ptr<int32_t>() : nullptr, int(S),
-                                    rows ? tokens : 0, int(block_table.size(1)), int(block_size), fqbind::current_stream(context_lens));
+    if (prefixes) token_prefix = new_tensor({tokens}, at::kInt, context_lens);
+    const int st = fq_paged_advance_prefix(lens.data_ptr<int32_t>(), end.data_ptr<int32_t>(), int(num_blocks), context_lens.data_ptr<int32_t>(),
+                                           free_start.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
+                                           block_table.data_ptr<int32_t>(), S <= 1 ? block_table.size(1) : block_table.stride(0),
+                                           prefixes ? prefix_ids->data_ptr<int32_t>() : nullptr, rows ? table.data_ptr<int32_t>() : nullptr,
+                                           rows ? token_lens.data_ptr<int32_t>() : nullptr, prefixes ? token_prefix.data_ptr<int32_t>() : nullptr,
+                                           int(S), rows ? tokens : 0, int(block_table.size(1)), int(block_size),
+                                           fqbind::current_stream(context_lens));
     fqbind::raise_on_error(st, "paged_advance");
     written(context_lens);
     written(free_start);
-    return {rows ? MaybeTensor(table) : std::nullopt, rows ? MaybeTensor(token_lens) : std::nullopt};
+    return {rows ? MaybeTensor(table) : std::nullopt, rows ? MaybeTensor(token_lens) : std::nullopt, prefixes ? MaybeTensor(token_prefix) : std::nullopt};
+}
+std::tuple<MaybeTensor, MaybeTensor> paged_advance(const Schedule& schedule, at::Tensor context_lens, at::Tensor free_start, const at::Tensor& block_table,
+                                                   int64_t num_blocks, int64_t block_size, bool rows) {
+    const auto r = advance(schedule, context_lens, free_start, block_table, num_blocks, block_size, rows, std::nullopt);
+    return {std::get<0>(r), std::get<1>(r)};
 }
 
 std::tuple<at::Tensor, MaybeTensor> paged_kv_decode(const at::Tensor& q, const at::Tensor& key_cache, const at::Tensor& value_cache,
@@ -327,6 +343,9 @@ void bind_paged_kv(py::module_& m) {
     m.def("paged_advance", &paged_advance, py::arg("schedule"), py::arg("context_lens"), py::arg("free_start"), py::arg("block_table"),
           py::arg("num_blocks"), py::arg("block_size"), py::arg("rows"),
           "After paged_schedule: context_lens and free_start for the next one, in place; with rows (token_table, token_lens) of its tokens");
+    m.def("paged_advance_prefix", &advance, py::arg("schedule"), py::arg("context_lens"), py::arg("free_start"), py::arg("block_table"),
+          py::arg("num_blocks"), py::arg("block_size"), py::arg("rows"), py::arg("prefix_ids"),
+          "paged_advance with the prefix of every token as well: (token_table, token_lens, token_prefix)");
     m.def("rotary_embedding", &rotary_embedding, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"),
           py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("inverse") = false, py::arg("q_out") = py::none(),
           py::arg("k_out") = py::none(), "Rotary positions on the first 2 * len(inv_freq) coordinates of every head");

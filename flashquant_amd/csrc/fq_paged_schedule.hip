@@ -187,6 +187,8 @@ struct AdvanceParams {
     const int32_t* table;
     int32_t* token_table;           // (num_tokens, max_blocks)
     int32_t* token_lens;
+    const int32_t* prefix_ids;      // of every request, with shared prefixes; else null
+    int32_t* token_prefix;
     int64_t table_row;
     int S, max_blocks, num_blocks, page_log2;
     int state_groups, parts;        // workgroups of the state, those of a token's row
@@ -215,6 +217,7 @@ __global__ __launch_bounds__(kScheduleThreads) void paged_advance_kernel(const A
     if (part == 0 && tid == 0) {
         const int64_t room = int64_t(p.max_blocks) << p.page_log2, upto = p.positions[token] + 1;
         p.token_lens[token] = s < 0 ? 0 : int(upto < room ? upto : room);
+        if (p.token_prefix != nullptr) p.token_prefix[token] = s < 0 ? -1 : p.prefix_ids[s];
     }
     const int32_t* from = p.table + int64_t(s < 0 ? 0 : s) * p.table_row;
     int32_t* to = p.token_table + int64_t(token) * p.max_blocks;
@@ -279,17 +282,27 @@ extern "C" int fq_paged_advance(const int32_t* seq_lens, const int32_t* free_end
                                 const int32_t* cu_seqlens, const int64_t* positions, const int32_t* block_table, int64_t block_table_stride,
                                 int32_t* token_table, int32_t* token_lens, int num_reqs, int64_t num_tokens, int max_blocks_per_seq,
                                 int block_size, void* stream) {
+    return fq_paged_advance_prefix(seq_lens, free_end, num_blocks, context_lens, free_start, cu_seqlens, positions, block_table, block_table_stride,
+                                   nullptr, token_table, token_lens, nullptr, num_reqs, num_tokens, max_blocks_per_seq, block_size, stream);
+}
+
+extern "C" int fq_paged_advance_prefix(const int32_t* seq_lens, const int32_t* free_end, int num_blocks, int32_t* context_lens,
+                                       int32_t* free_start, const int32_t* cu_seqlens, const int64_t* positions, const int32_t* block_table,
+                                       int64_t block_table_stride, const int32_t* prefix_ids, int32_t* token_table, int32_t* token_lens,
+                                       int32_t* token_prefix, int num_reqs, int64_t num_tokens, int max_blocks_per_seq, int block_size,
+                                       void* stream) {
     if (num_reqs < 0 || num_reqs > (1 << 30) || num_blocks < 0 || num_tokens < 0 || num_tokens > 0x7fffffffLL || max_blocks_per_seq <= 0 ||
         block_table_stride < max_blocks_per_seq || (num_reqs == 0 && num_tokens > 0))
         return FQ_ERR_BAD_SHAPE;
     if (block_size != 8 && block_size != 16 && block_size != 32) return FQ_ERR_UNSUPPORTED_BLOCK;
     if (int64_t(max_blocks_per_seq) * block_size > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if (!free_end || !free_start || (num_reqs > 0 && (!seq_lens || !context_lens)) ||
-        (num_tokens > 0 && (!cu_seqlens || !positions || !block_table || !token_table || !token_lens)))
+        (num_tokens > 0 && (!cu_seqlens || !positions || !block_table || !token_table || !token_lens || (token_prefix && !prefix_ids))))
         return FQ_ERR_NULL_POINTER;
     fq::AdvanceParams p;
     p.seq_lens = seq_lens; p.free_end = free_end; p.context = context_lens; p.free_start = free_start;
     p.cu = cu_seqlens; p.positions = positions; p.table = block_table; p.token_table = token_table; p.token_lens = token_lens;
+    p.prefix_ids = prefix_ids; p.token_prefix = token_prefix;
     p.table_row = block_table_stride;
     p.S = num_reqs; p.max_blocks = max_blocks_per_seq; p.num_blocks = num_blocks;
     p.page_log2 = block_size == 8 ? 3 : block_size == 16 ? 4 : 5;

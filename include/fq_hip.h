@@ -640,7 +640,14 @@ int fq_paged_schedule_capped(const int32_t* context_lens, const int32_t* query_l
  *   token_lens     (num_tokens,) int32 out: position + 1, at most max_blocks_per_seq * block_size; 0 behind the last token
  * With them as block table and lengths the decodes attend token by token, whichever requests bring none.  num_tokens may be 0
  * (no rows), and is 0 where num_reqs is.  No output may overlap another operand.
+ * fq_paged_advance_prefix: the same, and with token_prefix (num_tokens,) int32 out (or NULL) the entry of prefix_ids (num_reqs,) int32 of
+ * the request that a token is of; -1 behind the last token.  With it fq_paged_prefix_decode attends token by token.
  */
+int fq_paged_advance_prefix(const int32_t* seq_lens, const int32_t* free_end, int num_blocks, int32_t* context_lens, int32_t* free_start,
+                            const int32_t* cu_seqlens, const int64_t* positions, const int32_t* block_table, int64_t block_table_stride,
+                            const int32_t* prefix_ids, int32_t* token_table, int32_t* token_lens, int32_t* token_prefix, int num_reqs,
+                            int64_t num_tokens, int max_blocks_per_seq, int block_size, void* stream);
+
 int fq_paged_advance(const int32_t* seq_lens, const int32_t* free_end, int num_blocks, int32_t* context_lens, int32_t* free_start,
                      const int32_t* cu_seqlens, const int64_t* positions, const int32_t* block_table, int64_t block_table_stride,
                      int32_t* token_table, int32_t* token_lens, int num_reqs, int64_t num_tokens, int max_blocks_per_seq,

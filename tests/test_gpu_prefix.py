@@ -8,7 +8,7 @@ import torch
 
 from flashquant_amd import kernels as K
 from flashquant_amd.kernels._native import native
-from test_gpu_kv8 import BF, DEV, E4, E8, HEADS, HF, U8, attended, caches, check, gen, raw, stood_for
+from tests.test_gpu_kv8 import BF, DEV, E4, E8, HEADS, HF, U8, attended, caches, check, gen, raw, stood_for
 
 pytestmark = pytest.mark.gpu
 BITS = [16, 8]
