@@ -26,7 +26,7 @@ template <int D> struct PrefixCfg {
     static constexpr int NB = TT / 32, NKS = D / 16, NOB = D / 32, NU = TT / 16, NG = TT / 8;
     template <bool F8> static constexpr int depth() { return F8 ? 2 : 1; }   // tiles that are on their way
     static constexpr int SIDE = TT * D * 2;                // bytes of a tile's keys or values: 16 KB
-    static constexpr int LDS = 4 * SIDE + 2 * 3 * (TT / 4) * 4 + kPrefixRows * 4 + 2 * kPrefixMost * 4 + kPrefixSeqs * 2;
+    static constexpr int LDS = 4 * SIDE + 2 * 3 * (TT / 4) * 4 + kPrefixRows * 4 + 3 * kPrefixMost * 4 + kPrefixSeqs * 2;
 };
 
 // Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
@@ -62,7 +62,8 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
     // (all lengths and ids are asked for at once; what the sequences share is kept in LDS for the lists of members)
     int* count = list + kPrefixRows;
     int* shared_len = count + kPrefixMost;
-    int16_t* shares_of = reinterpret_cast<int16_t*>(shared_len + kPrefixMost);
+    int* leader = shared_len + kPrefixMost;                // the first of its members
+    int16_t* shares_of = reinterpret_cast<int16_t*>(leader + kPrefixMost);
     constexpr int kAhead = 4;
     int ids[kAhead], lens[kAhead];
     auto ask = [&](int s0) {
@@ -80,6 +81,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
     ask(0);
     for (int i = tid; i < p.num_prefixes; i += 256) {
         count[i] = 0;
+        leader[i] = p.S;
         const int n = p.prefix_lens[i] >> p.page_log2 << p.page_log2;
         shared_len[i] = n > 0 ? n : 0;
     }
@@ -96,7 +98,10 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
         for (int j = 0; j < kAhead; ++j) {
             const int s = s0 + 256 * j + tid, id = prefix_of(ids[j], lens[j]);
             if (s < kPrefixSeqs && s < p.S) shares_of[s] = int16_t(id);
-            if (id >= 0) atomicAdd(&count[id], 1);
+            if (id >= 0) {
+                atomicAdd(&count[id], 1);
+                atomicMin(&leader[id], s);
+            }
         }
     }
     __syncthreads();
@@ -144,6 +149,19 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
         const int n_members = __builtin_amdgcn_readfirstlane(count[prefix]), shared = __builtin_amdgcn_readfirstlane(shared_len[prefix]);
         const int tiles = (shared + TT - 1) / TT, groups = int(uint32_t(n_members + pp.members - 1) / uint32_t(pp.members));
         const int here = left < tiles - tile0 ? left : tiles - tile0, end = tile0 + here;
+        const int32_t* table = p.table + int64_t(__builtin_amdgcn_readfirstlane(leader[prefix])) * p.table_row;
+        const int blocks = shared >> p.page_log2;
+        // The pages of kAhead tiles, lane NG j + i that of the j-th tile's i-th eight tokens (-1: none of the cache), and those of the next ones.
+        constexpr int kAhead = kWave / NG;
+        auto entry_of = [&](int tile) { return ((tile + lane / NG) * TT + 8 * (lane % NG)) >> p.page_log2; };
+        auto read_entries = [&](int tile) {
+            const int b = entry_of(tile);
+            return table[b < blocks ? b : blocks - 1];
+        };
+        auto pages_of = [&](int tile, int block) {
+            return tile + lane / NG < end && entry_of(tile) < blocks && uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
+        };
+        const int first_entries = read_entries(tile0);
         // the group's members, in the order of the sequences
         if (w == 0) {
             int rank = 0;
@@ -159,8 +177,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
         }
         __syncthreads();
         const int members = n_members - group * pp.members < pp.members ? n_members - group * pp.members : pp.members;
-        const int rows = members * G, blocks = shared >> p.page_log2;
-        const int32_t* table = p.table + int64_t(list[0]) * p.table_row;
+        const int rows = members * G;
         if (tile0 == 0 && head == 0 && tid < members) pp.place[list[tid]] = int4{piece, 1 + (tiles - here + size - 1) / size, tid * G, 0};
         const int row = 32 * w + m32;
         const bool live = 32 * w < rows;
@@ -178,17 +195,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
         }
         const float scale = p.scale_log2 == 0.0f ? 1.0f : __builtin_fabsf(p.scale_log2);
 
-        // The pages of kAhead tiles, lane NG j + i that of the j-th tile's i-th eight tokens (-1: none of the cache), and those of the next ones.
-        constexpr int kAhead = kWave / NG;
-        auto entry_of = [&](int tile) { return ((tile + lane / NG) * TT + 8 * (lane % NG)) >> p.page_log2; };
-        auto read_entries = [&](int tile) {
-            const int b = entry_of(tile);
-            return table[b < blocks ? b : blocks - 1];
-        };
-        auto pages_of = [&](int tile, int block) {
-            return tile + lane / NG < end && entry_of(tile) < blocks && uint32_t(block) < uint32_t(p.num_blocks) ? block : -1;
-        };
-        int pages = pages_of(tile0, read_entries(tile0)), next = read_entries(tile0 + kAhead), asked = 0;      // asked: the number in `pages` of the tile asked for next
+        int pages = pages_of(tile0, first_entries), next = read_entries(tile0 + kAhead), asked = 0;      // asked: the number in `pages` of the tile asked for next
         constexpr int NW = F8 ? 2 : 4;                     // words of eight coordinates
         struct Part {
             uint32_t word[8][NW];
@@ -560,11 +567,14 @@ int launch_prefix(const fq::PrefixParams& pp, const PrefixPlan& plan, hipStream_
     const int st = plan.own.heads == 4 ? launch_attend_prefix<D, DT, F8, 4>(pp, plan, s)
                    : plan.own.heads == 2 ? launch_attend_prefix<D, DT, F8, 2>(pp, plan, s) : launch_attend_prefix<D, DT, F8, 1>(pp, plan, s);
     if (st != FQ_OK) return st;
-    const int64_t values = int64_t(pp.kv.S) * pp.kv.H_KV * pp.kv.G * D;
-    if (pp.kv.G * D % 256 == 0 && values / 256 >= 2 * fq_host::device_cu_count())
-        fq::paged_prefix_join_kernel<D, DT, PT, 64><<<unsigned(values / 256), 256, 0, s>>>(pp);
-    else
-        fq::paged_prefix_join_kernel<D, DT, PT, 16><<<unsigned(values / 64), 256, 0, s>>>(pp);
+    // As many values a workgroup as leave enough workgroups: then a thread has its values' pieces to itself, and the trips to memory that every
+    // workgroup begins with are fewer
+    const int64_t values = int64_t(pp.kv.S) * pp.kv.H_KV * pp.kv.G * D, enough = 2 * int64_t(fq_host::device_cu_count());
+    auto fits = [&](int per) { return pp.kv.G * D % per == 0 && values / per >= enough; };
+    if (fits(1024)) fq::paged_prefix_join_kernel<D, DT, PT, 256><<<unsigned(values / 1024), 256, 0, s>>>(pp);
+    else if (fits(512)) fq::paged_prefix_join_kernel<D, DT, PT, 128><<<unsigned(values / 512), 256, 0, s>>>(pp);
+    else if (fits(256)) fq::paged_prefix_join_kernel<D, DT, PT, 64><<<unsigned(values / 256), 256, 0, s>>>(pp);
+    else fq::paged_prefix_join_kernel<D, DT, PT, 16><<<unsigned(values / 64), 256, 0, s>>>(pp);
     return fq_host::check_launch();
 }
 
