@@ -1,4 +1,4 @@
-// Attention of one new token per sequence over a paged cache of 16-bit keys and values.
+// Attention of one new token per sequence over a paged cache of 16-bit keys and values, or of 8-bit rows.
 //
 //   o_h = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q_h . k_j - m),  c = sm_scale log2(e),  m = max_j c q_h . k_j
 //
@@ -28,6 +28,15 @@
 //     weights.
 // Measured: 32 sequences of 4096 tokens, 32 heads over 8 of 128, bf16, 84 us (6.4 TB/s); 61 of 500 to 16000, 64 over 8, fp16, 343 us
 // (6.6 TB/s); 3 of 40000 to 65536, 8 heads over 1, 21 us; one of 777, 32 over 8, 9.2 us.
+//
+// The same kernel reads rows of 8-bit codes with a power of two each (F8; half the bytes).  Codes are multiplied as they are, exact in
+// either 16-bit type, and the powers applied in float32: a key's to its score, a value's to its weight, whose two terms are then
+// bfloat16, which has their range.  What changes of the layout: a lane's 16 bytes of a key are two operands' eights, of the query as well; a line is
+// a key of 128 or half of one of 256 (of 64 codes it is two heads, and loads stay in the cache for the other's wavefront); values are
+// turned a byte at a time, two keys' words into pairs of one coordinate's codes, a quarter of a v_perm_b32 an element, then converted.
+// Powers lie by page and head, so that those of eight tokens are one load.  Two tiles on their way instead of one brought nothing
+// (32 x 4096 49.7 -> 50.6 us): the bytes in flight suffice.  Measured: 32 x 4096, 32 over 8 of 128, bf16, 49.6 us (5.5 TB/s); 57 of 400 to
+// 15000, 64 over 8, fp16, 162 us (6.1 TB/s); 1 x 900 10.1 us.
 #pragma once
 
 #include <type_traits>

@@ -4,7 +4,28 @@
 //
 //   o = (sum_{j in prefix} p_j v_j + sum_{j behind} p_j v_j) / (sum_{j in prefix} p_j + sum_{j behind} p_j)
 //
-// Members of prefix i are the sequences whose id it is and that are as long as it; no lists of them are asked for.
+// Members of prefix i are the sequences whose id it is and that are as long as it; no lists of them are asked for, and nothing on the
+// host knows a length: every workgroup counts members and tiles for itself, with all lengths and ids asked for at once.
+//
+// What bounds it: the own tokens HBM, the prefix the LDS.  One launch has workgroups of both, one of each on a CU, so that the ones' waits
+// for memory and the others' products overlap (apart, 96 sequences of 50 to 1200 tokens behind 6000: 37 + 44 us, together 52); a
+// second launch joins.
+//   * 128 rows (member, query head of the KV head), 32 a wavefront, against tiles of 16 KB of keys and as many of values in LDS,
+//     double buffered, one barrier a tile.  S^T = K Q^T and O^T = V^T P on v_mfma_f32_32x32x16, rows along the columns: a lane's
+//     scores are its own P operand, maximum and sum of a row two lanes' own.
+//   * Every thread brings eight coordinates of eight tokens through registers, asked for a tile ahead: half of the threads keys, as they are,
+//     16-byte pieces swizzled so that lanes reading one piece of 16 keys reach all banks; half of them values, turned (half a v_perm_b32 an
+//     element) into operands.  Codes become 16-bit on the way.
+//   * An operand from LDS serves one product of 32 rows: 128 KB a tile at 144 bytes a ns and CU are 0.9 us, the products 0.75, and
+//     a tile takes 1.4 to 1.8 on one workgroup a CU (2.4 beside one of own tokens), 1.07 of two.  64 rows a wavefront would halve that
+//     but need more registers than two workgroups leave; scores of the next tile under the weights of this one as well (300 spilled).
+//     Weights of 16 tokens run under the products of the 16 before them, whose values are read before that (with this 31.2 -> 28.0 us at 40
+//     sequences behind 32768 tokens).
+//   * Weights go to the second product as one 16-bit term: one more rounding of 2^-9 (fp16: 2^-12) of a weight, about what the result's own
+//     rounding is; the sums are of the unrounded ones.  Two terms, as the decode has them, would cost half of the products again.
+// Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 63 us (every sequence by
+// itself 330); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 70 us; 40 behind 32768, 8 over
+// 1, 8 bits, 28 us; 6 behind 2000 14.4 us.
 #include "fq_paged_kv_decode.hpp"
 
 namespace fq {
@@ -24,7 +45,6 @@ constexpr int kPrefixSeqs = 1024;         // sequences whose prefixes are kept i
 template <int D> struct PrefixCfg {
     static constexpr int TT = 8192 / D;                    // tokens of a tile
     static constexpr int NB = TT / 32, NKS = D / 16, NOB = D / 32, NU = TT / 16, NG = TT / 8;
-    template <bool F8> static constexpr int depth() { return F8 ? 2 : 1; }   // tiles that are on their way
     static constexpr int SIDE = TT * D * 2;                // bytes of a tile's keys or values: 16 KB
     static constexpr int LDS = 4 * SIDE + 2 * 3 * (TT / 4) * 4 + kPrefixRows * 4 + 3 * kPrefixMost * 4 + kPrefixSeqs * 2;
 };
@@ -49,7 +69,6 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
     using Elem = std::conditional_t<F8, uint8_t, uint16_t>;
     constexpr int TT = C::TT, NB = C::NB, NKS = C::NKS, NOB = C::NOB, NU = C::NU, NG = C::NG;
     constexpr bool POWERS = F8 && DT == FQ_F16;            // fp16 has no room for the powers of the rows: see below
-    constexpr int kDepth = C::template depth<F8>();
     const KvDecodeParams& p = pp.kv;
     uint8_t *lk = lds, *lv = lds + 2 * C::SIDE;
     float* powers = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, 3, TT / 4), see keep()
@@ -202,8 +221,8 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
             uint32_t scales[2];
             uint32_t there;                                // which eights of the tile are in the cache
         };
-        Part parts[kDepth];
-        auto load = [&](Part& part, int tile) __attribute__((always_inline)) {      // (no branch round the loads, so that nothing waits for them here)
+        Part part;
+        auto load = [&](int tile) __attribute__((always_inline)) {      // (no branch round the loads, so that nothing waits for them here)
             part.there = uint32_t(__ballot(pages >= 0) >> (NG * asked)) & ((1u << NG) - 1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -233,7 +252,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
         // power relative to the highest, E, of four neighbouring tokens (exact within 2^15 of it), and what is left, 2^E, is applied in
         // float32: to the scores (keys) and to the weights (values), where it is added to the score before the reference is chosen
         // and taken out of the sum of weights again.
-        auto keep = [&](const Part& part, int buffer) __attribute__((always_inline)) {
+        auto keep = [&](int buffer) __attribute__((always_inline)) {
             uint32_t word[8][4];
             int power[2] = {0, 0};
             if constexpr (F8) {
@@ -323,13 +342,11 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
 #pragma unroll
         for (int o = 0; o < 2; ++o) vread[o] = lv + 512 * hf + 16 * ((cr & 24) + ((cr & 7) ^ (4 * o + (cr >> 3))));
 
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) load(parts[d], tile0 + d);
-        int buffer = 0;
-        auto step = [&](int tile, Part& part) __attribute__((always_inline)) {
+        load(tile0);
+        for (int tile = tile0, buffer = 0; tile < end; ++tile, buffer ^= 1) {
             const uint32_t there = part.there;
-            keep(part, buffer);
-            load(part, tile + kDepth);                     // (of tiles behind the last: some page's, not used)
+            keep(buffer);
+            load(tile + 1);                                // (of the tile behind the last: some page's, not used)
             __syncthreads();
             if (live) {
                 float16v S[NB];
@@ -375,33 +392,44 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     m = higher;
                 }
                 const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<DT>;
+                // The weights of 16 tokens under the products of the 16 before them, whose values are read before that.
                 float sum = 0.0f;
-                uint4v P[NU];
-#pragma unroll
-                for (int u = 0; u < NU; ++u) {
+                uint4v P, V[2][NOB];
+                auto weights = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float sa = S[u / 2][8 * (u & 1) + 2 * i], sb = S[u / 2][8 * (u & 1) + 2 * i + 1];
                         const float a = __builtin_amdgcn_exp2f(POWERS ? sa - ref : __builtin_fmaf(sa, scale, -ref));
                         const float b = __builtin_amdgcn_exp2f(POWERS ? sb - ref : __builtin_fmaf(sb, scale, -ref));
-                        P[u][i] = round_pair<DT>(a, b);
+                        P[i] = round_pair<DT>(a, b);
                         if constexpr (POWERS) sum = __builtin_fmaf(a + b, table[NG + u / 2][2 * (u & 1) + i / 2], sum);
                         else sum += a + b;
                     }
+                };
+                auto read_values = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int ob = 0; ob < NOB; ++ob)
+                        V[u & 1][ob] = *reinterpret_cast<const uint4v*>(vread[ob & 1] + buffer * C::SIDE + (u * NOB + ob) * 1024);
+                };
+                read_values(0);
+                weights(0);
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (u + 1 < NU) read_values(u + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<DT>(V[u & 1][ob], P, O[ob]);
+                    if (u + 1 < NU) weights(u + 1);
 #pragma unroll
                     for (int ob = 0; ob < NOB; ++ob) {
-                        const uint4v v = *reinterpret_cast<const uint4v*>(vread[ob & 1] + buffer * C::SIDE + (u * NOB + ob) * 1024);
-                        O[ob] = wide_mfma<DT>(v, P[u], O[ob]);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x402, 28 / NOB, 0);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 l += sum;
             }
-            buffer ^= 1;
-        };
-        for (int tile = tile0; tile < end; tile += kDepth) {
-#pragma unroll
-            for (int d = 0; d < kDepth; ++d)
-                if (tile + d < end) step(tile + d, parts[d]);
         }
         l = sum_xor32(l);
         if (row < rows) {
@@ -618,7 +646,9 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
     const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes, int64_t(max_blocks_per_seq) * block_size);
     const PrefixRoom room = prefix_room(plan, num_seqs, H_Q, H_KV, D);
     // (units of work are counted in 32 bits)
-    if ((int64_t(num_seqs) / plan.members + num_prefixes) * (int64_t(max_blocks_per_seq) * block_size / (8192 / D) + 1) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    const int64_t max_tokens = int64_t(max_blocks_per_seq) * block_size;
+    if (int64_t(num_seqs) * ((max_tokens + fq::kKvTile - 1) / fq::kKvTile) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    if ((int64_t(num_seqs) / plan.members + num_prefixes) * (max_tokens / (8192 / D) + 1) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if (room.o / (size_t(D) * 4) * size_t(D / 32) > size_t(0x7fffffff)) return FQ_ERR_BAD_SHAPE;
     if (workspace_bytes < room.all) return FQ_ERR_WORKSPACE;
     if (!fq_host::aligned(workspace, 256)) return FQ_ERR_MISALIGNED;

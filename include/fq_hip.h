@@ -765,8 +765,9 @@ int fq_paged_kv8_decode(const void* q, const int64_t* q_strides, const uint8_t* 
  *                  is attended to by itself.  num_prefixes <= 1024
  *   workspace      fq_paged_prefix_decode_workspace_bytes bytes (does not shrink with num_seqs or num_prefixes), 256-byte aligned, any
  *                  contents
- * No window.  Weights over shared tokens keep 11 bits (fp16 pages), 8 (bf16) or, with scales, 8 and for fp16 queries 16; over a
- * sequence's own as in the decodes.  Maxima and sums are 32-bit.
+ * No window.  Weights over shared tokens are rounded to the type of q, over a sequence's own as in the decodes; maxima and sums are 32-bit.
+ * With scales and fp16 queries, shared values below 2^-31 count as 0 and shared rows lose what lies 2^-25 and more below the highest
+ * power of four neighbouring tokens.  num_seqs times the table's tokens is below 2^36.
  */
 size_t fq_paged_prefix_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int num_prefixes);
 int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
