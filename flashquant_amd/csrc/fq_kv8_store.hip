@@ -9,7 +9,7 @@
 //
 // What bounds it: each row is read and written once, so HBM does; for the few tokens of a decode step the launch and one trip to
 // memory do.  A row is 4, 8 or 16 neighbouring lanes of 16 values, the two eights of which lie apart as the pairs of a rotation do;
-// its maximum takes two to four DPP moves.  Angles as in fq_rotary.hip: one pair a thread, into LDS, for all heads of a token.
+// its maximum takes two to four DPP moves.  Angles: one pair a thread, into LDS, for all heads of a token.
 #include "fq_kv8.hpp"
 #include "fq_rotary.hpp"
 
@@ -43,11 +43,27 @@ struct Store8Params {
 __device__ __forceinline__ int64_t position_of(const Store8Params& p, int64_t token) {
     return p.wide_positions ? static_cast<const int64_t*>(p.positions)[token] : int64_t(static_cast<const int32_t*>(p.positions)[token]);
 }
+// scale times cos and sin of a pair's angle, rounded once: the nearest quarter turn is taken off exactly, then the Taylor series,
+// whose next terms are below 2^-36, all in 64 bits.  With both in 32 bits three times as many codes fell on the other side of a
+// rounding; a thread has at most four pairs, which costs nothing that could be measured.
 __device__ __forceinline__ float2v turn_of(const Store8Params& p, int64_t position, int pair) {
-    float2v cs = turn_cos_sin(double(position) * p.inv_freq[pair] * 0.15915494309189533576888);
-    cs.x *= p.scale;
-    cs.y *= p.scale;
-    return cs;
+    const double x = double(position) * p.inv_freq[pair] * 0.15915494309189533576888;
+    const double quarter = __builtin_rint(4.0 * x);
+    const double t = __builtin_fma(-0.25, quarter, x) * 6.283185307179586476925287, z = t * t;
+    double s = -1.0 / 39916800, c = 1.0 / 479001600;
+    s = __builtin_fma(z, s, 1.0 / 362880);
+    c = __builtin_fma(z, c, -1.0 / 3628800);
+    s = __builtin_fma(z, s, -1.0 / 5040);
+    c = __builtin_fma(z, c, 1.0 / 40320);
+    s = __builtin_fma(z, s, 1.0 / 120);
+    c = __builtin_fma(z, c, -1.0 / 720);
+    s = __builtin_fma(z, s, -1.0 / 6);
+    c = __builtin_fma(z, c, 1.0 / 24);
+    s = __builtin_fma(t * z, s, t);
+    c = __builtin_fma(z, __builtin_fma(z, c, -0.5), 1.0);
+    const int k = int(quarter - 4.0 * __builtin_floor(0.25 * quarter));      // 0 .. 3
+    const double a = (k & 1) ? s : c, b = (k & 1) ? c : s, scale = p.scale;
+    return float2v{float(scale * (k == 1 || k == 2 ? -a : a)), float(scale * (k >= 2 ? -b : b))};
 }
 
 // The power of a row whose largest finite magnitude is `most`: 2^-8 of its binade, and one more where it lies above 1.75 of it

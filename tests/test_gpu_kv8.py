@@ -114,8 +114,10 @@ def test_store(tokens, mapped, hq, hkv, d, rot, page, interleaved, layout, dtype
     before = [w.clone() for w in whole]
     got = K.rotary_paged_store8(q, k, v, positions, slots.to(DEV), freq, kc, vc, ks, vs, interleaved=interleaved, scale=0.9)
     assert got.shape == q.shape and got.dtype == dtype
-    if hq:                                                               # the queries of the 16-bit store
-        assert torch.equal(got, K.rotary_embedding(q, None, positions, freq, interleaved=interleaved, scale=0.9)[0])
+    if hq:                                                               # queries: half a step of their type
+        y, tol = turned(q, positions, freq, interleaved, 0.9)
+        info = torch.finfo(dtype)
+        assert ((got.double() - y).abs() <= tol + (y.abs() + tol) * info.eps / 2 + info.tiny * info.eps / 2).all()
     at = slots[stored].to(DEV)
     block, inside = at // page, at % page
     y, tol = turned(k, positions, freq, interleaved, 0.9)
