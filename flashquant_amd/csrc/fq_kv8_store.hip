@@ -10,6 +10,9 @@
 // What bounds it: each row is read and written once, so HBM does; for the few tokens of a decode step the launch and one trip to
 // memory do.  A row is 4, 8 or 16 neighbouring lanes of 16 values, the two eights of which lie apart as the pairs of a rotation do;
 // its maximum takes two to four DPP moves.  Angles: one pair a thread, into LDS, for all heads of a token.
+// Measured (whole calls): 48 tokens of 16 + 2 x 4 heads of 256 5.3 us; 9001 of 32 + 2 x 8 of 128 36 us, 203 MB, where a copy of as many bytes takes 39;
+// back to 16 bits, three sequences of up to 700 tokens 5.2 us, 44,000 tokens of 8 heads (275 MB, two thirds of them written) 67 us, and 61
+// into an output that is used again.
 #include "fq_kv8.hpp"
 #include "fq_rotary.hpp"
 

@@ -7,25 +7,25 @@
 // Members of prefix i are the sequences whose id it is and that are as long as it; no lists of them are asked for, and nothing on the
 // host knows a length: every workgroup counts members and tiles for itself, with all lengths and ids asked for at once.
 //
-// What bounds it: the own tokens HBM, the prefix the LDS.  One launch has workgroups of both, one of each on a CU, so that the ones' waits
-// for memory and the others' products overlap (apart, 96 sequences of 50 to 1200 tokens behind 6000: 37 + 44 us, together 52); a
-// second launch joins.
+// What bounds it: the own tokens HBM, the prefix each wavefront's chain of scores, maximum, weights and products.  One launch has
+// workgroups of both, one of each on a CU, so that the ones' waits for memory and the others' products overlap (96 sequences behind
+// 6000 tokens, whole calls: the prefix alone 35 us, 680 tokens each of their own 55, both 75); a second launch joins.
 //   * 128 rows (member, query head of the KV head), 32 a wavefront, against tiles of 16 KB of keys and as many of values in LDS,
 //     double buffered, one barrier a tile.  S^T = K Q^T and O^T = V^T P on v_mfma_f32_32x32x16, rows along the columns: a lane's
 //     scores are its own P operand, maximum and sum of a row two lanes' own.
 //   * Every thread brings eight coordinates of eight tokens through registers, asked for a tile ahead: half of the threads keys, as they are,
 //     16-byte pieces swizzled so that lanes reading one piece of 16 keys reach all banks; half of them values, turned (half a v_perm_b32 an
 //     element) into operands.  Codes become 16-bit on the way.
-//   * An operand from LDS serves one product of 32 rows: 128 KB a tile at 144 bytes a ns and CU are 0.9 us, the products 0.75, and
-//     a tile takes 1.4 to 1.8 on one workgroup a CU (2.4 beside one of own tokens), 1.07 of two.  64 rows a wavefront would halve that
-//     but need more registers than two workgroups leave; scores of the next tile under the weights of this one as well (300 spilled).
+//   * A tile takes 1.8 us on one workgroup a CU, 2.3 beside one of own tokens (256 sequences behind 8192 tokens: matrix cores busy 23 % of
+//     the cycles, LDS 19, vector units 36).  Two of the prefixes' on a CU took 4.3 for two tiles and a second prologue, which was
+//     no gain.  Scores of the next tile under the weights of this one need more registers than two workgroups leave (300 spilled).
 //     Weights of 16 tokens run under the products of the 16 before them, whose values are read before that (with this 31.2 -> 28.0 us at 40
 //     sequences behind 32768 tokens).
 //   * Weights go to the second product as one 16-bit term: one more rounding of 2^-9 (fp16: 2^-12) of a weight, about what the result's own
 //     rounding is; the sums are of the unrounded ones.  Two terms, as the decode has them, would cost half of the products again.
 // Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 63 us (every sequence by
-// itself 330); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 70 us; 40 behind 32768, 8 over
-// 1, 8 bits, 28 us; 6 behind 2000 14.4 us.
+// itself 301); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 69 us (224); 40 behind 32768,
+// 8 over 1, 8 bits, 28 us (60); 6 behind 2000 14.5 us (16).
 #include "fq_paged_kv_decode.hpp"
 
 namespace fq {
