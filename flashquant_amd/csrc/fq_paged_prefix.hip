@@ -17,7 +17,7 @@
 //     16-byte pieces swizzled so that lanes reading one piece of 16 keys reach all banks; half of them values, turned (half a v_perm_b32 an
 //     element) into operands.  Codes become 16-bit on the way.
 //   * A tile takes 1.8 us on one workgroup a CU, 2.3 beside one of own tokens (256 sequences behind 8192 tokens: matrix cores busy 23 % of
-//     the cycles, LDS 19, vector units 36).  Two of the prefixes' on a CU took 4.3 for two tiles and a second prologue, which was
+//     the cycles, LDS 19, vector units 32).  Two of the prefixes' on a CU took 4.3 for two tiles and a second prologue, which was
 //     no gain.  Scores of the next tile under the weights of this one need more registers than two workgroups leave (300 spilled).
 //     Weights of 16 tokens run under the products of the 16 before them, whose values are read before that (with this 31.2 -> 28.0 us at 40
 //     sequences behind 32768 tokens).
