@@ -101,7 +101,7 @@ class PageTable:
         self._share(seq, prefix)
 
     def join_prefix(self, seq: int, prefix: int) -> None:
-        """Sequence ``seq``, which has no tokens, begins with those of ``prefix``."""
+        """Sequence ``seq``, which has no tokens (their pages would be lost), begins with those of ``prefix``."""
         self._check(seq, prefix, made=True)
         self.block_table[seq] = self._prefix_table[prefix]
         self.context_lens[seq] = self.prefix_lens[prefix]
@@ -109,7 +109,7 @@ class PageTable:
 
     def drop_prefix(self, prefix: int) -> None:
         """Ends ``prefix``, which no sequence shares any more: its pages are free again."""
-        if not self._made[prefix]:
+        if not 0 <= prefix < len(self._made) or not self._made[prefix]:
             raise ValueError(f"prefix {prefix} is not in use")
         if prefix in self._prefix_of:
             raise ValueError(f"sequence {self._prefix_of.index(prefix)} still shares prefix {prefix}")

@@ -83,6 +83,17 @@ def test_refusals_of_prefixes():
         plain.make_prefix(0, 0)
 
 
+def test_a_prefix_that_does_not_exist_is_not_dropped():
+    """-1 is no prefix, whatever a list makes of it, and the last one keeps its pages."""
+    table = PageTable(20, 8, 1, 10, torch.device("cpu"), max_prefixes=2)
+    taken(table, 0, 16)
+    table.make_prefix(0, 1)
+    for prefix in (-1, -2, 2):
+        with pytest.raises(ValueError):
+            table.drop_prefix(prefix)
+    assert table.prefix_lens.tolist() == [0, 16] and int(table.free_start) == 2
+
+
 # ---- the C ABI ------------------------------------------------------------------------------------------------------------------
 
 def _p(v):
