@@ -122,7 +122,8 @@ __device__ __forceinline__ Store8Place place_of(const Store8Params& p, int64_t t
 }
 
 constexpr int kStore8Threads = 256;
-// angles of a workgroup's tokens: 16 rows of 256 coordinates reach into 7 tokens of three heads, 32 of 128 into 12, 64 of 64 into 23
+// angles of a workgroup's tokens: 16 rows of 256 coordinates reach into 8 tokens of two heads, 32 of 128 into 16, 64 of 64 into 32 (the
+// first row of each is a token's first), and into 7, 12 and 23 of three
 constexpr int kStore8Pairs = 1024;
 
 template <int D, int DT, bool INTERLEAVED, bool STREAM>

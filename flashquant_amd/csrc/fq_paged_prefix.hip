@@ -647,6 +647,7 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
     const PrefixRoom room = prefix_room(plan, num_seqs, H_Q, H_KV, D);
     // (units of work are counted in 32 bits)
     const int64_t max_tokens = int64_t(max_blocks_per_seq) * block_size;
+    if (max_tokens > 0x7fff0000LL) return FQ_ERR_BAD_SHAPE;          // tiles are asked for ahead
     if (int64_t(num_seqs) * ((max_tokens + fq::kKvTile - 1) / fq::kKvTile) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if ((int64_t(num_seqs) / plan.members + num_prefixes) * (max_tokens / (8192 / D) + 1) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if (room.o / (size_t(D) * 4) * size_t(D / 32) > size_t(0x7fffffff)) return FQ_ERR_BAD_SHAPE;

@@ -185,6 +185,8 @@ def test_prefix_status_codes(lib):
         assert status(**bad) == FQ_SHAPE, bad
     # more units of work than are counted
     assert status(S=1 << 20, mb=(1 << 27) - 4, P=1000, wb=1 << 62) == FQ_SHAPE
+    # tiles are asked for ahead, and their tokens are counted in 32 bits
+    assert status(S=1, mb=(1 << 27) - 4096, P=1, wb=0) == FQ_WS and status(S=1, mb=(1 << 27) - 4095, P=1, wb=0) == FQ_SHAPE
     for name in ("q", "qs", "kc", "kcs", "vc", "vcs", "table", "lens", "ids", "plens", "out", "ws"):
         assert status(**{name: _p(0)}) == FQ_NULL, name
     for name in eight:
