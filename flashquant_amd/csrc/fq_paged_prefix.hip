@@ -9,7 +9,7 @@
 //
 // What bounds it: the own tokens HBM, the prefix each wavefront's chain of scores, maximum, weights and products.  One launch has
 // workgroups of both, one of each on a CU, so that the ones' waits for memory and the others' products overlap (96 sequences behind
-// 6000 tokens, whole calls: the prefix alone 35 us, 680 tokens each of their own 55, both 75); a second launch joins.
+// 6000 tokens, whole calls: the prefix alone 35 us, 680 tokens each of their own 55, both 71); a second launch joins.
 //   * 128 rows (member, query head of the KV head), 32 a wavefront, against tiles of 16 KB of keys and as many of values in LDS,
 //     double buffered, one barrier a tile.  S^T = K Q^T and O^T = V^T P on v_mfma_f32_32x32x16, rows along the columns: a lane's
 //     scores are its own P operand, maximum and sum of a row two lanes' own.
@@ -23,8 +23,8 @@
 //     sequences behind 32768 tokens).
 //   * Weights go to the second product as one 16-bit term: one more rounding of 2^-9 (fp16: 2^-12) of a weight, about what the result's own
 //     rounding is; the sums are of the unrounded ones.  Two terms, as the decode has them, would cost half of the products again.
-// Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 63 us (every sequence by
-// itself 301); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 69 us (224); 40 behind 32768,
+// Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 61 us (every sequence by
+// itself 301); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 65 us (224); 40 behind 32768,
 // 8 over 1, 8 bits, 28 us (60); 6 behind 2000 14.5 us (16).
 #include "fq_paged_kv_decode.hpp"
 
@@ -126,26 +126,42 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
     __syncthreads();
     auto tiles_of = [&](int i) { return (shared_len[i] + TT - 1) / TT; };
     auto groups_of = [&](int i) { return int(uint32_t(count[i] + pp.members - 1) / uint32_t(pp.members)); };
-    auto units_of = [&](int i) { return i < p.num_prefixes ? tiles_of(i) * groups_of(i) : 0; };      // (the host bounds their sum)
-    uint32_t total = 0;
-    for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) total += wave_sum(uint32_t(units_of(i0 + lane)));
-    int size = int((total + uint32_t(pp.shares) - 1) / uint32_t(pp.shares));
+    // in tiles, or in shares of `each` tiles that end with their group of rows (the host bounds the sum of either)
+    auto units_of = [&](int i, int each) { return i < p.num_prefixes ? (tiles_of(i) + each - 1) / each * groups_of(i) : 0; };
+    auto sum_of = [&](int each) {
+        uint32_t sum = 0;
+        for (int i0 = 0; i0 < p.num_prefixes; i0 += kWave) sum += wave_sum(uint32_t(units_of(i0 + lane, each)));
+        return sum;
+    };
+    const uint32_t total = sum_of(1);
+    int size = int((total + uint32_t(pp.shares) - 1) / uint32_t(pp.shares)), each = 1;
     if (size < pp.min_tiles) size = pp.min_tiles;
-    if (int64_t(x) * size >= int64_t(total)) return;
-    const int wanted = x * size;
-    int left = int(total) - wanted < size ? int(total) - wanted : size;
+    // A share that goes on into another group takes as long as with four tiles more: better is one of up to three more, if all then end with
+    // their groups (150 sequences behind three prefixes, 8 bits, 72 -> 68 us; 128 of 50 tokens behind 4096, whose shares end so anyway,
+    // 31.2 -> 31.7: the sums).
+    uint32_t pieces = 0;
+    for (int n = size; each == 1 && n < size + 4; ++n) {
+        pieces = sum_of(n);
+        if (pieces <= uint32_t(pp.shares)) each = n;
+    }
+    if (each > 1) size = each;
+    const int64_t begin = each > 1 ? x : int64_t(x) * size;
+    if (begin >= int64_t(each > 1 ? pieces : total)) return;
+    const int wanted = int(begin);
+    int left = each > 1 || int(total) - wanted > size ? size : int(total) - wanted;
     int prefix = 0, group = 0, tile0 = 0, piece = x;       // piece: the share and the groups of rows before this one
     for (int i0 = 0, before = 0; i0 < p.num_prefixes; i0 += kWave) {
-        const int units = units_of(i0 + lane), gs = units > 0 ? groups_of(i0 + lane) : 0;
+        const int units = units_of(i0 + lane, each), gs = units > 0 ? groups_of(i0 + lane) : 0;
         const int upto = before + sum_upto(units), groups_upto = sum_upto(gs);
         const uint64_t past = __ballot(upto > wanted);
         if (past != 0) {
             const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
             prefix = i0 + at;
             const int inside = wanted - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(units, at));
-            const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(prefix));
-            group = inside / tiles;
-            tile0 = inside - group * tiles;
+            const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(prefix)), per = (tiles + each - 1) / each;
+            group = inside / per;
+            tile0 = (inside - group * per) * each;
+            if (each > 1 && left > tiles - tile0) left = tiles - tile0;
             piece += __builtin_amdgcn_readlane(groups_upto, at) - __builtin_amdgcn_readlane(gs, at) + group;
             break;
         }
@@ -648,7 +664,8 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
     // (units of work are counted in 32 bits)
     const int64_t max_tokens = int64_t(max_blocks_per_seq) * block_size;
     if (max_tokens > 0x7fff0000LL) return FQ_ERR_BAD_SHAPE;          // tiles are asked for ahead
-    if (int64_t(num_seqs) * ((max_tokens + fq::kKvTile - 1) / fq::kKvTile) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
+    const int between = plan.own.waves * (f8 ? 2 : 1);
+    if (int64_t(num_seqs) * ((max_tokens + fq::kKvTile - 1) / fq::kKvTile + between) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if ((int64_t(num_seqs) / plan.members + num_prefixes) * (max_tokens / (8192 / D) + 1) > 0x7fffffffLL) return FQ_ERR_BAD_SHAPE;
     if (room.o / (size_t(D) * 4) * size_t(D / 32) > size_t(0x7fffffff)) return FQ_ERR_BAD_SHAPE;
     if (workspace_bytes < room.all) return FQ_ERR_WORKSPACE;
@@ -663,6 +680,7 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
     p.part_l = reinterpret_cast<float*>(ws + room.o + room.m);
     p.place = reinterpret_cast<int2*>(ws + room.o + 2 * room.m);
     pp.place = reinterpret_cast<int4*>(ws + room.o + 2 * room.m + room.place);
+    p.between = between;
     p.prefix_ids = prefix_ids;
     p.prefix_lens = prefix_lens;
     p.num_prefixes = num_prefixes;

@@ -112,6 +112,24 @@ def test_groups_of_rows(members, hq, hkv, d, bits):
 
 
 @pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("hq,hkv", [(2, 1), (8, 8)])
+@pytest.mark.parametrize("own", [[1] * 40 + [0] * 660, [0, 0, 33, 0, 64, 0, 0, 0, 1, 0] * 70, [5000] + [0] * 598 + [3], [0] * 598 + [2, 900], [0] * 600])
+def test_shares_that_hold_little(own, hq, hkv, bits):
+    """Batches too large to be kept in registers with few tokens of their own: shares smaller than what a sequence counts for, shares without
+    a tile, one long sequence among many."""
+    ids = [(0, 1, -1)[s % 3] for s in range(len(own))]
+    check_prefix(*prefix_case([130, 700], ids, own, hq, hkv, 64, 16, BF, bits, seed=len(own) + hq))
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("members,tokens", [(17, [2048]), (100, [2112]), (48, [8192, 64, 1000]), (33, [64] * 5), (9, [16384])])
+def test_shares_and_groups_of_rows(members, tokens, bits):
+    """Prefixes whose tiles go evenly into shares, almost so, and not at all."""
+    ids = [s % len(tokens) for s in range(members)]
+    check_prefix(*prefix_case(tokens, ids, [s % 5 for s in range(members)], 32, 4, 128, 32, BF, bits, seed=members))
+
+
+@pytest.mark.parametrize("bits", BITS)
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_missing_pages_and_what_lies_beyond(d, bits):
     """Pages outside the cache in the prefix and behind it; NaN in all that is not seen, a prefix that ends inside a tile."""
