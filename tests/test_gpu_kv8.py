@@ -138,6 +138,13 @@ def test_store(tokens, mapped, hq, hkv, d, rot, page, interleaved, layout, dtype
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq", [0, 1])
+def test_store_of_the_fewest_heads(hq, d):
+    """A workgroup's rows reach into the most tokens, all of each turned."""
+    test_store(150, 150, hq, 1, d, d, 16, False, "apart", BF)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("off", [0, 1, 3])
 def test_store_has_the_same_bits_at_every_alignment(off, d):
     """Rows at odd addresses, columns apart, int32 positions: the kernel for any row gives what the wide one does."""
