@@ -21,8 +21,9 @@
 //     no gain.  Scores of the next tile under the weights of this one need more registers than two workgroups leave (300 spilled).
 //     Weights of 16 tokens run under the products of the 16 before them, whose values are read before that (with this 31.2 -> 28.0 us at 40
 //     sequences behind 32768 tokens).
-//   * Weights go to the second product as one 16-bit term: one more rounding of 2^-9 (fp16: 2^-12) of a weight, about what the result's own
-//     rounding is; the sums are of the unrounded ones.  Two terms, as the decode has them, would cost half of the products again.
+//   * Weights go to the second product as two 16-bit terms (16 significant bits and more), as over a sequence's own tokens; the sums are of
+//     the unrounded ones.  With one term a bf16 result was off by up to another 2^-8 of what was summed (0.0020 in the mean against 64
+//     bits, where its own rounding is 0.0017); the second costs 256 sequences behind 8192 tokens 69 -> 76 us, 96 behind 6000 61 -> 62.
 // Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 61 us (every sequence by
 // itself 301); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 65 us (224); 40 behind 32768,
 // 8 over 1, 8 bits, 28 us (60); 6 behind 2000 14.5 us (16).
@@ -410,7 +411,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                 const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<DT>;
                 // The weights of 16 tokens under the products of the 16 before them, whose values are read before that.
                 float sum = 0.0f;
-                uint4v P, V[2][NOB];
+                uint4v P, rest, V[2][NOB];                 // rest: what P's rounding left
                 auto weights = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -418,6 +419,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                         const float a = __builtin_amdgcn_exp2f(POWERS ? sa - ref : __builtin_fmaf(sa, scale, -ref));
                         const float b = __builtin_amdgcn_exp2f(POWERS ? sb - ref : __builtin_fmaf(sb, scale, -ref));
                         P[i] = round_pair<DT>(a, b);
+                        rest[i] = round_pair<DT>(a - low_value<DT>(P[i]), b - high_value<DT>(P[i]));
                         if constexpr (POWERS) sum = __builtin_fmaf(a + b, table[NG + u / 2][2 * (u & 1) + i / 2], sum);
                         else sum += a + b;
                     }
@@ -435,12 +437,14 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     if (u + 1 < NU) read_values(u + 1);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
+                    for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<DT>(V[u & 1][ob], rest, O[ob]);
+#pragma unroll
                     for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<DT>(V[u & 1][ob], P, O[ob]);
                     if (u + 1 < NU) weights(u + 1);
 #pragma unroll
-                    for (int ob = 0; ob < NOB; ++ob) {
+                    for (int i = 0; i < 2 * NOB; ++i) {
                         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x402, 28 / NOB, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x402, 24 / NOB, 0);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
