@@ -47,7 +47,7 @@ template <int D> struct PrefixCfg {
     static constexpr int TT = 8192 / D;                    // tokens of a tile
     static constexpr int NB = TT / 32, NKS = D / 16, NOB = D / 32, NU = TT / 16, NG = TT / 8;
     static constexpr int SIDE = TT * D * 2;                // bytes of a tile's keys or values: 16 KB
-    static constexpr int LDS = 4 * SIDE + 2 * 3 * (TT / 4) * 4 + kPrefixRows * 4 + 3 * kPrefixMost * 4 + kPrefixSeqs * 2;
+    static constexpr int LDS = 4 * SIDE + 2 * TT * 4 + kPrefixRows * 4 + 3 * kPrefixMost * 4 + kPrefixSeqs * 2;
 };
 
 // Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
@@ -69,11 +69,12 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
     using C = PrefixCfg<D>;
     using Elem = std::conditional_t<F8, uint8_t, uint16_t>;
     constexpr int TT = C::TT, NB = C::NB, NKS = C::NKS, NOB = C::NOB, NU = C::NU, NG = C::NG;
-    constexpr bool POWERS = F8 && DT == FQ_F16;            // fp16 has no room for the powers of the rows: see below
+    constexpr int PT = F8 ? FQ_BF16 : DT;                  // of weights and values in the second product
+    constexpr bool POWERS = F8 && DT == FQ_F16;            // fp16 has no room for the powers of the rows: see keep()
     const KvDecodeParams& p = pp.kv;
     uint8_t *lk = lds, *lv = lds + 2 * C::SIDE;
-    float* powers = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, 3, TT / 4), see keep()
-    int* list = reinterpret_cast<int*>(powers + 2 * 3 * (TT / 4));        // the sequences of the rows
+    float* powers = reinterpret_cast<float*>(lds + 4 * C::SIDE);          // (2, 2, TT / 2), see keep()
+    int* list = reinterpret_cast<int*>(powers + 2 * TT);                  // the sequences of the rows
     const int tid = threadIdx.x, lane = tid & 63, m32 = lane & 31, hf = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int head = workgroup % p.H_KV, x = workgroup / p.H_KV, G = p.G;
@@ -265,39 +266,39 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                 next = read_entries(tile + 1 + kAhead);
             }
         };
-        // Into LDS, as the products read them.  Codes become bfloat16 with the powers of their rows, exactly; to fp16 they go with their
-        // power relative to the highest, E, of four neighbouring tokens (exact within 2^15 of it), and what is left, 2^E, is applied in
-        // float32: to the scores (keys) and to the weights (values), where it is added to the score before the reference is chosen
-        // and taken out of the sum of weights again.
+        // Into LDS, as the products read them.  Codes become bfloat16 with the powers of their rows, exactly; keys that meet fp16 queries
+        // become fp16 without them, as exactly, and the powers are applied to the scores in float32.
         auto keep = [&](int buffer) __attribute__((always_inline)) {
             uint32_t word[8][4];
-            int power[2] = {0, 0};
             if constexpr (F8) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t bits = part.scales[h];
-                    float up[4] = {row_scale<0>(bits), row_scale<1>(bits), row_scale<2>(bits), row_scale<3>(bits)};
-                    if constexpr (POWERS) {
-                        float most = __builtin_fmaxf(__builtin_fmaxf(up[0], up[1]), __builtin_fmaxf(up[2], up[3]));
-                        // (values below 2^-31 are 0 in an fp16 result)
-                        if (brings_values) most = __builtin_fmaxf(most, 0x1p-40f);
-                        power[h] = int(float_to_bits(most) >> 23) - 127;
+                    const float up[4] = {row_scale<0>(bits), row_scale<1>(bits), row_scale<2>(bits), row_scale<3>(bits)};
+                    if (POWERS && !brings_values) {
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) up[t] = __builtin_ldexpf(up[t], -power[h]);
-                    }
+                        for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
+                            for (int i = 0; i < 2; ++i) {
+                                word[4 * h + t][2 * i] = codes_pair<DT, false>(part.word[4 * h + t][i]);
+                                word[4 * h + t][2 * i + 1] = codes_pair<DT, true>(part.word[4 * h + t][i]);
+                            }
+                        // tokens 8 i + 4 hf + 0 .. 3 at place (hf, i)
+                        if (ic == 0) {
+                            const int four = (h ? token1 : token0) / 4;
+                            *reinterpret_cast<float4v*>(powers + buffer * TT + 4 * ((four & 1) * NG + (four >> 1))) =
+                                float4v{p.scale_log2 * up[0], p.scale_log2 * up[1], p.scale_log2 * up[2], p.scale_log2 * up[3]};
+                        }
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t codes = part.word[4 * h + t][i];
-                            if constexpr (DT == FQ_BF16) {
+                        for (int t = 0; t < 4; ++t)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t codes = part.word[4 * h + t][i];
                                 word[4 * h + t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up[t], false));
                                 word[4 * h + t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up[t], true));
-                            } else {
-                                word[4 * h + t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, up[t], false));
-                                word[4 * h + t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, up[t], true));
                             }
-                        }
+                    }
                 }
             } else {
 #pragma unroll
@@ -326,22 +327,6 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                 for (int i = 0; i < 8; ++i) {
                     const int r = token0 + i;
                     *reinterpret_cast<uint4v*>(lk + buffer * C::SIDE + r * (2 * D) + 16 * (ic ^ key_swizzle<D>(r))) = uint4v{word[i][0], word[i][1], word[i][2], word[i][3]};
-                }
-            }
-            if constexpr (POWERS) {
-                // tables by four tokens, 8 i + 4 hf + 0 .. 3 at place (hf, i): of keys, of values, and of values inverted
-                if (ic == 0) {
-                    float* to = powers + buffer * 3 * (TT / 4);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int four = (h ? token1 : token0) / 4, at = (four & 1) * NG + (four >> 1);
-                        if (brings_values) {
-                            to[TT / 4 + at] = float(power[h]);
-                            to[TT / 2 + at] = __builtin_ldexpf(1.0f, -power[h]);
-                        } else {
-                            to[at] = __builtin_ldexpf(p.scale_log2, power[h]);
-                        }
-                    }
                 }
             }
         };
@@ -374,14 +359,16 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     for (int ks = 0; ks < NKS; ++ks)
                         S[b] = wide_mfma<DT>(*reinterpret_cast<const uint4v*>(kread + buffer * C::SIDE + b * (64 * D) + ((32 * ks) ^ kswizzle)), qb[ks], S[b]);
                 }
-                const float4v* table = reinterpret_cast<const float4v*>(powers + buffer * 3 * (TT / 4) + hf * NG);
                 if constexpr (POWERS) {
+                    const float4v* table = reinterpret_cast<const float4v*>(powers + buffer * TT + hf * (TT / 2));
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const float4v times = table[b], plus = table[NG / 2 + b];
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) S[b][e] = __builtin_fmaf(S[b][e], times[e / 4], plus[e / 4]);
-                    }
+                        for (int i = 0; i < 4; ++i) {
+                            const float4v times = table[4 * b + i];
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) S[b][4 * i + t] *= times[t];
+                        }
                 }
                 if (there != (1u << NG) - 1) {
 #pragma unroll
@@ -408,7 +395,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                         for (int e = 0; e < 16; ++e) O[ob][e] *= shrink;
                     m = higher;
                 }
-                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<DT>;
+                const float ref = m == -__builtin_inff() ? 0.0f : m - kKvLift<PT>;
                 // The weights of 16 tokens under the products of the 16 before them, whose values are read before that.
                 float sum = 0.0f;
                 uint4v P, rest, V[2][NOB];                 // rest: what P's rounding left
@@ -418,10 +405,9 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                         const float sa = S[u / 2][8 * (u & 1) + 2 * i], sb = S[u / 2][8 * (u & 1) + 2 * i + 1];
                         const float a = __builtin_amdgcn_exp2f(POWERS ? sa - ref : __builtin_fmaf(sa, scale, -ref));
                         const float b = __builtin_amdgcn_exp2f(POWERS ? sb - ref : __builtin_fmaf(sb, scale, -ref));
-                        P[i] = round_pair<DT>(a, b);
-                        rest[i] = round_pair<DT>(a - low_value<DT>(P[i]), b - high_value<DT>(P[i]));
-                        if constexpr (POWERS) sum = __builtin_fmaf(a + b, table[NG + u / 2][2 * (u & 1) + i / 2], sum);
-                        else sum += a + b;
+                        P[i] = round_pair<PT>(a, b);
+                        rest[i] = round_pair<PT>(a - low_value<PT>(P[i]), b - high_value<PT>(P[i]));
+                        sum += a + b;
                     }
                 };
                 auto read_values = [&](int u) __attribute__((always_inline)) {
@@ -437,9 +423,9 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     if (u + 1 < NU) read_values(u + 1);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<DT>(V[u & 1][ob], rest, O[ob]);
+                    for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<PT>(V[u & 1][ob], rest, O[ob]);
 #pragma unroll
-                    for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<DT>(V[u & 1][ob], P, O[ob]);
+                    for (int ob = 0; ob < NOB; ++ob) O[ob] = wide_mfma<PT>(V[u & 1][ob], P, O[ob]);
                     if (u + 1 < NU) weights(u + 1);
 #pragma unroll
                     for (int i = 0; i < 2 * NOB; ++i) {
@@ -461,7 +447,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                     *reinterpret_cast<float4v*>(p.part_o + at * D + 32 * ob + 16 * (e / 8) + 8 * hf + e % 8) =
                         float4v{O[ob][e], O[ob][e + 1], O[ob][e + 2], O[ob][e + 3]};
             if (hf == 0) {
-                p.part_m[at] = POWERS ? m + (kKvLift<FQ_BF16> - kKvLift<FQ_F16>) : m;      // (as the parts of the own tokens have it)
+                p.part_m[at] = m;
                 p.part_l[at] = l;
             }
         }

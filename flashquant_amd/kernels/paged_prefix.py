@@ -34,11 +34,10 @@ def paged_prefix_decode(
     tokens of a prefix, of which whole pages are shared.  The rows of ``block_table`` of a prefix's sequences begin with the same pages
     (one of them is read for all); ``seq_lens`` counts shared tokens, and a sequence shorter than its prefix is attended to by itself.
 
-    Weights have 16 significant bits, as there.  Over 8-bit pages with float16 queries, shared values below 2**-31 count as 0 and
-    rows that lie more than 2**15 below the highest of their four neighbours lose digits that no such result shows.
-    ``out`` and ``return_lse`` as in ``paged_kv_decode``; ``workspace``: at least ``_C.paged_prefix_decode_workspace_bytes(num_seqs, H_Q,
-    H_KV, head_dim, num_prefixes)`` bytes, enough for smaller batches too; it holds nothing from one call to the next, and calls that may run
-    at the same time need one each.  There is no window.  No gradient is recorded.  A sequence's last bits may depend on the others."""
+    Weights have 16 significant bits, as there, and 8-bit rows count as what they stand for.  ``out`` and ``return_lse`` as in
+    ``paged_kv_decode``; ``workspace``: at least ``_C.paged_prefix_decode_workspace_bytes(num_seqs, H_Q, H_KV, head_dim, num_prefixes)``
+    bytes, enough for smaller batches too; it holds nothing from one call to the next, and calls that may run at the same time need one
+    each.  There is no window.  No gradient is recorded.  A sequence's last bits may depend on the others."""
     require_gpu(q, "q")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])

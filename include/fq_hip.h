@@ -766,9 +766,7 @@ int fq_paged_kv8_decode(const void* q, const int64_t* q_strides, const uint8_t* 
  *   workspace      fq_paged_prefix_decode_workspace_bytes bytes (does not shrink with num_seqs or num_prefixes), 256-byte aligned, any
  *                  contents
  * No window.  Weights are rounded as in the decodes, to two 16-bit terms; maxima and sums are 32-bit.
- * With scales and fp16 queries, shared values below 2^-31 count as 0 and shared rows lose what lies 2^-25 and more below the highest
- * power of four neighbouring tokens.  num_seqs times the table's tokens is below 2^36, the
- * tokens of a row of the table at most 2^31 - 2^16.
+ * num_seqs times the table's tokens is below 2^36, the tokens of a row of the table at most 2^31 - 2^16.
  */
 size_t fq_paged_prefix_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int num_prefixes);
 int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
