@@ -23,4 +23,11 @@ template <int K> __device__ __forceinline__ float row_scale(uint32_t w) {
     else return bits_to_float((w << (23 - 8 * K)) & 0x7f800000u);
 }
 
+// The nearest number that the type holds.  A finite value near its end may have been rounded up to a code that stands for 2^16 (2^128):
+// it comes back as the largest of the type, not as an infinity, which no code stands for.  (NaN stays.)
+template <int DT> __device__ __forceinline__ float held(float x) {
+    constexpr float most = DT == FQ_BF16 ? 0x1.fep127f : 65504.0f;
+    return __builtin_fabsf(x) > most ? __builtin_copysignf(most, x) : x;
+}
+
 }  // namespace fq

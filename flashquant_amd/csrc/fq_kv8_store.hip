@@ -13,6 +13,8 @@
 // Measured (whole calls): 48 tokens of 16 + 2 x 4 heads of 256 5.3 us; 9001 of 32 + 2 x 8 of 128 36 us, 203 MB, where a copy of as many bytes takes 39;
 // back to 16 bits, three sequences of up to 700 tokens 5.2 us, 44,000 tokens of 8 heads (275 MB, two thirds of them written) 67 us, and 61
 // into an output that is used again.
+#include <type_traits>
+
 #include "fq_kv8.hpp"
 #include "fq_rotary.hpp"
 
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(kStore8Threads) void rotary_store8_any_kernel(const
     if (lane == 0) *at.scale = uint8_t(power + 127);
 }
 
-// Tokens back as 16-bit rows, code 2^E rounded to the type (bfloat16: exact but for its smallest numbers).  Reads a byte and writes
+// Tokens back as 16-bit rows, code 2^E rounded to the type (bfloat16: exact but for its smallest numbers), finite what is beyond it.  Reads a byte and writes
 // two, HBM-bound.  A thread has N pieces of 16 values, 256 pieces apart, and asks for all of them before it uses one; a piece is an
 // eight of each half of a row, so that a store of neighbouring threads takes whole lines (16 values in one place: 67 us for 60).
 // The sequence of a workgroup's first token is found by 64 lanes at a time, a later token's from there.
@@ -335,22 +337,34 @@ __global__ __launch_bounds__(256) void paged_kv8_read_kernel(const Read8Params p
             scale[k] = p.scales[v][int64_t(block[k]) * p.scale_block[v] + int64_t(head[k]) * p.scale_head[v] + in_page];
         }
     }
+    auto write = [&](auto ends) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        if (token[k] >= p.tokens || !(inside[k] || p.fill)) continue;
-        const float up = row_scale<0>(scale[k]);
-        uint32_t o[8];
+        for (int k = 0; k < N; ++k) {
+            if (token[k] >= p.tokens || !(inside[k] || p.fill)) continue;
+            const float up = row_scale<0>(scale[k]);
+            uint32_t o[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2v x = codes_f32<false>(w[k][i]) * up, y = codes_f32<true>(w[k][i]) * up;
-            o[2 * i] = rounded_words<DT>(x.x, x.y);
-            o[2 * i + 1] = rounded_words<DT>(y.x, y.y);
+            for (int i = 0; i < 4; ++i) {
+                float2v x = codes_f32<false>(w[k][i]) * up, y = codes_f32<true>(w[k][i]) * up;
+                if constexpr (decltype(ends)::value) {
+                    x = float2v{held<DT>(x.x), held<DT>(x.y)};
+                    y = float2v{held<DT>(y.x), held<DT>(y.y)};
+                }
+                o[2 * i] = rounded_words<DT>(x.x, x.y);
+                o[2 * i + 1] = rounded_words<DT>(y.x, y.y);
+            }
+            uint16_t* dst = p.out[side[k]] + (token[k] * p.H + head[k]) * D + c[k];
+            const uint4v lo = {o[0], o[1], o[2], o[3]}, hi = {o[4], o[5], o[6], o[7]};
+            *reinterpret_cast<uint4v*>(dst) = lo;
+            *reinterpret_cast<uint4v*>(dst + D / 2) = hi;
         }
-        uint16_t* dst = p.out[side[k]] + (token[k] * p.H + head[k]) * D + c[k];
-        const uint4v lo = {o[0], o[1], o[2], o[3]}, hi = {o[4], o[5], o[6], o[7]};
-        *reinterpret_cast<uint4v*>(dst) = lo;
-        *reinterpret_cast<uint4v*>(dst + D / 2) = hi;
-    }
+    };
+    // Rows that can hold what is beyond the type are few, and looked for (of every value, 41,000 tokens of 8 heads of 128 60 -> 66 us).
+    uint32_t highest = scale[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) highest = highest > scale[k] ? highest : scale[k];
+    if (__any(highest >= (DT == FQ_BF16 ? 127 + 120 : 127 + 8))) write(std::true_type{});
+    else write(std::false_type{});
 }
 
 }  // namespace fq

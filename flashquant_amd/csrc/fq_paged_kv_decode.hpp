@@ -255,6 +255,12 @@ __device__ __forceinline__ float scale_of(const uint2v& w, int k) {
     return (k & 3) == 0 ? row_scale<0>(word) : (k & 3) == 1 ? row_scale<1>(word) : (k & 3) == 2 ? row_scale<2>(word) : row_scale<3>(word);
 }
 
+// Four values of a result.  Over codes they are finite where the mean of what was stored is.
+template <int DT> __device__ __forceinline__ uint2v result_words(float4v o, bool f8) {
+    if (f8) o = float4v{held<DT>(o.x), held<DT>(o.y), held<DT>(o.z), held<DT>(o.w)};
+    return uint2v{round_pair<DT>(o.x, o.y), round_pair<DT>(o.z, o.w)};
+}
+
 // HW heads of a workgroup, TW wavefronts of each; SHARED: a share of all tiles, else one sequence.  F8: rows of codes.  OWN (with
 // SHARED): the tokens behind a shared prefix, left as partial results.
 template <int D, int DT, bool F8, int HW, int TW, bool SHARED, bool OWN>
@@ -581,8 +587,7 @@ __device__ __forceinline__ void kv_decode_workgroup(const KvDecodeParams& p, int
                         for (int e = 0; e < VE; e += 4) {
                             if (complete)
                                 *reinterpret_cast<uint2v*>(p.out + (orow + n) * D + c + e) =
-                                    uint2v{round_pair<DT>(acc[h][e][r] * inv, acc[h][e + 1][r] * inv),
-                                           round_pair<DT>(acc[h][e + 2][r] * inv, acc[h][e + 3][r] * inv)};
+                                    result_words<DT>(float4v{acc[h][e][r], acc[h][e + 1][r], acc[h][e + 2][r], acc[h][e + 3][r]} * inv, F8);
                             else
                                 *reinterpret_cast<float4v*>(p.part_o + (row + n) * D + c + e) =
                                     float4v{acc[h][e][r], acc[h][e + 1][r], acc[h][e + 2][r], acc[h][e + 3][r]};
@@ -637,7 +642,7 @@ __device__ __forceinline__ void kv_decode_workgroup(const KvDecodeParams& p, int
                 const float inv = scale[h / G * 16 + h % G];
                 const int64_t at = i - int64_t(mine) * G * D;        // from this wavefront's head on
                 if (complete)
-                    *reinterpret_cast<uint2v*>(p.out + orow * D + at) = uint2v{round_pair<DT>(o.x * inv, o.y * inv), round_pair<DT>(o.z * inv, o.w * inv)};
+                    *reinterpret_cast<uint2v*>(p.out + orow * D + at) = result_words<DT>(o * inv, F8);
                 else
                     *reinterpret_cast<float4v*>(p.part_o + row * D + at) = o;
             }
@@ -735,7 +740,7 @@ __global__ __launch_bounds__(256) void paged_kv_join_kernel(const KvDecodeParams
         for (int r = 0; r < R; ++r) all += rows[r][q];
         const float inv = inverse_sum(den);
         const int64_t out = group * p.G;
-        *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(all.x * inv, all.y * inv), round_pair<DT>(all.z * inv, all.w * inv)};
+        *reinterpret_cast<uint2v*>(p.out + out * D + c) = result_words<DT>(all * inv, p.ks != nullptr);
         if (c % D == 0 && p.lse != nullptr)
             p.lse[out + h] = den == 0.0f ? -__builtin_inff() : (highest - kKvLift<PT> + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
     }

@@ -230,7 +230,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                 for (int ks = 0; ks < NKS; ++ks) qb[ks] = p.scale_log2 == 0.0f ? uint4v{0u, 0u, 0u, 0u} : qb[ks] ^ 0x80008000u;
             }
         }
-        const float scale = p.scale_log2 == 0.0f ? 1.0f : __builtin_fabsf(p.scale_log2);
+        const float scale = p.scale_log2 == 0.0f ? 1.0f : (F8 ? 2.0f : 1.0f) * __builtin_fabsf(p.scale_log2);       // (codes: half keys)
 
         int pages = pages_of(tile0, first_entries), next = read_entries(tile0 + kAhead), asked = 0;      // asked: the number in `pages` of the tile asked for next
         constexpr int NW = F8 ? 2 : 4;                     // words of eight coordinates
@@ -266,8 +266,8 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
                 next = read_entries(tile + 1 + kAhead);
             }
         };
-        // Into LDS, as the products read them.  Codes become bfloat16 with the powers of their rows, exactly; keys that meet fp16 queries
-        // become fp16 without them, as exactly, and the powers are applied to the scores in float32.
+        // Into LDS, as the products read them.  Codes become bfloat16 with half the powers of their rows, exactly (half: a code may stand for
+        // 2^128); keys that meet fp16 queries become fp16 without them, as exactly, and the powers are applied to the scores in float32.
         auto keep = [&](int buffer) __attribute__((always_inline)) {
             uint32_t word[8][4];
             if constexpr (F8) {
@@ -295,8 +295,8 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 const uint32_t codes = part.word[4 * h + t][i];
-                                word[4 * h + t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up[t], false));
-                                word[4 * h + t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, up[t], true));
+                                word[4 * h + t][2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 0.5f * up[t], false));
+                                word[4 * h + t][2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 0.5f * up[t], true));
                             }
                     }
                 }
@@ -445,7 +445,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
                     *reinterpret_cast<float4v*>(p.part_o + at * D + 32 * ob + 16 * (e / 8) + 8 * hf + e % 8) =
-                        float4v{O[ob][e], O[ob][e + 1], O[ob][e + 2], O[ob][e + 3]};
+                        float4v{O[ob][e], O[ob][e + 1], O[ob][e + 2], O[ob][e + 3]} * (F8 ? 2.0f : 1.0f);
             if (hf == 0) {
                 p.part_m[at] = m;
                 p.part_l[at] = l;
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(256) void paged_prefix_join_kernel(const PrefixPara
         for (int r = 0; r < R; ++r) all += rows[r][q];
         const float inv = inverse_sum(den);
         const int64_t out = unit * p.G;
-        *reinterpret_cast<uint2v*>(p.out + out * D + c) = uint2v{round_pair<DT>(all.x * inv, all.y * inv), round_pair<DT>(all.z * inv, all.w * inv)};
+        *reinterpret_cast<uint2v*>(p.out + out * D + c) = result_words<DT>(all * inv, p.ks != nullptr);
         if (in_row == 0 && p.lse != nullptr)
             p.lse[out + h] = den == 0.0f ? -__builtin_inff() : (highest - kKvLift<PT> + __builtin_amdgcn_logf(den)) * (1.0f / kLog2e);
     }

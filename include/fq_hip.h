@@ -720,7 +720,8 @@ int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_
  *   below -118 (a row of zeros: that) or above 120; the codes are rounded to nearest even.  Infinite values become NaN.
  *   D in {64, 128, 256}.  Fastest where half is a multiple of 8 and rows lie at multiples of 16 bytes.
  *
- * fq_paged_kv8_read: tokens back as 16-bit rows, code * 2^(byte - 127) rounded to fp16 or bf16 (bf16: exact from 2^-126 on).
+ * fq_paged_kv8_read: tokens back as 16-bit rows, code * 2^(byte - 127) rounded to fp16 or bf16 (bf16: exact from 2^-126 on); what is
+ *   beyond the type's largest number comes back as that.
  *   cu_seqlens     (num_seqs + 1,) int32, not decreasing: sequence s gives tokens starts[s] (int32; NULL: 0) and on to rows
  *                  cu_seqlens[s] .. cu_seqlens[s + 1] of the outputs
  *   keys, values   (num_tokens, H_KV, D) out.  Rows of tokens that are not on a page of the cache, or before the sequence's first or
@@ -729,7 +730,7 @@ int fq_paged_kv_decode(const void* q, const int64_t* q_strides, const void* key_
  *   Codes 16-byte aligned with strides that are multiples of 16.
  *
  * fq_paged_kv8_decode: fq_paged_kv_decode over such a cache; q, out fp16 or bf16.  The codes are multiplied as they are and the powers
- *   applied in float32, so nothing is rounded that was not in the cache.  Scale bytes 1 to 254.  Codes aligned as above, scales 8
+ *   applied in float32, so nothing is rounded that was not in the cache.  There are no infinities in it, and none come out.  Scale bytes 1 to 254.  Codes aligned as above, scales 8
  *   bytes with strides that are multiples of 8.  Workspace as there.
  */
 int fq_rotary_paged_store8(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int H_Q, const void* k,
