@@ -8,7 +8,7 @@ that it can be captured in a graph."""
 from __future__ import annotations
 
 import math
-from typing import List, NamedTuple, Optional, Tuple
+from typing import List, NamedTuple, Optional, Set, Tuple
 
 import torch
 
@@ -27,8 +27,9 @@ class PagedStep(NamedTuple):
 
     The tokens are packed: sequences that bring none have none, wherever they are in the table, and what is behind the last token is
     padding.  ``token_table`` (num_tokens, max_blocks) and ``token_lens`` (num_tokens,) int32 hold, token by token, the pages of its
-    sequence and how many tokens it sees (itself the last; padding: none); None where ``num_tokens`` is above ``max_seqs``.  Where the
-    table has prefixes, ``token_prefix`` (num_tokens,) int32 is the one of a token's sequence (or -1) and ``prefix_lens`` their tokens."""
+    sequence and how many tokens it sees (itself the last; padding: none); None where ``num_tokens`` is above ``max_seqs``.  Where enough
+    sequences share a prefix of the table, ``token_prefix`` (num_tokens,) int32 is the one of a token's sequence (or -1: it attends by
+    itself) and ``prefix_lens`` their tokens; else both are None."""
     slot_mapping: torch.Tensor
     positions: torch.Tensor
     seq_lens: torch.Tensor
@@ -51,7 +52,15 @@ def _rows(q: torch.Tensor, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]
 
 class PageTable:
     """Block tables, lengths and the list of free pages of ``max_seqs`` sequences, all on the GPU, and up to ``max_prefixes`` prefixes
-    that sequences share: whole pages that belong to the prefix and not to a sequence."""
+    that sequences share: whole pages that belong to the prefix and not to a sequence.
+
+    A prefix is attended to once for all where at least three sequences share it.  Whether any is, ``schedule`` decides on the host: a
+    graph captured before never attends so (its results are right), one captured after follows every prefix that comes and goes."""
+
+    # Sequences that share a prefix of 2000 tokens, 32 heads over 8 of 128 (us, shared / every one by itself): 16 prefixes of two at 16 bits
+    # 39 / 36, at 8 bits 37 / 26; 20 of three 49 / 82 and 47 / 49; 16 of four 40 / 56 and 38 / 40.  (Of 512 tokens 10 of three 18 / 12: the host
+    # does not know lengths; of 6000 at 16 bits 32 of two 154 / 235.)
+    _enough = 3
 
     def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_blocks_per_seq: int,
                  device: Optional[torch.device] = None, *, max_prefixes: int = 0) -> None:
@@ -68,12 +77,15 @@ class PageTable:
         self._pages = torch.arange(num_blocks + 1, **i32)
         self.free_blocks = self._pages[:num_blocks]
         self.free_start = torch.zeros(1, **i32)
-        # pages and tokens of the prefixes, the prefix of every sequence; on the host which sequences share one, and which there are
+        # pages and tokens of the prefixes, the prefix of every sequence, and where enough share it; on the host which sequences share one,
+        # which there are, and which enough share
         self.prefix_ids = torch.full((max_seqs,), -1, **i32)
+        self._shared_ids = torch.full((max_seqs,), -1, **i32)
         self.prefix_lens = torch.zeros(max_prefixes, **i32)
         self._prefix_table = torch.full((max_prefixes, max_blocks_per_seq), -1, **i32)
         self._prefix_of: List[int] = [-1] * max_seqs
         self._made: List[bool] = [False] * max_prefixes
+        self._shared: Set[int] = set()
 
     def schedule(self, query_lens: torch.Tensor, num_tokens: int) -> PagedStep:
         """Gives ``query_lens[s]`` (int32) new tokens of sequence s their pages, slots and positions and counts them into the
@@ -83,9 +95,9 @@ class PageTable:
                            free_start=self.free_start, capped=True)
         rows = num_tokens <= self.block_table.shape[0]
         state = s, self.context_lens, self.free_start, self.block_table, self.num_blocks, self.block_size, rows
-        if not any(self._made):
+        if not self._shared:
             return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, *native().paged_advance(*state))
-        token_table, token_lens, token_prefix = native().paged_advance_prefix(*state, self.prefix_ids)
+        token_table, token_lens, token_prefix = native().paged_advance_prefix(*state, self._shared_ids)
         return PagedStep(s.slot_mapping, s.positions, s.seq_lens, s.cu_seqlens, self.block_table, s.free_end, token_table, token_lens, token_prefix,
                          self.prefix_lens if rows else None)
 
@@ -127,8 +139,7 @@ class PageTable:
         mine = (row >= 0) & (column < held)
         if prefix >= 0:
             mine &= column >= self.prefix_lens[prefix] // self.block_size
-            self.prefix_ids[seq] = -1
-            self._prefix_of[seq] = -1
+            self._leave(seq, prefix)
         self._free(mine, row)
         self.block_table[seq] = -1
         self.context_lens[seq] = 0
@@ -144,6 +155,22 @@ class PageTable:
     def _share(self, seq: int, prefix: int) -> None:
         self.prefix_ids[seq] = prefix
         self._prefix_of[seq] = prefix
+        self._settle(prefix, seq)
+
+    def _leave(self, seq: int, prefix: int) -> None:
+        self.prefix_ids[seq] = -1
+        self._shared_ids[seq] = -1
+        self._prefix_of[seq] = -1
+        self._settle(prefix)
+
+    def _settle(self, prefix: int, joined: Optional[int] = None) -> None:
+        """After a change of its sequences: whether ``prefix`` is attended to once for them."""
+        members = [s for s, p in enumerate(self._prefix_of) if p == prefix]
+        before, now = prefix in self._shared, len(members) >= self._enough
+        changed = members if now != before else [joined] if now and joined is not None else []
+        for s in changed:
+            self._shared_ids[s] = prefix if now else -1
+        (self._shared.add if now else self._shared.discard)(prefix)
 
     def _free(self, mine: torch.Tensor, row: torch.Tensor) -> None:
         count = mine.sum(dtype=torch.int32)
