@@ -36,9 +36,6 @@ struct TileCfg {
     static constexpr int UNIT = 32 * D + 64;               // floats of a unit's piece: its rows, 32 maxima, 32 sums
 };
 
-// Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
-__device__ __forceinline__ int coord_of_row(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
-
 typedef uint4v uint4a __attribute__((aligned(4)));
 
 // Rows of a norm n are at most n * span * sqrt(D) long (`span`: the largest centroid).  Those of 2^14 and more are stored divided

@@ -111,6 +111,9 @@ __device__ __forceinline__ void build_byte_table(uint32_t* table, const float* _
     fill_byte_table(table, centroids[lane & 15], wave, waves, lane);
 }
 
+// Coordinate (of 32) in row r of a 32-row matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
+__device__ __forceinline__ int coord_of_row(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
+
 // Cross-lane helpers that stay in the VALU (no LDS round trip).
 template <int CTRL>
 __device__ __forceinline__ float dpp_mov(float v) {

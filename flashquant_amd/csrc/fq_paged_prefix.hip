@@ -50,9 +50,6 @@ template <int D> struct PrefixCfg {
     static constexpr int LDS = 4 * SIDE + 2 * TT * 4 + kPrefixRows * 4 + 3 * kPrefixMost * 4 + kPrefixSeqs * 2;
 };
 
-// Coordinate (of 32) in row r of a matrix operand: result register e of lane half h is then coordinate 16 (e / 8) + 8 h + e % 8.
-__device__ __forceinline__ int coord_of_row(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
-
 // Where a key's 16-byte pieces lie in its row of LDS, so that lanes that read one piece of 16 neighbouring keys reach all banks.
 template <int D> __device__ __forceinline__ int key_swizzle(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
 
