@@ -239,7 +239,8 @@ class PagedKV8Layer:
 
     def read(self, cu_seqlens: torch.Tensor, num_tokens: int, starts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys (rotated) and values of the table's sequences, (num_tokens, heads, head_dim) each: of sequence s its tokens from
-        ``starts[s]`` (0 without) on, to rows ``cu_seqlens[s]`` .. ``cu_seqlens[s + 1]``; what the attention of a prompt's next chunk takes."""
+        ``starts[s]`` (0 without) on, to rows ``cu_seqlens[s]`` .. ``cu_seqlens[s + 1]``, for a prompt's attention over 16-bit rows (which is
+        the caller's: what this package has takes packed ones)."""
         return paged_kv8_read(self.keys, self.values, self.key_scales, self.value_scales, self.table.block_table, cu_seqlens, num_tokens,
                               starts=starts, dtype=self.dtype)
 

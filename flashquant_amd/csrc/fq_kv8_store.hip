@@ -11,7 +11,7 @@
 // memory do.  A row is 4, 8 or 16 neighbouring lanes of 16 values, the two eights of which lie apart as the pairs of a rotation do;
 // its maximum takes two to four DPP moves.  Angles: one pair a thread, into LDS, for all heads of a token.
 // Measured (whole calls): 48 tokens of 16 + 2 x 4 heads of 256 5.3 us; 9001 of 32 + 2 x 8 of 128 36 us, 203 MB, where a copy of as many bytes takes 39;
-// back to 16 bits, three sequences of up to 700 tokens 5.2 us, 44,000 tokens of 8 heads (275 MB, two thirds of them written) 67 us, and 61
+// back to 16 bits, three sequences of up to 700 tokens 5.2 us, 44,000 tokens of 8 heads (275 MB, two thirds of them written) 68 us, and 61
 // into an output that is used again.
 #include <type_traits>
 
@@ -125,7 +125,7 @@ __device__ __forceinline__ Store8Place place_of(const Store8Params& p, int64_t t
 
 constexpr int kStore8Threads = 256;
 // angles of a workgroup's tokens: 16 rows of 256 coordinates reach into 8 tokens of two heads, 32 of 128 into 16, 64 of 64 into 32 (the
-// first row of each is a token's first), and into 7, 12 and 23 of three
+// first row of each is a token's first), and into 6, 12 and 22 of three
 constexpr int kStore8Pairs = 1024;
 
 template <int D, int DT, bool INTERLEAVED, bool STREAM>

@@ -35,8 +35,8 @@
 // a key of 128 or half of one of 256 (of 64 codes it is two heads, and loads stay in the cache for the other's wavefront); values are
 // turned a byte at a time, two keys' words into pairs of one coordinate's codes, a quarter of a v_perm_b32 an element, then converted.
 // Powers lie by page and head, so that those of eight tokens are one load.  Two tiles on their way instead of one brought nothing
-// (32 x 4096 49.7 -> 50.6 us): the bytes in flight suffice.  Measured: 32 x 4096, 32 over 8 of 128, bf16, 49.6 us (5.5 TB/s); 57 of 400 to
-// 15000, 64 over 8, fp16, 162 us (6.1 TB/s); 1 x 900 10.1 us.
+// (32 x 4096 49.7 -> 50.6 us): the bytes in flight suffice.  Measured: 32 x 4096, 32 over 8 of 128, bf16, 49.8 us (5.4 TB/s); 57 of 400 to
+// 15000, 64 over 8, fp16, 162 us (6.1 TB/s), 16 over 4 of 256, bf16, 143 us (6.2); 32 x 4096, 32 over 8 of 64 40 us (3.4); 1 x 900 9.6 us.
 #pragma once
 
 #include <type_traits>
@@ -49,7 +49,7 @@ namespace fq {
 constexpr int kKvTile = 32;               // keys of a wavefront's step
 // Weights are kept times 2^lift.  fp16: up, so that their second terms stay normal.  bf16 has the exponents of float32, and a value may
 // lie near 2^128: down, so that no wavefront's sum of up to 2^20 such values overflows where their average does not (what underflows
-// instead are products below 2^-106).
+// instead are products below 2^-106; over codes, whose power is the weight's, below 2^-97).
 template <int DT> constexpr float kKvLift = DT == FQ_F16 ? 10.0f : -20.0f;
 
 struct KvDecodeParams {
@@ -243,8 +243,9 @@ template <int DT> __device__ __forceinline__ float high_value(uint32_t w) {
     if constexpr (DT == FQ_BF16) return bits_to_float(w & 0xffff0000u);
     else return f16_to_float(uint16_t(w >> 16));
 }
-// A row of 64 codes is half a line, whose other half, the next head's, another wavefront asks for: that one has to find it in the
-// cache (16 x 2000 tokens, 32 heads over 8 of 64: 15.2 us, 21.4 past it).
+// A row of 64 codes is half a line, whose other half, the next head's, another wavefront asks for: of this workgroup, if it has several
+// heads, and that one has to find it in the cache (16 x 2000 tokens, 32 heads over 8 of 64: 15.2 us, 21.4 past it); else of the next
+// workgroup, which is on another XCD and fetches the line again (20 sequences that see 1500 tokens: 57.8 MB for 27.5).
 template <bool PAST, typename T> __device__ __forceinline__ T kv_load(const T* p) {
     if constexpr (PAST) return __builtin_nontemporal_load(p);
     else return *p;
@@ -774,6 +775,7 @@ struct KvPlan {
 // The workgroup: four heads and two wavefronts of each draw best where there is much (see above); where a call has at most two
 // tiles for every wavefront of the card, two heads of two, of which a CU has two, spread it further: 1 x 1000 12.2 -> 10.1 us,
 // 1 x 4000 13.6 -> 12.0, 8 heads over 1, 4 x 1500 14.6 -> 12.6; but 61 of 500 to 16000 343 -> 355.
+// Rows of codes are divided alike; these crossings are of 16-bit rows.
 // tables of so many tiles are never divided
 int kv_whole_tiles(int D) { return D == 256 ? 10 : D == 128 ? 14 : 24; }
 KvPlan kv_plan(int S, int H_KV, int D, int64_t max_tokens, int window) {

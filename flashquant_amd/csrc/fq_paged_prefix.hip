@@ -8,25 +8,30 @@
 // host knows a length: every workgroup counts members and tiles for itself, with all lengths and ids asked for at once.
 //
 // What bounds it: the own tokens HBM, the prefix each wavefront's chain of scores, maximum, weights and products.  One launch has
-// workgroups of both, one of each on a CU, so that the ones' waits for memory and the others' products overlap (96 sequences behind
-// 6000 tokens, whole calls: the prefix alone 35 us, 680 tokens each of their own 55, both 71); a second launch joins.
+// workgroups of both, and a second one joins.  At D 64 and 128 a CU has one of each, so that the ones' waits for memory and the others'
+// products overlap (96 sequences behind 6000 tokens, 128, whole calls: the prefix alone 33 us, 50 to 1200 tokens each of their own 48,
+// both 63).  At 256 a wavefront has 447 to 457 registers and a CU one workgroup: the prefixes', which come first, and then the others
+// (47, 50, both 92).
 //   * 128 rows (member, query head of the KV head), 32 a wavefront, against tiles of 16 KB of keys and as many of values in LDS,
 //     double buffered, one barrier a tile.  S^T = K Q^T and O^T = V^T P on v_mfma_f32_32x32x16, rows along the columns: a lane's
 //     scores are its own P operand, maximum and sum of a row two lanes' own.
 //   * Every thread brings eight coordinates of eight tokens through registers, asked for a tile ahead: half of the threads keys, as they are,
 //     16-byte pieces swizzled so that lanes reading one piece of 16 keys reach all banks; half of them values, turned (half a v_perm_b32 an
 //     element) into operands.  Codes become 16-bit on the way.
-//   * A tile takes 1.8 us on one workgroup a CU, 2.3 beside one of own tokens (256 sequences behind 8192 tokens: matrix cores busy 23 % of
-//     the cycles, LDS 19, vector units 32).  Two of the prefixes' on a CU took 4.3 for two tiles and a second prologue, which was
-//     no gain.  Scores of the next tile under the weights of this one need more registers than two workgroups leave (300 spilled).
-//     Weights of 16 tokens run under the products of the 16 before them, whose values are read before that (with this 31.2 -> 28.0 us at 40
-//     sequences behind 32768 tokens).
+//   * A tile takes 1.6 us on one workgroup a CU, fp16 over codes 1.8 (256 sequences behind 8192 and 16384 tokens; matrix cores busy 29 % of
+//     the cycles, LDS 16, vector units 34).  Two of the prefixes' on a CU were no gain (with one term of a weight, see below, 4.3 us for two
+//     tiles where one took 1.8, and a second prologue).  Scores of the next tile under the weights of this one need more registers than
+//     two workgroups leave (300 spilled; as it is, at 128, 4 or 5 of 256).  Weights of 16 tokens run under the products of the 16 before
+//     them, whose values are read before that (with this 31.2 -> 28.0 us at 40 sequences behind 32768 tokens).
 //   * Weights go to the second product as two 16-bit terms (16 significant bits and more), as over a sequence's own tokens; the sums are of
 //     the unrounded ones.  With one term a bf16 result was off by up to another 2^-8 of what was summed (0.0020 in the mean against 64
 //     bits, where its own rounding is 0.0017); the second costs 256 sequences behind 8192 tokens 69 -> 76 us, 96 behind 6000 61 -> 62.
-// Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 61 us (every sequence by
-// itself 301); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 65 us (224); 40 behind 32768,
-// 8 over 1, 8 bits, 28 us (60); 6 behind 2000 14.5 us (16).
+// Measured (whole calls): 96 sequences of 50 to 1200 tokens behind 6000, 32 heads over 8 of 128, bf16, 63 us (every sequence by
+// itself 298); 150 of up to 900 behind three prefixes of 2848 to 5728 or none, 64 over 8, fp16 over 8 bits, 72 us (219); 40 behind 32768,
+// 8 over 1, 8 bits, 29 us (59); 6 behind 2000 15 us (16); 64 of up to 600 behind two of 3000 to 4000, 32 over 8 of 64, 22 us (69), 8 bits
+// 21 (41); 40 of them behind two of 2000 to 3000, 16 over 4 of 256, 36 us (71), 8 bits 34 (42).  It does not pay where sequences have
+// much more of their own than they share: 50 of 8000 behind 2000 287 us (285), 8 bits 167 (155); nor for one or two a prefix, as a tile
+// takes as long for four rows as for 128.
 #include "fq_paged_kv_decode.hpp"
 
 namespace fq {
@@ -463,7 +468,7 @@ __device__ __forceinline__ void prefix_workgroup(const PrefixParams& pp, int wor
 }
 
 // The first workgroups take the prefixes, the others what the sequences have behind them: those wait for the matrix cores, these for
-// memory, so a CU has one of each.
+// memory, so a CU has one of each (of 256 coordinates: one).
 template <int D, int DT, bool F8, int HW>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefix_kernel(const PrefixParams pp) {
     extern __shared__ __attribute__((aligned(256))) uint8_t prefix_lds[];
@@ -550,7 +555,7 @@ struct PrefixPlan {
     int shares, min_tiles, members, most_pieces;
     int most_own;            // shares of the own tokens in any table
 };
-PrefixPlan prefix_plan(int S, int H_KV, int G, int D, int num_prefixes, int64_t max_tokens) {
+PrefixPlan prefix_plan(int S, int H_KV, int G, int num_prefixes, int64_t max_tokens) {
     const int64_t cus = fq_host::device_cu_count();
     PrefixPlan r;
     const int together = H_KV % 4 == 0 ? 4 : H_KV % 2 == 0 ? 2 : 1;
@@ -619,7 +624,7 @@ int launch_prefix_type(const fq::PrefixParams& pp, const PrefixPlan& plan, bool 
 
 extern "C" size_t fq_paged_prefix_decode_workspace_bytes(int num_seqs, int H_Q, int H_KV, int D, int num_prefixes) {
     if (check_kv_shape(num_seqs, H_Q, H_KV, D, 16, 1, 1) != FQ_OK || num_seqs == 0 || num_prefixes < 0 || num_prefixes > fq::kPrefixMost) return 0;
-    return prefix_room(prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes, 0), num_seqs, H_Q, H_KV, D).all;
+    return prefix_room(prefix_plan(num_seqs, H_KV, H_Q / H_KV, num_prefixes, 0), num_seqs, H_Q, H_KV, D).all;
 }
 
 extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, const void* key_cache, const int64_t* key_strides,
@@ -646,7 +651,7 @@ extern "C" int fq_paged_prefix_decode(const void* q, const int64_t* q_strides, c
         (f8 && !(codes_aligned(key_cache, key_strides, key_scales, key_scale_strides) &&
                  codes_aligned(value_cache, value_strides, value_scales, value_scale_strides))))
         return FQ_ERR_MISALIGNED;
-    const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, D, num_prefixes, int64_t(max_blocks_per_seq) * block_size);
+    const PrefixPlan plan = prefix_plan(num_seqs, H_KV, H_Q / H_KV, num_prefixes, int64_t(max_blocks_per_seq) * block_size);
     const PrefixRoom room = prefix_room(plan, num_seqs, H_Q, H_KV, D);
     // (units of work are counted in 32 bits)
     const int64_t max_tokens = int64_t(max_blocks_per_seq) * block_size;
