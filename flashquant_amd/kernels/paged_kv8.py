@@ -61,9 +61,9 @@ def paged_kv8_read(
     (``block_table`` (num_seqs, max_blocks) int32) gives its tokens from ``starts[s]`` on (int32; 0 without) to rows ``cu_seqlens[s]`` ..
     ``cu_seqlens[s + 1]`` (int32, not decreasing, num_seqs + 1 of them); ``num_tokens`` is the room for all of them.
 
-    Values are exact in bfloat16 and rounded in float16; what is beyond the type's largest number comes back as that.  Rows of tokens on pages outside the cache (an
-    entry of -1), or beyond the table, are 0.  Rows behind the last sequence are 0; in ``out`` = (keys, values), contiguous, they are left
-    as they were.  No gradient is recorded."""
+    Values are exact in bfloat16 and rounded in float16; what is beyond the type's largest number comes back as that.  Rows of tokens on
+    pages outside the cache (an entry of -1), or beyond the table, are 0.  Rows behind the last sequence are 0; in ``out`` = (keys,
+    values), contiguous, they are left as they were.  No gradient is recorded."""
     require_gpu(key_cache, "key_cache")
     return native().paged_kv8_read(key_cache, value_cache, key_scales, value_scales, block_table, cu_seqlens, num_tokens, starts, dtype, out)
 
